@@ -1,0 +1,624 @@
+// Causal attention over packed documents for sm_100a: the plan of a packed buffer, and the forward pass.
+//
+//   o_i = sum_j p_ij v_j,  p_ij = exp(scale q_i.k_j) / sum,  over lo_i <= j <= i
+//
+// Documents lie one behind the other in a buffer of rows; lo_i is the first row of row i's document, or i - window + 1
+// where that is later.  Tiles are cut from the buffer, not from the documents: lo grows with i, so the keys that a query
+// tile sees are the tiles from its least lo to its own, whatever documents lie in it, and many short documents share one
+// tile.  Rows of no document get zeros.
+//
+// Roles (384 threads, one persistent block per SM): warps 0-3 and 4-7 softmax, one query tile of 128 rows each, a row per
+// thread; warp 8 issues the MMAs, warp 9 the copies.  The two query tiles share the key and value tiles: two heads of one
+// group on the same rows where the group is even (nothing is masked for one tile only), else the next 128 rows.
+// S and O live in tensor memory (2 x 128 + 2 x DP columns).  The probabilities go back over the scores they came from, as
+// bf16, and are the A operand of P V from there.  While one tile's softmax runs, the tensor cores do P V of the other
+// and its next scores.  O is brought to a new maximum only when a row's maximum has grown by 2^8: until then its
+// probabilities are at most 2^8 too large, and so is their sum.  Statistics and sums are fp32; probabilities are rounded
+// to bf16 once, as the operand of P V.
+#include "packed_attention.cuh"
+
+namespace slab {
+
+// ================================================================ plan
+__global__ void packed_bounds_kernel(const int* cu, int docs, int rows, int* base, int* status) {
+  const PackedPlan p = packed_plan(base, rows);
+  const int row = blockIdx.x * PA_TILE + threadIdx.x;
+  if (blockIdx.x == 0) {                         // offsets that fall, or pass the buffer's end, are reported
+    bool bad = threadIdx.x == 0 && (cu[0] != 0 || cu[docs] > rows);
+    for (int s = threadIdx.x; s < docs; s += PA_TILE) bad |= cu[s + 1] < cu[s];
+    if (bad) atomicCAS(status, 0, ST_BAD_INDEX);
+  }
+  int lo = row + 1, hi = row;
+  if (row < rows) {
+    int a = 0, b = docs;                         // documents that end at or before this row
+    while (a < b) {
+      const int mid = (a + b) >> 1;
+      if (cu[mid + 1] <= row) a = mid + 1; else b = mid;
+    }
+    if (a < docs && cu[a] <= row) {
+      lo = max(cu[a], 0);
+      hi = min(cu[a + 1], rows);
+    }
+    const_cast<int*>(p.doc_lo)[row] = lo;
+    const_cast<int*>(p.doc_hi)[row] = hi;
+  }
+  int least = lo <= row ? lo : PA_NONE, most = lo <= row ? hi : 0;
+  least = __reduce_min_sync(0xffffffffu, least);
+  most = __reduce_max_sync(0xffffffffu, most);
+  __shared__ int l[4], m[4];
+  if ((threadIdx.x & 31) == 0) { l[threadIdx.x >> 5] = least; m[threadIdx.x >> 5] = most; }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const_cast<int*>(p.tile_lo)[blockIdx.x] = min(min(l[0], l[1]), min(l[2], l[3]));
+    const_cast<int*>(p.tile_hi)[blockIdx.x] = max(max(m[0], m[1]), max(m[2], m[3]));
+  }
+}
+
+// Documents of token rows [batch][seq]: one starts with every row of the batch and behind every end-of-document token.
+// starts[2 t], starts[2 t + 1]: last and first start among the tile's positions (-1, PA_NONE: none).
+__device__ __forceinline__ bool pa_starts(const long long* tokens, int i, int seq, long long end) {
+  return i % seq == 0 || tokens[i - 1] == end;
+}
+__global__ void packed_starts_kernel(const long long* tokens, int rows, int seq, long long end, int* starts) {
+  const int row = blockIdx.x * PA_TILE + threadIdx.x;
+  const bool s = row < rows && pa_starts(tokens, row, seq, end);
+  const int last = __reduce_max_sync(0xffffffffu, s ? row : -1), first = __reduce_min_sync(0xffffffffu, s ? row : PA_NONE);
+  __shared__ int l[4], m[4];
+  if ((threadIdx.x & 31) == 0) { l[threadIdx.x >> 5] = last; m[threadIdx.x >> 5] = first; }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    starts[2 * blockIdx.x] = max(max(l[0], l[1]), max(l[2], l[3]));
+    starts[2 * blockIdx.x + 1] = min(min(m[0], m[1]), min(m[2], m[3]));
+  }
+}
+__global__ void packed_token_bounds_kernel(const long long* tokens, int rows, int seq, long long end, const int* starts, int* base) {
+  const PackedPlan p = packed_plan(base, rows);
+  const int row = blockIdx.x * PA_TILE + threadIdx.x;
+  __shared__ int before, behind;
+  __shared__ uint32_t mask[4];
+  if (threadIdx.x == 0) { before = 0; behind = rows; }
+  __syncthreads();
+  int lo = 0, hi = rows;
+  for (int u = threadIdx.x; u < (int)gridDim.x; u += PA_TILE) {
+    if (u < (int)blockIdx.x) lo = max(lo, starts[2 * u]);
+    if (u > (int)blockIdx.x) hi = min(hi, starts[2 * u + 1]);
+  }
+  atomicMax(&before, lo);
+  atomicMin(&behind, hi);
+  const uint32_t bits = __ballot_sync(0xffffffffu, row < rows && pa_starts(tokens, row, seq, end));
+  if ((threadIdx.x & 31) == 0) mask[threadIdx.x >> 5] = bits;
+  __syncthreads();
+  // last start at or before this row, first one behind it
+  lo = before;
+  hi = behind;
+  const int w = threadIdx.x >> 5, at = threadIdx.x & 31;
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t le = k < w ? mask[k] : k == w ? mask[k] & (0xffffffffu >> (31 - at)) : 0u;
+    if (le) lo = blockIdx.x * PA_TILE + k * 32 + 31 - __clz(le);
+  }
+  for (int k = 3; k >= 0; --k) {
+    const uint32_t gt = k > w ? mask[k] : k == w && at < 31 ? mask[k] & (0xffffffffu << (at + 1)) : 0u;
+    if (gt) hi = blockIdx.x * PA_TILE + k * 32 + __ffs(gt) - 1;
+  }
+  if (row < rows) {
+    const_cast<int*>(p.doc_lo)[row] = lo;
+    const_cast<int*>(p.doc_hi)[row] = hi;
+  }
+  if (threadIdx.x == 0) const_cast<int*>(p.tile_lo)[blockIdx.x] = lo;       // row 0 of the tile has its least lo
+  if (row == min(rows, ((int)blockIdx.x + 1) * PA_TILE) - 1) const_cast<int*>(p.tile_hi)[blockIdx.x] = hi;
+}
+
+__device__ __forceinline__ int pa_key_tiles(const PackedPlan& p, int t) {
+  const int lo = p.tile_lo[t];
+  return lo == PA_NONE ? 0 : t - lo / PA_TILE + 1;
+}
+__device__ __forceinline__ int pa_query_tiles(const PackedPlan& p, int t) {
+  const int hi = p.tile_hi[t];
+  return hi == 0 ? 0 : (hi - 1) / PA_TILE - t + 1;
+}
+// A tile's place is the number of tiles with more work, or as much and a lower index.
+__global__ void packed_order_kernel(int rows, int* base) {
+  const PackedPlan p = packed_plan(base, rows);
+  const int tiles = gridDim.x, pairs = (tiles + 1) / 2, t = blockIdx.x;
+  auto pair_tiles = [&](int i) {
+    const int n1 = 2 * i + 1 < tiles ? pa_key_tiles(p, 2 * i + 1) : 0;
+    return max(n1, pa_key_tiles(p, 2 * i) + (n1 > 0));
+  };
+  const int nq = pa_key_tiles(p, t), nk = pa_query_tiles(p, t), np = t < pairs ? pair_tiles(t) : 0;
+  int bq = 0, bk = 0, bp = 0;
+  for (int u = threadIdx.x; u < tiles; u += blockDim.x) {
+    const int q = pa_key_tiles(p, u), k = pa_query_tiles(p, u);
+    bq += q > nq || (q == nq && u < t);
+    bk += k > nk || (k == nk && u < t);
+    if (u < pairs && t < pairs) {
+      const int x = pair_tiles(u);
+      bp += x > np || (x == np && u < t);
+    }
+  }
+  __shared__ int sum[3];
+  if (threadIdx.x < 3) sum[threadIdx.x] = 0;
+  __syncthreads();
+  atomicAdd(&sum[0], bq);
+  atomicAdd(&sum[1], bk);
+  atomicAdd(&sum[2], bp);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const_cast<int*>(p.q_order)[sum[0]] = t;
+    const_cast<int*>(p.k_order)[sum[1]] = t;
+    if (t < pairs) const_cast<int*>(p.pair_order)[sum[2]] = t;
+  }
+}
+
+// ================================================================ forward
+constexpr int PF_THREADS = 384;
+constexpr float PF_SLACK = 8.f;              // a row's maximum may be this far (log2) below the true one
+
+struct PackedFwdParams {
+  __nv_bfloat16* out;      // [rows, Hq, D]
+  float* lse;              // [Hq, tiles * 128], base-2 log-sum-exp of the scaled scores; +inf where a row sees nothing
+  const int* plan;
+  PackedRows q, k, v;
+  int rows, Hq, Hkv, D;
+  int window;              // 0: whole document
+  int head_pairs;          // two heads of a group share a block, else two tiles of rows
+  float scale_log2;        // softmax scale * log2(e)
+  int* status;
+};
+
+template <int DP>
+struct PackedFwdSmem {
+  static constexpr int TILE = PA_TILE * DP * 2;
+  static constexpr int STAGES = DP == 128 ? 5 : 8;         // key and value tiles in turn
+  static constexpr int Q_OFF = 1024, KV_OFF = Q_OFF + 2 * TILE, TOTAL = KV_OFF + STAGES * TILE;
+  static_assert(TOTAL <= 232448, "shared memory budget");
+};
+
+struct PackedFwdItem {
+  int row[2], head[2], hk;
+  int j0, n;               // first key tile, key tiles
+};
+__device__ __forceinline__ PackedFwdItem pf_item(const PackedFwdParams& p, const PackedPlan& plan, int idx) {
+  PackedFwdItem it;
+  const int tiles = (p.rows + PA_TILE - 1) / PA_TILE;
+  int lo, last;
+  if (p.head_pairs) {
+    const int hp = p.Hq >> 1, o = idx / hp, t = plan.q_order[o];
+    it.head[0] = 2 * (idx - o * hp);
+    it.head[1] = it.head[0] + 1;
+    it.row[0] = it.row[1] = t * PA_TILE;
+    lo = plan.tile_lo[t];
+    last = t;
+  } else {
+    const int o = idx / p.Hq, t = 2 * plan.pair_order[o];
+    it.head[0] = it.head[1] = idx - o * p.Hq;
+    it.row[0] = t * PA_TILE;
+    it.row[1] = it.row[0] + PA_TILE;
+    lo = plan.tile_lo[t];
+    last = t;
+    if (t + 1 < tiles && plan.tile_lo[t + 1] != PA_NONE) {
+      lo = min(lo, plan.tile_lo[t + 1]);
+      last = t + 1;
+    }
+  }
+  it.hk = it.head[0] / (p.Hq / p.Hkv);
+  const int first = p.window > 0 ? max(lo, it.row[0] - p.window + 1) : lo;
+  it.j0 = lo == PA_NONE ? 0 : first / PA_TILE;
+  it.n = lo == PA_NONE ? 0 : last - it.j0 + 1;
+  return it;
+}
+__device__ __forceinline__ void pf_uniform(PackedFwdItem& it) {
+  it.row[0] = warp_uniform(it.row[0]);
+  it.row[1] = warp_uniform(it.row[1]);
+  it.head[0] = warp_uniform(it.head[0]);
+  it.head[1] = warp_uniform(it.head[1]);
+  it.hk = warp_uniform(it.hk);
+  it.j0 = warp_uniform(it.j0);
+  it.n = warp_uniform(it.n);
+}
+
+// One row over its visible keys lo .. row alone (a whole warp)
+__device__ __noinline__ void pf_redo(const PackedFwdParams& p, int row, int head, int lo) {
+  const int hk = head / (p.Hq / p.Hkv), padded = (p.rows + PA_TILE - 1) / PA_TILE * PA_TILE;
+  const float4 q = pa_row4(p.q, row, head, p.D);
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  float m = -INFINITY, l = 0.f;
+  for (int j = lo; j <= row; ++j) {
+    const float s = pa_dot4(q, pa_row4(p.k, j, hk, p.D)) * p.scale_log2;
+    if (pa_nan(s)) { l = s; break; }                                   // and so is the whole row
+    if (s == -INFINITY) continue;
+    const float top = fmaxf(m, s), alpha = m == -INFINITY ? 0.f : pa_exp2(m - top), e = pa_exp2(s - top);
+    l = fmaf(l, alpha, e);
+    o = make_float4(o.x * alpha, o.y * alpha, o.z * alpha, o.w * alpha);
+    pa_add4(o, e, pa_row4(p.v, j, hk, p.D));
+    m = top;
+    if (pa_nan(l)) break;
+  }
+  const float bad = __int_as_float(0x7fffffff), inv = pa_nan(l) || l == 0.f ? bad : 1.f / l;
+  pa_put4(p.out + ((size_t)row * p.Hq + head) * p.D, p.D, o, inv);
+  if ((threadIdx.x & 31) == 0) p.lse[(size_t)head * padded + row] = pa_nan(inv) ? bad : m + log2f(l);
+}
+
+template <int DP>
+__global__ void __launch_bounds__(PF_THREADS, 1)
+packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                  const __grid_constant__ CUtensorMap map_v, const PackedFwdParams p, const int items) {
+  using L = PackedFwdSmem<DP>;
+  constexpr int NST = L::STAGES;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if (smem_u32(smem) & 1023u) {
+    if (threadIdx.x == 0) atomicCAS(p.status, 0, ST_BAD_INDEX);
+    return;
+  }
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(smem);
+  uint64_t* q_empty = q_full + 2;
+  uint64_t* kv_full = q_empty + 2;
+  uint64_t* kv_empty = kv_full + NST;
+  uint64_t* s_full = kv_empty + NST;
+  uint64_t* p_full = s_full + 2;
+  uint64_t* o_full = p_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  uint8_t* q_s = smem + L::Q_OFF;
+  uint8_t* kv_s = smem + L::KV_OFF;
+  const int warp = warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const PackedPlan plan = packed_plan(p.plan, p.rows);
+
+  if (threadIdx.x == 0) {
+    for (int g = 0; g < 2; ++g) {
+      mbar_init(&q_full[g], 1);
+      mbar_init(&q_empty[g], 1);
+      mbar_init(&s_full[g], 1);
+      mbar_init(&p_full[g], 4);
+      mbar_init(&o_full[g], 1);
+    }
+    for (int s = 0; s < NST; ++s) {
+      mbar_init(&kv_full[s], 1);
+      mbar_init(&kv_empty[s], 1);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+    prefetch_tmap(&map_q);
+    prefetch_tmap(&map_k);
+    prefetch_tmap(&map_v);
+  }
+  if (warp == 8) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;            // S of tile g at 128 g, O at 256 + 128 g
+
+  if (warp >= 8) {
+    reg_dec<72>();
+    if (warp == 9) {
+      // ------------------------------------------------------------ copies: Q, Q, then K, V, K, V ...
+      int pos = 0, done = 0;                   // tiles put into the ring, items before this one
+      bool ok = true;
+      for (int r = 0; ok; ++r) {
+        const int idx = pa_item(r);
+        if (r * (int)gridDim.x >= items) break;
+        if (idx >= items) continue;
+        PackedFwdItem it = pf_item(p, plan, idx);
+        pf_uniform(it);
+        if (it.n == 0) continue;
+        auto load_q = [&](int g) {
+          ok = ok && mbar_wait_warp(&q_empty[g], (done & 1) ^ 1, abort_flag, p.status, ST_PATTN_EMPTY);
+          if (ok && elect_one()) {
+            mbar_arrive_expect_tx(&q_full[g], L::TILE);
+            pa_load_tile<DP>(q_s + g * L::TILE, &map_q, &q_full[g], it.head[g], it.row[g]);
+          }
+        };
+        auto load_kv = [&](const CUtensorMap* map, int j) {
+          const int s = pos % NST;
+          ok = ok && mbar_wait_warp(&kv_empty[s], ((pos / NST) & 1) ^ 1, abort_flag, p.status, ST_PATTN_EMPTY);
+          if (ok && elect_one()) {
+            mbar_arrive_expect_tx(&kv_full[s], L::TILE);
+            pa_load_tile<DP>(kv_s + s * L::TILE, map, &kv_full[s], it.hk, j * PA_TILE);
+          }
+          ++pos;
+        };
+        load_q(0);
+        load_kv(&map_k, it.j0);
+        load_q(1);
+        for (int i = 0; ok && i < it.n; ++i) {
+          load_kv(&map_v, it.j0 + i);
+          if (i + 1 < it.n) load_kv(&map_k, it.j0 + i + 1);
+        }
+        ++done;
+      }
+    } else if (warp == 8) {
+      // ------------------------------------------------------------ MMAs
+      constexpr uint32_t idesc_qk = make_idesc(1, 1, 0, 0, PA_TILE, PA_TILE);
+      constexpr uint32_t idesc_pv = make_idesc(1, 1, 0, 1, PA_TILE, DP);
+      const uint64_t qd = make_smem_desc(smem_u32(q_s), 16, 1024, 2);
+      const uint64_t kd = make_smem_desc(smem_u32(kv_s), 16, 1024, 2);
+      const uint64_t vd = make_smem_desc(smem_u32(kv_s), 16384, 1024, 2);     // the same bytes, key rows as the reduction
+      constexpr uint32_t STEP = L::TILE >> 4;
+      int r = 0, left = 0;                     // steps of the item whose scores were issued last that are still to issue
+      int n_item = 0, items_seen = 0, step = 0;
+      bool ok = true, more = true;
+      auto next_item = [&]() {                 // length of the next item that has keys; more = false behind the last
+        while (true) {
+          if (r * (int)gridDim.x >= items) { more = false; return; }
+          const int idx = pa_item(r++);
+          if (idx >= items) continue;
+          const int n = warp_uniform(pf_item(p, plan, idx).n);
+          if (n > 0) { left = n; n_item = n; ++items_seen; return; }
+        }
+      };
+      // ring positions: K of step s at 2 s, V at 2 s + 1
+      auto wait_tile = [&](int pos) {
+        ok = ok && mbar_wait_warp(&kv_full[pos % NST], (pos / NST) & 1, abort_flag, p.status, ST_PATTN_KV_FULL);
+      };
+      auto scores = [&](int g, int st) {       // scores of step st for tile g
+        if (g == 0) wait_tile(2 * st);
+        if (left == n_item) ok = ok && mbar_wait_warp(&q_full[g], (items_seen - 1) & 1, abort_flag, p.status, ST_PATTN_Q);
+        if (!ok) return;
+        tc_fence_after();
+        const int s = (2 * st) % NST;
+        if (elect_one()) {
+          pa_mma_ss<DP>(tmem + g * 128, qd + g * STEP, kd + s * STEP, idesc_qk);
+          umma_commit(&s_full[g]);
+          if (g == 1) umma_commit(&kv_empty[s]);
+          if (left == 1) umma_commit(&q_empty[g]);
+        }
+      };
+      next_item();
+      if (more) {
+        scores(0, 0);
+        scores(1, 0);
+      }
+      int i = 0, n = n_item;                   // the step whose P V comes next, of n
+      while (ok && more) {
+        // what follows this step: the item's next one, or the first of the next item
+        const bool last = i == n - 1;
+        --left;
+        if (last) next_item();
+        for (int g = 0; g < 2; ++g) {
+          ok = ok && mbar_wait_warp(&p_full[g], step & 1, abort_flag, p.status, ST_PATTN_P);
+          if (g == 0) wait_tile(2 * step + 1);
+          if (!ok) break;
+          tc_fence_after();
+          const int s = (2 * step + 1) % NST;
+          if (elect_one()) {
+#pragma unroll
+            for (int kk = 0; kk < PA_TILE / 16; ++kk)
+              umma_f16_ts(tmem + 256 + g * 128, tmem + g * 128 + kk * 8, vd + s * STEP + kk * (2048 >> 4), idesc_pv,
+                          (i | kk) != 0 ? 1u : 0u);
+            if (last) umma_commit(&o_full[g]);
+            if (g == 1) umma_commit(&kv_empty[s]);
+          }
+          if (!last || more) scores(g, step + 1);
+        }
+        ++step;
+        if (last) { i = 0; n = n_item; } else ++i;
+      }
+    }
+  } else {
+    reg_inc<216>();
+    // ------------------------------------------------------------ softmax: a query row per thread
+    const int g = warp >> 2, lg = warp & 3;
+    const int r128 = lg * 32 + lane;
+    const uint32_t s_addr = tmem + g * 128 + (uint32_t(lg * 32) << 16);
+    const uint32_t o_addr = tmem + 256 + g * 128 + (uint32_t(lg * 32) << 16);
+    const int tiles = (p.rows + PA_TILE - 1) / PA_TILE;
+    int step = 0, done = 0;
+    bool ok = true;
+    for (int r = 0; ok; ++r) {
+      const int idx = pa_item(r);
+      if (r * (int)gridDim.x >= items) break;
+      if (idx >= items) continue;
+      const PackedFwdItem it = pf_item(p, plan, idx);
+      const int row = it.row[g] + r128, head = it.head[g];
+      int lo = PA_NONE;                        // first key of this row
+      if (row < p.rows) {
+        lo = plan.doc_lo[row];
+        if (p.window > 0) lo = max(lo, row - p.window + 1);
+      }
+      const bool sees = lo <= row;
+      float m = -INFINITY;                     // maximum (log2 units) that the sums are relative to
+      float2 l2 = make_float2(0.f, 0.f);
+      for (int i = 0; i < it.n; ++i, ++step) {
+        const int kv0 = (it.j0 + i) * PA_TILE;
+        ok = mbar_wait_warp(&s_full[g], step & 1, abort_flag, p.status, ST_PATTN_S);
+        if (!ok) break;
+        tc_fence_after();
+        float s[128];
+#pragma unroll
+        for (int c = 0; c < 128; c += 32) tmem_ld_32x32(s_addr + c, *reinterpret_cast<uint32_t(*)[32]>(&s[c]));
+        tmem_ld_wait();
+        // keys first .. first + span of this tile are visible
+        int first = max(lo - kv0, 0);
+        const int lastk = min(row - kv0, 127);
+        const bool part = !sees || first > 0 || lastk < 127;
+        if (__any_sync(0xffffffffu, part)) {
+          const bool none = !sees || first > lastk;
+          if (none) first = 1 << 20;
+          const uint32_t span = none ? 0u : (uint32_t)(lastk - first);
+#pragma unroll
+          for (int c = 0; c < 128; ++c) s[c] = (uint32_t)(c - first) <= span ? s[c] : -INFINITY;
+        }
+        float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+        for (int c = 4; c < 128; c += 8) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], c + 4 + k < 128 ? fmaxf(s[c + k], s[c + 4 + k]) : s[c + k]);
+        }
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
+        if (m == -INFINITY) m = top;           // nothing has been added yet: no product to bring to this maximum
+        const float old = m;
+        const bool grow = top > m + PF_SLACK;
+        if (__any_sync(0xffffffffu, grow)) {
+          float alpha = 1.f;
+          if (grow) {
+            alpha = pa_exp2(old - top);
+            m = top;
+          }
+          l2 = pa_mul2(l2, make_float2(alpha, alpha));
+#pragma unroll
+          for (int c = 0; c < DP; c += 32) {
+            uint32_t o[32];
+            tmem_ld_32x32(o_addr + c, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+            tmem_st_32x32(o_addr + c, o);
+          }
+        }
+        const float base = m == -INFINITY ? 0.f : -m;
+        const float2 c2 = make_float2(p.scale_log2, p.scale_log2), b2 = make_float2(base, base);
+#pragma unroll
+        for (int c = 0; c < 128; c += 32) {
+          uint32_t packed[16];
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            float2 x = pa_fma2(make_float2(s[c + 2 * k], s[c + 2 * k + 1]), c2, b2);
+            x.x = pa_exp2(x.x);
+            x.y = pa_exp2(x.y);
+            l2 = pa_add2(l2, x);
+            packed[k] = pa_pack(x.x, x.y);
+          }
+          tmem_st_32x16(s_addr + c / 2, packed);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[g]);
+      }
+      if (!ok) break;
+      const float l = l2.x + l2.y;
+      const float inv = 1.f / l;               // (a row that sees nothing gets zeros)
+      if (it.n > 0) {
+        ok = mbar_wait_warp(&o_full[g], done & 1, abort_flag, p.status, ST_PATTN_OUT);
+        if (!ok) break;
+        tc_fence_after();
+        ++done;
+      }
+      __nv_bfloat16* o_row = p.out + ((size_t)row * p.Hq + head) * p.D;
+      float sum = l;                           // finite if all of the row is (or as good as: else it is made again for nothing)
+#pragma unroll
+      for (int c = 0; c < DP; c += 32) {
+        uint32_t o[32];
+        if (it.n > 0) {
+          tmem_ld_32x32(o_addr + c, o);
+          tmem_ld_wait();
+        }
+#pragma unroll
+        for (int k = 0; k < 32; ++k) sum += fabsf(__uint_as_float(o[k]));
+        if (row < p.rows) {
+#pragma unroll
+          for (int k = 0; k < 32; k += 8) {
+            if (c + k < p.D) {
+              uint4 v = make_uint4(0u, 0u, 0u, 0u);
+              if (sees) {
+                v.x = pa_pack(__uint_as_float(o[k]) * inv, __uint_as_float(o[k + 1]) * inv);
+                v.y = pa_pack(__uint_as_float(o[k + 2]) * inv, __uint_as_float(o[k + 3]) * inv);
+                v.z = pa_pack(__uint_as_float(o[k + 4]) * inv, __uint_as_float(o[k + 5]) * inv);
+                v.w = pa_pack(__uint_as_float(o[k + 6]) * inv, __uint_as_float(o[k + 7]) * inv);
+              }
+              *reinterpret_cast<uint4*>(o_row + c + k) = v;
+            }
+          }
+        }
+      }
+      if (it.row[g] < tiles * PA_TILE)
+        p.lse[(size_t)head * tiles * PA_TILE + row] = sees ? m + log2f(l) : INFINITY;
+      for (uint32_t again = __ballot_sync(0xffffffffu, sees && !(pa_finite(sum) && l > 0.f)); again; again &= again - 1) {
+        const int who = __ffs(again) - 1;
+        __syncwarp();
+        pf_redo(p, it.row[g] + lg * 32 + who, head, __shfl_sync(0xffffffffu, lo, who));
+      }
+    }
+  }
+
+  // ---------------------------------------------------------------- teardown
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) {
+    uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 100000) __nanosleep(1000);   // let copies in flight land
+    __syncthreads();
+  }
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <int DP>
+static int packed_fwd_launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const PackedFwdParams& p,
+                             cudaStream_t stream) {
+  const int tiles = (p.rows + PA_TILE - 1) / PA_TILE;
+  const long items = p.head_pairs ? (long)tiles * (p.Hq / 2) : (long)((tiles + 1) / 2) * p.Hq;
+  if (items > 0x3fffffff) return -12;
+  SLAB_CUDA_CHECK(cudaFuncSetAttribute(packed_fwd_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       PackedFwdSmem<DP>::TOTAL));
+  const int grid = items < sm_count() ? (int)items : sm_count();
+  packed_fwd_kernel<DP><<<grid, PF_THREADS, PackedFwdSmem<DP>::TOTAL, stream>>>(mq, mk, mv, p, (int)items);
+  return (int)cudaGetLastError();
+}
+
+}  // namespace slab
+
+// int32 words of a plan for `rows` rows
+extern "C" long slab_packed_plan_words(int rows) {
+  const long tiles = ((long)rows + slab::PA_TILE - 1) / slab::PA_TILE;
+  return 2l * rows + 4 * tiles + (tiles + 1) / 2;
+}
+
+// cu [docs + 1] int32: rows of document s are cu[s] .. cu[s + 1] - 1
+extern "C" int slab_packed_plan(const void* cu, int docs, int rows, void* plan, void* status, void* stream) {
+  using namespace slab;
+  if (rows <= 0 || docs < 0) return -10;
+  const int tiles = (rows + PA_TILE - 1) / PA_TILE;
+  cudaStream_t st = (cudaStream_t)stream;
+  packed_bounds_kernel<<<tiles, PA_TILE, 0, st>>>((const int*)cu, docs, rows, (int*)plan, (int*)status);
+  packed_order_kernel<<<tiles, 128, 0, st>>>(rows, (int*)plan);
+  return (int)cudaGetLastError();
+}
+
+// The same from token ids [batch * seq] (int64): a document ends behind every `end` token and with every row of the batch.
+// starts: scratch, 2 int32 per tile.
+extern "C" int slab_packed_plan_tokens(const void* tokens, int rows, int seq, long end, void* starts, void* plan, void* stream) {
+  using namespace slab;
+  if (rows <= 0 || seq <= 0) return -10;
+  const int tiles = (rows + PA_TILE - 1) / PA_TILE;
+  cudaStream_t st = (cudaStream_t)stream;
+  packed_starts_kernel<<<tiles, PA_TILE, 0, st>>>((const long long*)tokens, rows, seq, end, (int*)starts);
+  packed_token_bounds_kernel<<<tiles, PA_TILE, 0, st>>>((const long long*)tokens, rows, seq, end, (const int*)starts, (int*)plan);
+  packed_order_kernel<<<tiles, 128, 0, st>>>(rows, (int*)plan);
+  return (int)cudaGetLastError();
+}
+
+// q [rows, Hq, D], k and v [rows, Hkv, D] bf16 with the given token and head strides (elements, multiples of 8; bases on 16
+// bytes), out [rows, Hq, D] contiguous, lse [Hq, tiles * 128] fp32.  D a multiple of 8 up to 128.
+extern "C" int slab_packed_attn_fwd(const void* q, const void* k, const void* v, void* out, void* lse, const void* plan,
+                                    int rows, int hq, int hkv, int d, long q_ts, long q_hs, long k_ts, long k_hs, long v_ts,
+                                    long v_hs, int window, float scale, void* status, void* stream) {
+  using namespace slab;
+  if (rows <= 0 || hq <= 0 || hkv <= 0 || hq % hkv || d <= 0 || d > 128 || d % 8 || window < 0 || !(scale > 0.f)) return -10;
+  if ((q_ts | q_hs | k_ts | k_hs | v_ts | v_hs) & 7) return -11;
+  static thread_local bool ctx_ready = false;
+  if (!ctx_ready) { cudaFree(0); ctx_ready = true; }
+  CUtensorMap mq, mk, mv;
+  int rc;
+  if ((rc = pa_make_map(&mq, q, rows, hq, d, q_ts, q_hs)) != 0) return rc;
+  if ((rc = pa_make_map(&mk, k, rows, hkv, d, k_ts, k_hs)) != 0) return rc;
+  if ((rc = pa_make_map(&mv, v, rows, hkv, d, v_ts, v_hs)) != 0) return rc;
+  PackedFwdParams p;
+  p.out = (__nv_bfloat16*)out;
+  p.lse = (float*)lse;
+  p.plan = (const int*)plan;
+  p.q = {(const __nv_bfloat16*)q, q_ts, q_hs};
+  p.k = {(const __nv_bfloat16*)k, k_ts, k_hs};
+  p.v = {(const __nv_bfloat16*)v, v_ts, v_hs};
+  p.rows = rows; p.Hq = hq; p.Hkv = hkv; p.D = d;
+  p.window = window;
+  p.head_pairs = (hq / hkv) % 2 == 0;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.status = (int*)status;
+  return d <= 64 ? packed_fwd_launch<64>(mq, mk, mv, p, (cudaStream_t)stream)
+                 : packed_fwd_launch<128>(mq, mk, mv, p, (cudaStream_t)stream);
+}

@@ -1,0 +1,183 @@
+// What the packed-document attention kernels share: tensor memory operands, the documents' plan, item order.
+#pragma once
+#include "common.cuh"
+#include "tma_host.cuh"
+
+namespace slab {
+
+constexpr int PA_TILE = 128;                 // rows of a tile, on the query and on the key side
+constexpr int PA_NONE = 0x7fffffff;          // tile_lo of a tile without rows of a document
+
+enum : int {
+  ST_PATTN_Q = 40,         // waited for a query tile
+  ST_PATTN_KV_FULL = 41,   // waited for a key or value tile
+  ST_PATTN_EMPTY = 42,     // producer waited for a free buffer
+  ST_PATTN_S = 43,         // softmax waited for scores
+  ST_PATTN_P = 44,         // MMA issuer waited for probabilities (or their gradient)
+  ST_PATTN_OUT = 45,       // softmax waited for the finished accumulators
+};
+
+// The plan of a packed buffer (packed_bounds_kernel), int32:
+//   doc_lo[rows], doc_hi[rows]   first row of the row's document, one past its last; a row of no document: row + 1, row
+//   tile_lo[tiles], tile_hi[tiles]   least doc_lo and greatest doc_hi of the tile's rows
+//   q_order, k_order [tiles], pair_order[pairs]   query tiles, key tiles, pairs of query tiles by falling work
+struct PackedPlan {
+  const int* doc_lo;
+  const int* doc_hi;
+  const int* tile_lo;
+  const int* tile_hi;
+  const int* q_order;
+  const int* k_order;
+  const int* pair_order;
+};
+inline __host__ __device__ PackedPlan packed_plan(const int* base, int rows) {
+  const int tiles = (rows + PA_TILE - 1) / PA_TILE;
+  PackedPlan p;
+  p.doc_lo = base;
+  p.doc_hi = p.doc_lo + rows;
+  p.tile_lo = p.doc_hi + rows;
+  p.tile_hi = p.tile_lo + tiles;
+  p.q_order = p.tile_hi + tiles;
+  p.k_order = p.q_order + tiles;
+  p.pair_order = p.k_order + tiles;
+  return p;
+}
+
+// Items are listed by falling work; a persistent block takes one of every round, and rounds run forwards and backwards in
+// turn, so that no block has the longest of each.
+__device__ __forceinline__ int pa_item(int round) {
+  return round * (int)gridDim.x + ((round & 1) ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x);
+}
+
+// ---------------------------------------------------------------- tensor memory
+// D[tmem] (+)= A[tmem] * B[smem desc]: A as 16-bit pairs, row = lane, 8 columns per 16 of the reduction.
+__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::
+          "r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void reg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void reg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+__device__ __forceinline__ uint32_t pa_pack(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+// two fp32 lanes in one instruction
+__device__ __forceinline__ float2 pa_fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
+  return d;
+}
+__device__ __forceinline__ float2 pa_add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return d;
+}
+__device__ __forceinline__ float2 pa_mul2(float2 a, float2 b) {
+  float2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return d;
+}
+__device__ __forceinline__ float pa_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// ---------------------------------------------------------------- rows made again
+// A product with tiles also multiplies what a row must not see, by zero: where that is no number, so is the result.  Rows
+// whose result is not finite are therefore made again by their warp over the visible keys (queries) alone, and then hold
+// what the formula gives.  A lane has four neighbouring columns.
+struct PackedRows {
+  const __nv_bfloat16* p;
+  long ts, hs;             // token and head stride, elements
+};
+__device__ __forceinline__ float4 pa_row4(const PackedRows& t, int row, int head, int d) {
+  const int c = (threadIdx.x & 31) * 4;
+  if (c >= d) return make_float4(0.f, 0.f, 0.f, 0.f);
+  const uint2 v = *reinterpret_cast<const uint2*>(t.p + (size_t)row * t.ts + (size_t)head * t.hs + c);
+  const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v.x));
+  const float2 b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v.y));
+  return make_float4(a.x, a.y, b.x, b.y);
+}
+__device__ __forceinline__ float pa_dot4(const float4& a, const float4& b) {
+  return warp_sum(fmaf(a.x, b.x, fmaf(a.y, b.y, fmaf(a.z, b.z, a.w * b.w))));
+}
+__device__ __forceinline__ void pa_add4(float4& a, float f, const float4& b) {
+  a.x = fmaf(f, b.x, a.x);
+  a.y = fmaf(f, b.y, a.y);
+  a.z = fmaf(f, b.z, a.z);
+  a.w = fmaf(f, b.w, a.w);
+}
+__device__ __forceinline__ void pa_put4(__nv_bfloat16* to, int d, const float4& v, float f) {
+  const int c = (threadIdx.x & 31) * 4;
+  if (c < d) *reinterpret_cast<uint2*>(to + c) = make_uint2(pa_pack(v.x * f, v.y * f), pa_pack(v.z * f, v.w * f));
+}
+__device__ __forceinline__ bool pa_finite(float v) { return (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u; }
+__device__ __forceinline__ bool pa_nan(float v) { return (__float_as_uint(v) & 0x7fffffffu) > 0x7f800000u; }
+
+// Tile of 128 rows x DP columns of one head, as boxes of 64 columns ([128 rows][128 bytes], 128-byte swizzle).  Columns at
+// or beyond the head's width and rows at or beyond the buffer's end read as zero.
+template <int DP>
+__device__ __forceinline__ void pa_load_tile(uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int head, int row) {
+#pragma unroll
+  for (int jb = 0; jb < DP / 64; ++jb) tma_load_3d(dst + jb * 16384, map, bar, jb * 64, head, row);
+}
+// S[tmem] = A B^T over the head's columns, both K-major in shared memory (descriptors of the tiles' first bytes)
+template <int DP>
+__device__ __forceinline__ void pa_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
+#pragma unroll
+  for (int kk = 0; kk < DP / 16; ++kk) {
+    const uint32_t off = ((kk >> 2) * 16384 + (kk & 3) * 32) >> 4;
+    umma_f16(d, a + off, b + off, idesc, kk != 0 ? 1u : 0u);
+  }
+}
+
+// ---------------------------------------------------------------- host
+// [rows, heads, dim] with any token and head strides, read in boxes of 64 columns x 1 head x 128 rows.
+inline int pa_make_map(CUtensorMap* m, const void* base, int rows, int heads, int dim, long token_stride, long head_stride) {
+  TmaEncodeTiledFn enc = tma_encode_fn();
+  if (!enc) return -1;
+  cuuint64_t dims[3] = {(cuuint64_t)dim, (cuuint64_t)heads, (cuuint64_t)rows};
+  cuuint64_t strides[2] = {(cuuint64_t)head_stride * 2, (cuuint64_t)token_stride * 2};
+  cuuint32_t box[3] = {64, 1, PA_TILE};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : -2 - (int)r;
+}
+
+}  // namespace slab

@@ -1,0 +1,868 @@
+// Gradients of causal attention over packed documents (packed_attention.cu) for sm_100a.
+//
+//   p_ij = exp2(scale_log2 q_i.k_j - lse_i)     delta_i = do_i.o_i      ds_ij = p_ij (do_i.v_j - delta_i)
+//   dv_j = sum_i p_ij do_i      dk_j = scale sum_i ds_ij q_i      dq_i = scale sum_j ds_ij k_j
+//
+// Two kernels behind a small one for delta: one per query tile for dq, one per key tile for dk and dv.  Each makes the
+// scores and their gradient again (7 products of 128 x 128 x D a tile pair where one kernel could do with 5), but no sum
+// leaves the tensor cores before it is whole: no atomics, no fp32 copy of dq, and the same bits every time.
+//
+// Roles as in the forward pass (384 threads): warps 0-3 and 4-7 take the left and the right 64 columns of every 128 x 128
+// tile, a row per thread; warp 8 issues the MMAs, warp 9 the copies.  p and ds go back over the scores and products they
+// came from, as bf16, and are the A operand of the next product from tensor memory.  Statistics, p - delta and all sums
+// are fp32; p and ds are rounded to bf16 once, as operands.
+#include "packed_attention.cuh"
+
+namespace slab {
+
+constexpr int PB_THREADS = 384;
+
+struct PackedBwdParams {
+  __nv_bfloat16 *dq, *dk, *dv;   // [rows, heads, D] contiguous
+  float* partial;                // [splits][2][rows, Hkv, D]: dk and dv of a part of every group's heads, or null (splits 1)
+  const float *lse, *delta;      // [Hq, tiles * 128]
+  const int* plan;
+  PackedRows q, k, v, dout;
+  int rows, Hq, Hkv, D;
+  int window;
+  int splits;
+  float scale, scale_log2;
+  int* status;
+};
+
+// bytes (a multiple of 16) from global to shared memory, counted on a barrier; both addresses on 16 bytes
+__device__ __forceinline__ void pb_bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+// ================================================================ delta
+// A group of 16 lanes per (row, head); rows behind the buffer's end, up to whole tiles, get zero.
+__global__ void __launch_bounds__(256)
+packed_delta_kernel(const __nv_bfloat16* out, const __nv_bfloat16* dout, float* delta, int rows, int padded, int hq, int d,
+                    long do_ts, long do_hs) {
+  const long unit = (long)blockIdx.x * 16 + (threadIdx.x >> 4);          // rows fastest: neighbours write side by side
+  const int sub = threadIdx.x & 15;
+  const int head = (int)(unit / padded), row = (int)(unit - (long)head * padded);
+  float sum = 0.f;
+  if (head < hq && row < rows && sub * 8 < d) {
+    float a[8], b[8];
+    unpack8(*reinterpret_cast<const bf16x8*>(out + ((size_t)row * hq + head) * d + sub * 8), a);
+    unpack8(*reinterpret_cast<const bf16x8*>(dout + (size_t)row * do_ts + (size_t)head * do_hs + sub * 8), b);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum = fmaf(a[i], b[i], sum);
+  }
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (sub == 0 && head < hq) delta[(size_t)head * padded + row] = sum;
+}
+
+// ================================================================ common to both
+// 64 scores of a row become probabilities: columns first .. first + span are visible.
+__device__ __forceinline__ void pb_mask(float (&s)[64], int first, uint32_t span) {
+#pragma unroll
+  for (int c = 0; c < 64; ++c) s[c] = (uint32_t)(c - first) <= span ? s[c] : 0.f;
+}
+__device__ __forceinline__ void pb_load64(uint32_t taddr, float (&s)[64]) {
+  tmem_ld_32x32(taddr, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
+  tmem_ld_32x32(taddr + 32, *reinterpret_cast<uint32_t(*)[32]>(&s[32]));
+  tmem_ld_wait();
+}
+__device__ __forceinline__ void pb_store64(uint32_t taddr, const float (&s)[64]) {
+#pragma unroll
+  for (int c = 0; c < 64; c += 32) {
+    uint32_t v[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) v[k] = pa_pack(s[c + 2 * k], s[c + 2 * k + 1]);
+    tmem_st_32x16(taddr + c / 2, v);
+  }
+  tmem_st_wait();
+}
+// A from tensor memory: 128 rows x 128 of the reduction, the left 64 at a, the right ones 64 columns on
+template <int DP>
+__device__ __forceinline__ void pb_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+#pragma unroll
+  for (int kk = 0; kk < 8; ++kk)
+    umma_f16_ts(d, a + (kk >> 2) * 64 + (kk & 3) * 8, b + kk * (2048 >> 4), idesc, (accumulate || kk != 0) ? 1u : 0u);
+}
+
+// ================================================================ dq
+template <int DP>
+struct PackedDqSmem {
+  static constexpr int TILE = PA_TILE * DP * 2;
+  static constexpr int KST = DP == 128 ? 3 : 5, VST = DP == 128 ? 2 : 4;
+  static constexpr int Q_OFF = 1024, DO_OFF = Q_OFF + TILE, K_OFF = DO_OFF + TILE, V_OFF = K_OFF + KST * TILE,
+                       TOTAL = V_OFF + VST * TILE;
+  static_assert(TOTAL <= 232448, "shared memory budget");
+};
+
+struct PackedDqItem {
+  int row, head, hk, j0, n;
+};
+__device__ __forceinline__ PackedDqItem pb_dq_item(const PackedBwdParams& p, const PackedPlan& plan, int idx) {
+  PackedDqItem it;
+  const int o = idx / p.Hq, t = plan.q_order[o], lo = plan.tile_lo[t];
+  it.head = idx - o * p.Hq;
+  it.hk = it.head / (p.Hq / p.Hkv);
+  it.row = t * PA_TILE;
+  const int first = p.window > 0 ? max(lo, it.row - p.window + 1) : lo;
+  it.j0 = lo == PA_NONE ? 0 : first / PA_TILE;
+  it.n = lo == PA_NONE ? 0 : t - it.j0 + 1;
+  it.row = warp_uniform(it.row);
+  it.head = warp_uniform(it.head);
+  it.hk = warp_uniform(it.hk);
+  it.j0 = warp_uniform(it.j0);
+  it.n = warp_uniform(it.n);
+  return it;
+}
+
+// A walk over an issuer's steps (key tiles of item after item), which may run ahead of another one.
+template <typename NextLen>
+struct StepWalk {
+  NextLen next;            // length of the next item with steps, 0 behind the last
+  int n = 0, i = 0, seen = 0, step = 0;
+  bool more = true;
+  __device__ __forceinline__ explicit StepWalk(NextLen f) : next(f) { fetch(); }
+  __device__ __forceinline__ void fetch() {
+    n = next();
+    i = 0;
+    more = n > 0;
+    ++seen;
+  }
+  __device__ __forceinline__ void advance() {
+    ++step;
+    if (++i == n) fetch();
+  }
+  __device__ __forceinline__ bool first() const { return i == 0; }
+  __device__ __forceinline__ bool last() const { return i == n - 1; }
+  __device__ __forceinline__ uint32_t item_parity() const { return (seen - 1) & 1; }
+};
+
+// p and ds of one pair of rows (a whole warp)
+__device__ __forceinline__ float2 pb_pair(const PackedBwdParams& p, int head, int row, const float4& q, const float4& k,
+                                          const float4& v, const float4& dout) {
+  const size_t at = (size_t)head * ((p.rows + PA_TILE - 1) / PA_TILE * PA_TILE) + row;
+  const float prob = pa_exp2(fmaf(pa_dot4(q, k), p.scale_log2, -p.lse[at]));
+  return make_float2(prob, prob * (pa_dot4(dout, v) - p.delta[at]));
+}
+// Columns c0 .. c0 + cols - 1 of dq of one row, over its visible keys lo .. row alone (a whole warp)
+__device__ __noinline__ void pb_redo_dq(const PackedBwdParams& p, int row, int head, int lo, int c0, int cols) {
+  const int hk = head / (p.Hq / p.Hkv);
+  const float4 q = pa_row4(p.q, row, head, p.D), dout = pa_row4(p.dout, row, head, p.D);
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int j = lo; j <= row; ++j) {
+    const float4 k = pa_row4(p.k, j, hk, p.D);
+    const float ds = pb_pair(p, head, row, q, k, pa_row4(p.v, j, hk, p.D), dout).y;
+    pa_add4(sum, ds, k);
+    if (pa_nan(ds)) { sum = make_float4(ds, ds, ds, ds); break; }
+  }
+  if ((uint32_t)((threadIdx.x & 31) * 4 - c0) < (uint32_t)cols)
+    pa_put4(p.dq + ((size_t)row * p.Hq + head) * p.D, p.D, sum, p.scale);
+}
+// dk or dv of one key row for heads h0 .. h0 + heads - 1 over the queries row .. hi - 1 alone (a whole warp)
+__device__ __noinline__ void pb_redo_dkv(const PackedBwdParams& p, bool dv, int row, int hk, int h0, int heads, int part, int hi) {
+  const float4 k = pa_row4(p.k, row, hk, p.D), v = pa_row4(p.v, row, hk, p.D);
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  bool bad = false;
+  for (int h = h0; h < h0 + heads && !bad; ++h) {
+    for (int i = row; i < hi && !bad; ++i) {
+      const float4 q = pa_row4(p.q, i, h, p.D), dout = pa_row4(p.dout, i, h, p.D);
+      const float2 w = pb_pair(p, h, i, q, k, v, dout);
+      pa_add4(sum, dv ? w.x : w.y, dv ? dout : q);
+      bad = pa_nan(dv ? w.x : w.y);
+    }
+  }
+  if (bad) sum.x = sum.y = sum.z = sum.w = __int_as_float(0x7fffffff);
+  const size_t at = ((size_t)row * p.Hkv + hk) * p.D;
+  const float f = dv ? 1.f : p.scale;
+  if (p.splits > 1) {
+    const int c = (threadIdx.x & 31) * 4;
+    if (c < p.D)
+      *reinterpret_cast<float4*>(p.partial + (size_t)(2 * part + (dv ? 1 : 0)) * p.rows * p.Hkv * p.D + at + c) =
+          make_float4(sum.x * f, sum.y * f, sum.z * f, sum.w * f);
+  } else {
+    pa_put4((dv ? p.dv : p.dk) + at, p.D, sum, f);
+  }
+}
+
+template <int DP>
+__global__ void __launch_bounds__(PB_THREADS, 1)
+packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                 const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do,
+                 const PackedBwdParams p, const int items) {
+  using L = PackedDqSmem<DP>;
+  constexpr int KST = L::KST, VST = L::VST;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if (smem_u32(smem) & 1023u) {
+    if (threadIdx.x == 0) atomicCAS(p.status, 0, ST_BAD_INDEX);
+    return;
+  }
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(smem);
+  uint64_t* q_empty = q_full + 1;
+  uint64_t* do_full = q_empty + 1;
+  uint64_t* do_empty = do_full + 1;
+  uint64_t* s_full = do_empty + 1;             // [2]
+  uint64_t* dp_full = s_full + 2;
+  uint64_t* ds_full = dp_full + 1;
+  uint64_t* dq_full = ds_full + 1;
+  uint64_t* k_full = dq_full + 1;
+  uint64_t* k_empty = k_full + KST;
+  uint64_t* v_full = k_empty + KST;
+  uint64_t* v_empty = v_full + VST;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_empty + VST);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  uint8_t *q_s = smem + L::Q_OFF, *do_s = smem + L::DO_OFF, *k_s = smem + L::K_OFF, *v_s = smem + L::V_OFF;
+  const int warp = warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const PackedPlan plan = packed_plan(p.plan, p.rows);
+
+  if (threadIdx.x == 0) {
+    for (uint64_t* b = q_full; b < v_empty + VST; ++b) mbar_init(b, b == ds_full ? 8 : 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    prefetch_tmap(&map_q);
+    prefetch_tmap(&map_k);
+    prefetch_tmap(&map_v);
+    prefetch_tmap(&map_do);
+  }
+  if (warp == 8) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;            // S at 0 and 128 in turn, dP at 256, dQ at 384
+
+  if (warp >= 8) {
+    reg_dec<72>();
+    if (warp == 9) {
+      int pos = 0, done = 0;
+      bool ok = true;
+      auto load = [&](uint8_t* dst, const CUtensorMap* map, uint64_t* full, uint64_t* empty, uint32_t parity, int head, int row) {
+        ok = ok && mbar_wait_warp(empty, parity, abort_flag, p.status, ST_PATTN_EMPTY);
+        if (ok && elect_one()) {
+          mbar_arrive_expect_tx(full, L::TILE);
+          pa_load_tile<DP>(dst, map, full, head, row);
+        }
+      };
+      for (int r = 0; ok && r * (int)gridDim.x < items; ++r) {
+        const int idx = pa_item(r);
+        if (idx >= items) continue;
+        const PackedDqItem it = pb_dq_item(p, plan, idx);
+        if (it.n == 0) continue;
+        load(q_s, &map_q, q_full, q_empty, (done & 1) ^ 1, it.head, it.row);
+        for (int i = 0; ok && i < it.n; ++i, ++pos) {
+          const int ks = pos % KST, vs = pos % VST, row = (it.j0 + i) * PA_TILE;
+          load(k_s + ks * L::TILE, &map_k, &k_full[ks], &k_empty[ks], ((pos / KST) & 1) ^ 1, it.hk, row);
+          if (i == 0) load(do_s, &map_do, do_full, do_empty, (done & 1) ^ 1, it.head, it.row);
+          load(v_s + vs * L::TILE, &map_v, &v_full[vs], &v_empty[vs], ((pos / VST) & 1) ^ 1, it.hk, row);
+        }
+        ++done;
+      }
+    } else if (warp == 8) {
+      constexpr uint32_t idesc_s = make_idesc(1, 1, 0, 0, PA_TILE, PA_TILE);
+      constexpr uint32_t idesc_d = make_idesc(1, 1, 0, 1, PA_TILE, DP);
+      constexpr uint32_t STEP = L::TILE >> 4;
+      const uint64_t qd = make_smem_desc(smem_u32(q_s), 16, 1024, 2), dod = make_smem_desc(smem_u32(do_s), 16, 1024, 2);
+      const uint64_t kd = make_smem_desc(smem_u32(k_s), 16, 1024, 2), vd = make_smem_desc(smem_u32(v_s), 16, 1024, 2);
+      const uint64_t kt = make_smem_desc(smem_u32(k_s), 16384, 1024, 2);      // K with its rows as the reduction
+      bool ok = true;
+      auto lens = [&, r = 0]() mutable {
+        while (r * (int)gridDim.x < items) {
+          const int idx = pa_item(r++);
+          if (idx >= items) continue;
+          const int n = pb_dq_item(p, plan, idx).n;
+          if (n > 0) return n;
+        }
+        return 0;
+      };
+      StepWalk<decltype(lens)> ws(lens), wp(lens), wq(lens);                  // scores run two steps ahead, dP one
+      auto scores = [&]() {
+        if (!ok || !ws.more) return;
+        const int s = ws.step % KST;
+        ok = mbar_wait_warp(&k_full[s], (ws.step / KST) & 1, abort_flag, p.status, ST_PATTN_KV_FULL);
+        if (ws.first()) ok = ok && mbar_wait_warp(q_full, ws.item_parity(), abort_flag, p.status, ST_PATTN_Q);
+        if (!ok) return;
+        tc_fence_after();
+        if (elect_one()) {
+          pa_mma_ss<DP>(tmem + (ws.step & 1) * 128, qd, kd + s * STEP, idesc_s);
+          umma_commit(&s_full[ws.step & 1]);
+          if (ws.last()) umma_commit(q_empty);
+        }
+        ws.advance();
+      };
+      auto dprob = [&]() {
+        if (!ok || !wp.more) return;
+        const int s = wp.step % VST;
+        ok = mbar_wait_warp(&v_full[s], (wp.step / VST) & 1, abort_flag, p.status, ST_PATTN_KV_FULL);
+        if (wp.first()) ok = ok && mbar_wait_warp(do_full, wp.item_parity(), abort_flag, p.status, ST_PATTN_Q);
+        if (!ok) return;
+        tc_fence_after();
+        if (elect_one()) {
+          pa_mma_ss<DP>(tmem + 256, dod, vd + s * STEP, idesc_s);
+          umma_commit(dp_full);
+          umma_commit(&v_empty[s]);
+          if (wp.last()) umma_commit(do_empty);
+        }
+        wp.advance();
+      };
+      scores();
+      dprob();
+      scores();
+      while (ok && wq.more) {
+        ok = mbar_wait_warp(ds_full, wq.step & 1, abort_flag, p.status, ST_PATTN_P);
+        if (!ok) break;
+        dprob();                               // the softmax has read dP
+        if (!ok) break;
+        tc_fence_after();
+        const int s = wq.step % KST;
+        if (elect_one()) {
+          pb_mma_ts<DP>(tmem + 384, tmem + (wq.step & 1) * 128, kt + s * STEP, idesc_d, !wq.first());
+          umma_commit(&k_empty[s]);
+          if (wq.last()) umma_commit(dq_full);
+        }
+        wq.advance();
+        scores();
+      }
+    }
+  } else {
+    reg_inc<216>();
+    const int g = warp >> 2, lg = warp & 3;
+    const uint32_t base = tmem + (uint32_t(lg * 32) << 16);
+    const int padded = (p.rows + PA_TILE - 1) / PA_TILE * PA_TILE;
+    int step = 0, done = 0;
+    bool ok = true;
+    for (int r = 0; ok && r * (int)gridDim.x < items; ++r) {
+      const int idx = pa_item(r);
+      if (idx >= items) continue;
+      const PackedDqItem it = pb_dq_item(p, plan, idx);
+      const int row = it.row + lg * 32 + lane;
+      int lo = PA_NONE;
+      if (row < p.rows) {
+        lo = plan.doc_lo[row];
+        if (p.window > 0) lo = max(lo, row - p.window + 1);
+      }
+      const bool sees = lo <= row;
+      const float nlse = -p.lse[(size_t)it.head * padded + row], delta = p.delta[(size_t)it.head * padded + row];
+      const float2 c2 = make_float2(p.scale_log2, p.scale_log2), b2 = make_float2(nlse, nlse), d2 = make_float2(-delta, -delta);
+      for (int i = 0; i < it.n; ++i, ++step) {
+        const int c0 = (it.j0 + i) * PA_TILE + g * 64;         // first key of this thread's columns
+        ok = mbar_wait_warp(&s_full[step & 1], (step >> 1) & 1, abort_flag, p.status, ST_PATTN_S);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t s_addr = base + (step & 1) * 128 + g * 64;
+        float s[64];
+        pb_load64(s_addr, s);
+#pragma unroll
+        for (int c = 0; c < 64; c += 2) {
+          const float2 x = pa_fma2(make_float2(s[c], s[c + 1]), c2, b2);
+          s[c] = pa_exp2(x.x);
+          s[c + 1] = pa_exp2(x.y);
+        }
+        int first = max(lo - c0, 0);
+        const int lastk = min(row - c0, 63);
+        const bool none = !sees || first > lastk;
+        const bool part = none || first > 0 || lastk < 63;
+        if (none) first = 1 << 20;
+        const uint32_t span = none ? 0u : (uint32_t)(lastk - first);
+        const bool masked = __any_sync(0xffffffffu, part);
+        if (masked) pb_mask(s, first, span);
+        ok = mbar_wait_warp(dp_full, step & 1, abort_flag, p.status, ST_PATTN_S);
+        if (!ok) break;
+        tc_fence_after();
+        float t[64];
+        pb_load64(base + 256 + g * 64, t);
+#pragma unroll
+        for (int c = 0; c < 64; c += 2) {
+          const float2 x = pa_mul2(make_float2(s[c], s[c + 1]), pa_add2(make_float2(t[c], t[c + 1]), d2));
+          s[c] = x.x;
+          s[c + 1] = x.y;
+        }
+        if (masked) pb_mask(s, first, span);   // zero times what a hidden key holds may be no number
+        pb_store64(s_addr, s);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(ds_full);
+      }
+      if (!ok) break;
+      if (it.n > 0) {
+        ok = mbar_wait_warp(dq_full, done & 1, abort_flag, p.status, ST_PATTN_OUT);
+        if (!ok) break;
+        tc_fence_after();
+        ++done;
+      }
+      __nv_bfloat16* dq_row = p.dq + ((size_t)row * p.Hq + it.head) * p.D;
+      float sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < DP / 2; k += 32) {
+        const int c = g * (DP / 2) + k;
+        uint32_t o[32];
+        if (it.n > 0) {
+          tmem_ld_32x32(base + 384 + c, o);
+          tmem_ld_wait();
+        }
+#pragma unroll
+        for (int e = 0; e < 32; ++e) sum += fabsf(__uint_as_float(o[e]));
+        if (row < p.rows) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            if (c + e < p.D) {
+              uint4 v = make_uint4(0u, 0u, 0u, 0u);
+              if (sees) {
+                v.x = pa_pack(__uint_as_float(o[e]) * p.scale, __uint_as_float(o[e + 1]) * p.scale);
+                v.y = pa_pack(__uint_as_float(o[e + 2]) * p.scale, __uint_as_float(o[e + 3]) * p.scale);
+                v.z = pa_pack(__uint_as_float(o[e + 4]) * p.scale, __uint_as_float(o[e + 5]) * p.scale);
+                v.w = pa_pack(__uint_as_float(o[e + 6]) * p.scale, __uint_as_float(o[e + 7]) * p.scale);
+              }
+              *reinterpret_cast<uint4*>(dq_row + c + e) = v;
+            }
+          }
+        }
+      }
+      for (uint32_t m = __ballot_sync(0xffffffffu, sees && !pa_finite(sum)); m; m &= m - 1) {
+        const int who = __ffs(m) - 1;
+        __syncwarp();
+        pb_redo_dq(p, it.row + lg * 32 + who, it.head, __shfl_sync(0xffffffffu, lo, who), g * (DP / 2), DP / 2);
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) {
+    uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 100000) __nanosleep(1000);   // let copies in flight land
+    __syncthreads();
+  }
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// ================================================================ dk, dv
+template <int DP>
+struct PackedDkvSmem {
+  static constexpr int TILE = PA_TILE * DP * 2;
+  static constexpr int ST = DP == 128 ? 2 : 3;
+  static constexpr int STAT_OFF = 1024, K_OFF = STAT_OFF + 4096, V_OFF = K_OFF + TILE, Q_OFF = V_OFF + TILE,
+                       DO_OFF = Q_OFF + ST * TILE, TOTAL = DO_OFF + ST * TILE;     // STAT: lse[ST][128], delta[ST][128]
+  static_assert(ST * 1024 <= 4096 && K_OFF % 1024 == 0 && TOTAL <= 232448, "shared memory budget");
+};
+
+struct PackedDkvItem {
+  int tile, row, hk, part;
+  int h0, heads;           // query heads of this part of the group
+  int tiles, n;            // query tiles of each, steps over all
+};
+__device__ __forceinline__ PackedDkvItem pb_dkv_item(const PackedBwdParams& p, const PackedPlan& plan, int idx) {
+  PackedDkvItem it;
+  const int per = p.Hkv * p.splits, o = idx / per, rest = idx - o * per, G = p.Hq / p.Hkv;
+  it.tile = plan.k_order[o];
+  it.hk = rest / p.splits;
+  it.part = rest - it.hk * p.splits;
+  const int a = it.part * G / p.splits, b = (it.part + 1) * G / p.splits;
+  it.h0 = it.hk * G + a;
+  it.heads = b - a;
+  it.row = it.tile * PA_TILE;
+  int hi = plan.tile_hi[it.tile];
+  if (p.window > 0) hi = min(hi, it.row + PA_TILE - 1 + p.window);
+  it.tiles = hi <= 0 ? 0 : (hi - 1) / PA_TILE - it.tile + 1;
+  it.tile = warp_uniform(it.tile);
+  it.row = warp_uniform(it.row);
+  it.hk = warp_uniform(it.hk);
+  it.part = warp_uniform(it.part);
+  it.h0 = warp_uniform(it.h0);
+  it.heads = warp_uniform(it.heads);
+  it.tiles = warp_uniform(it.tiles);
+  it.n = it.tiles * it.heads;
+  return it;
+}
+
+template <int DP>
+__global__ void __launch_bounds__(PB_THREADS, 1)
+packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                  const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do,
+                  const PackedBwdParams p, const int items) {
+  using L = PackedDkvSmem<DP>;
+  constexpr int ST = L::ST;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if (smem_u32(smem) & 1023u) {
+    if (threadIdx.x == 0) atomicCAS(p.status, 0, ST_BAD_INDEX);
+    return;
+  }
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(smem);
+  uint64_t* k_empty = k_full + 1;
+  uint64_t* v_full = k_empty + 1;
+  uint64_t* v_empty = v_full + 1;
+  uint64_t* s_full = v_empty + 1;
+  uint64_t* p_full = s_full + 1;
+  uint64_t* dp_full = p_full + 1;
+  uint64_t* ds_full = dp_full + 1;
+  uint64_t* out_full = ds_full + 1;
+  uint64_t* q_full = out_full + 1;
+  uint64_t* q_empty = q_full + ST;
+  uint64_t* do_full = q_empty + ST;
+  uint64_t* do_empty = do_full + ST;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(do_empty + ST);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  float* lse_s = reinterpret_cast<float*>(smem + L::STAT_OFF);
+  float* delta_s = lse_s + ST * PA_TILE;
+  uint8_t *k_s = smem + L::K_OFF, *v_s = smem + L::V_OFF, *q_s = smem + L::Q_OFF, *do_s = smem + L::DO_OFF;
+  const int warp = warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const PackedPlan plan = packed_plan(p.plan, p.rows);
+  const int padded = (p.rows + PA_TILE - 1) / PA_TILE * PA_TILE;
+
+  if (threadIdx.x == 0) {
+    for (uint64_t* b = k_full; b < do_empty + ST; ++b) mbar_init(b, b == p_full || b == ds_full ? 8 : 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    prefetch_tmap(&map_q);
+    prefetch_tmap(&map_k);
+    prefetch_tmap(&map_v);
+    prefetch_tmap(&map_do);
+  }
+  if (warp == 8) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;            // S^T at 0, dP^T at 128, dV at 256, dK at 384
+
+  if (warp >= 8) {
+    reg_dec<72>();
+    if (warp == 9) {
+      int pos = 0, done = 0;
+      bool ok = true;
+      auto load = [&](uint8_t* dst, const CUtensorMap* map, uint64_t* full, uint64_t* empty, uint32_t parity, int head, int row,
+                      float* stat_dst, const float* stat) {
+        ok = ok && mbar_wait_warp(empty, parity, abort_flag, p.status, ST_PATTN_EMPTY);
+        if (ok && elect_one()) {
+          mbar_arrive_expect_tx(full, L::TILE + (stat ? PA_TILE * 4 : 0));
+          pa_load_tile<DP>(dst, map, full, head, row);
+          if (stat) pb_bulk_load(stat_dst, stat + (size_t)head * padded + row, PA_TILE * 4, full);
+        }
+      };
+      for (int r = 0; ok && r * (int)gridDim.x < items; ++r) {
+        const int idx = pa_item(r);
+        if (idx >= items) continue;
+        const PackedDkvItem it = pb_dkv_item(p, plan, idx);
+        if (it.n == 0) continue;
+        load(k_s, &map_k, k_full, k_empty, (done & 1) ^ 1, it.hk, it.row, nullptr, nullptr);
+        int head = it.h0, t = 0;
+        for (int i = 0; ok && i < it.n; ++i, ++pos) {
+          const int s = pos % ST, row = (it.tile + t) * PA_TILE;
+          const uint32_t parity = ((pos / ST) & 1) ^ 1;
+          load(q_s + s * L::TILE, &map_q, &q_full[s], &q_empty[s], parity, head, row, lse_s + s * PA_TILE, p.lse);
+          if (i == 0) load(v_s, &map_v, v_full, v_empty, (done & 1) ^ 1, it.hk, it.row, nullptr, nullptr);
+          load(do_s + s * L::TILE, &map_do, &do_full[s], &do_empty[s], parity, head, row, delta_s + s * PA_TILE, p.delta);
+          if (++t == it.tiles) { t = 0; ++head; }
+        }
+        ++done;
+      }
+    } else if (warp == 8) {
+      constexpr uint32_t idesc_s = make_idesc(1, 1, 0, 0, PA_TILE, PA_TILE);
+      constexpr uint32_t idesc_d = make_idesc(1, 1, 0, 1, PA_TILE, DP);
+      constexpr uint32_t STEP = L::TILE >> 4;
+      const uint64_t kd = make_smem_desc(smem_u32(k_s), 16, 1024, 2), vd = make_smem_desc(smem_u32(v_s), 16, 1024, 2);
+      const uint64_t qd = make_smem_desc(smem_u32(q_s), 16, 1024, 2), dod = make_smem_desc(smem_u32(do_s), 16, 1024, 2);
+      const uint64_t qt = make_smem_desc(smem_u32(q_s), 16384, 1024, 2), dot = make_smem_desc(smem_u32(do_s), 16384, 1024, 2);
+      bool ok = true;
+      auto lens = [&, r = 0]() mutable {
+        while (r * (int)gridDim.x < items) {
+          const int idx = pa_item(r++);
+          if (idx >= items) continue;
+          const int n = pb_dkv_item(p, plan, idx).n;
+          if (n > 0) return n;
+        }
+        return 0;
+      };
+      StepWalk<decltype(lens)> w(lens);        // the step whose scores and dP come next
+      auto scores = [&]() {
+        if (!ok || !w.more) return;
+        const int s = w.step % ST;
+        ok = mbar_wait_warp(&q_full[s], (w.step / ST) & 1, abort_flag, p.status, ST_PATTN_Q);
+        if (w.first()) ok = ok && mbar_wait_warp(k_full, w.item_parity(), abort_flag, p.status, ST_PATTN_KV_FULL);
+        if (!ok) return;
+        tc_fence_after();
+        if (elect_one()) {
+          pa_mma_ss<DP>(tmem, kd, qd + s * STEP, idesc_s);
+          umma_commit(s_full);
+          if (w.last()) umma_commit(k_empty);
+        }
+      };
+      auto dprob = [&]() {
+        if (!ok || !w.more) return;
+        const int s = w.step % ST;
+        ok = mbar_wait_warp(&do_full[s], (w.step / ST) & 1, abort_flag, p.status, ST_PATTN_Q);
+        if (w.first()) ok = ok && mbar_wait_warp(v_full, w.item_parity(), abort_flag, p.status, ST_PATTN_KV_FULL);
+        if (!ok) return;
+        tc_fence_after();
+        if (elect_one()) {
+          pa_mma_ss<DP>(tmem + 128, vd, dod + s * STEP, idesc_s);
+          umma_commit(dp_full);
+          if (w.last()) umma_commit(v_empty);
+        }
+      };
+      scores();
+      dprob();
+      while (ok && w.more) {
+        const int s = w.step % ST;
+        const uint32_t parity = w.step & 1;
+        const bool first = w.first(), last = w.last();
+        w.advance();                           // now at the step behind this one
+        ok = mbar_wait_warp(p_full, parity, abort_flag, p.status, ST_PATTN_P);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+          pb_mma_ts<DP>(tmem + 256, tmem, dot + s * STEP, idesc_d, !first);
+          umma_commit(&do_empty[s]);
+        }
+        scores();
+        ok = ok && mbar_wait_warp(ds_full, parity, abort_flag, p.status, ST_PATTN_P);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+          pb_mma_ts<DP>(tmem + 384, tmem + 128, qt + s * STEP, idesc_d, !first);
+          umma_commit(&q_empty[s]);
+          if (last) umma_commit(out_full);
+        }
+        dprob();
+      }
+    }
+  } else {
+    reg_inc<216>();
+    const int g = warp >> 2, lg = warp & 3;
+    const uint32_t base = tmem + (uint32_t(lg * 32) << 16);
+    int step = 0, done = 0;
+    bool ok = true;
+    const float2 c2 = make_float2(p.scale_log2, p.scale_log2);
+    for (int r = 0; ok && r * (int)gridDim.x < items; ++r) {
+      const int idx = pa_item(r);
+      if (idx >= items) continue;
+      const PackedDkvItem it = pb_dkv_item(p, plan, idx);
+      const int row = it.row + lg * 32 + lane;                 // key row of this thread
+      int hi = 0;                                              // one past the last query row that sees it
+      if (row < p.rows) {
+        hi = plan.doc_hi[row];
+        if (p.window > 0) hi = min(hi, row + p.window);
+      }
+      int t = 0;
+      for (int i = 0; i < it.n; ++i, ++step) {
+        const int c0 = (it.tile + t) * PA_TILE + g * 64;       // first query row of this thread's columns
+        if (++t == it.tiles) t = 0;
+        const int slot = step % ST;
+        const uint32_t slot_parity = (step / ST) & 1;
+        ok = mbar_wait_warp(s_full, step & 1, abort_flag, p.status, ST_PATTN_S) &&
+             mbar_wait_warp(&q_full[slot], slot_parity, abort_flag, p.status, ST_PATTN_Q);
+        if (!ok) break;
+        tc_fence_after();
+        float s[64];
+        pb_load64(base + g * 64, s);
+        const float4* lse4 = reinterpret_cast<const float4*>(lse_s + slot * PA_TILE + g * 64);
+#pragma unroll
+        for (int c = 0; c < 64; c += 4) {
+          const float4 b = lse4[c / 4];
+          const float2 x = pa_fma2(make_float2(s[c], s[c + 1]), c2, make_float2(-b.x, -b.y));
+          const float2 y = pa_fma2(make_float2(s[c + 2], s[c + 3]), c2, make_float2(-b.z, -b.w));
+          s[c] = pa_exp2(x.x);
+          s[c + 1] = pa_exp2(x.y);
+          s[c + 2] = pa_exp2(y.x);
+          s[c + 3] = pa_exp2(y.y);
+        }
+        int first = max(row - c0, 0);
+        const int lastq = min(hi - 1 - c0, 63);
+        const bool none = first > lastq;
+        const bool masked = __any_sync(0xffffffffu, none || first > 0 || lastq < 63);
+        if (none) first = 1 << 20;
+        const uint32_t span = none ? 0u : (uint32_t)(lastq - first);
+        if (masked) pb_mask(s, first, span);
+        pb_store64(base + g * 64, s);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full);
+        ok = mbar_wait_warp(dp_full, step & 1, abort_flag, p.status, ST_PATTN_S) &&
+             mbar_wait_warp(&do_full[slot], slot_parity, abort_flag, p.status, ST_PATTN_Q);
+        if (!ok) break;
+        tc_fence_after();
+        float u[64];
+        pb_load64(base + 128 + g * 64, u);
+        const float4* delta4 = reinterpret_cast<const float4*>(delta_s + slot * PA_TILE + g * 64);
+#pragma unroll
+        for (int c = 0; c < 64; c += 4) {
+          const float4 b = delta4[c / 4];
+          const float2 x = pa_mul2(make_float2(s[c], s[c + 1]), pa_add2(make_float2(u[c], u[c + 1]), make_float2(-b.x, -b.y)));
+          const float2 y = pa_mul2(make_float2(s[c + 2], s[c + 3]), pa_add2(make_float2(u[c + 2], u[c + 3]), make_float2(-b.z, -b.w)));
+          s[c] = x.x;
+          s[c + 1] = x.y;
+          s[c + 2] = y.x;
+          s[c + 3] = y.y;
+        }
+        if (masked) pb_mask(s, first, span);   // zero times what a hidden row holds may be no number
+        pb_store64(base + 128 + g * 64, s);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(ds_full);
+      }
+      if (!ok) break;
+      if (it.n > 0) {
+        ok = mbar_wait_warp(out_full, done & 1, abort_flag, p.status, ST_PATTN_OUT);
+        if (!ok) break;
+        tc_fence_after();
+        ++done;
+      }
+      // the first group of warps writes dV, the second dK
+      const bool any = hi > row;
+      const float f = g == 0 ? 1.f : p.scale;
+      const size_t at = ((size_t)row * p.Hkv + it.hk) * p.D;
+      __nv_bfloat16* to = (g == 0 ? p.dv : p.dk) + at;
+      float* part = p.partial + ((size_t)(2 * it.part + (g == 0)) * p.rows * p.Hkv) * p.D + at;
+      float sum = 0.f;
+#pragma unroll
+      for (int c = 0; c < DP; c += 32) {
+        uint32_t o[32];
+        if (it.n > 0) {
+          tmem_ld_32x32(base + 256 + (g == 0 ? 0 : 128) + c, o);
+          tmem_ld_wait();
+        }
+#pragma unroll
+        for (int e = 0; e < 32; ++e) sum += fabsf(__uint_as_float(o[e]));
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[e] = any ? __float_as_uint(__uint_as_float(o[e]) * f) : 0u;
+        if (row < p.rows) {
+          if (p.splits > 1) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              if (c + e < p.D) *reinterpret_cast<uint4*>(part + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; e += 8) {
+              if (c + e < p.D) {
+                uint4 v;
+                v.x = pa_pack(__uint_as_float(o[e]), __uint_as_float(o[e + 1]));
+                v.y = pa_pack(__uint_as_float(o[e + 2]), __uint_as_float(o[e + 3]));
+                v.z = pa_pack(__uint_as_float(o[e + 4]), __uint_as_float(o[e + 5]));
+                v.w = pa_pack(__uint_as_float(o[e + 6]), __uint_as_float(o[e + 7]));
+                *reinterpret_cast<uint4*>(to + c + e) = v;
+              }
+            }
+          }
+        }
+      }
+      for (uint32_t m = __ballot_sync(0xffffffffu, any && !pa_finite(sum)); m; m &= m - 1) {
+        const int who = __ffs(m) - 1;
+        __syncwarp();
+        pb_redo_dkv(p, g == 0, it.row + lg * 32 + who, it.hk, it.h0, it.heads, it.part, __shfl_sync(0xffffffffu, hi, who));
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) {
+    uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 100000) __nanosleep(1000);   // let copies in flight land
+    __syncthreads();
+  }
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// dk, dv = the parts' sums, in the parts' order
+__global__ void __launch_bounds__(256)
+packed_join_kernel(const float* partial, __nv_bfloat16* dk, __nv_bfloat16* dv, long n, int splits) {
+  const long v = ((long)blockIdx.x * 256 + threadIdx.x) * 8;
+  if (v >= 2 * n) return;
+  float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < splits; ++s) {
+    const float4* src = reinterpret_cast<const float4*>(partial + 2 * n * s + v);
+    const float4 a = __ldcs(src), b = __ldcs(src + 1);
+    sum[0] += a.x; sum[1] += a.y; sum[2] += a.z; sum[3] += a.w;
+    sum[4] += b.x; sum[5] += b.y; sum[6] += b.z; sum[7] += b.w;
+  }
+  __nv_bfloat16* to = v < n ? dk + v : dv + (v - n);
+  *reinterpret_cast<bf16x8*>(to) = pack8(sum);
+}
+
+template <int DP>
+static int packed_bwd_launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mdo,
+                             const PackedBwdParams& p, cudaStream_t stream) {
+  const long tiles = (p.rows + PA_TILE - 1) / PA_TILE;
+  const long dq_items = tiles * p.Hq, dkv_items = tiles * p.Hkv * p.splits;
+  if (dq_items > 0x3fffffff || dkv_items > 0x3fffffff) return -12;
+  SLAB_CUDA_CHECK(cudaFuncSetAttribute(packed_dq_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, PackedDqSmem<DP>::TOTAL));
+  SLAB_CUDA_CHECK(cudaFuncSetAttribute(packed_dkv_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, PackedDkvSmem<DP>::TOTAL));
+  const int sms = sm_count();
+  packed_dkv_kernel<DP><<<dkv_items < sms ? (int)dkv_items : sms, PB_THREADS, PackedDkvSmem<DP>::TOTAL, stream>>>(
+      mq, mk, mv, mdo, p, (int)dkv_items);
+  packed_dq_kernel<DP><<<dq_items < sms ? (int)dq_items : sms, PB_THREADS, PackedDqSmem<DP>::TOTAL, stream>>>(
+      mq, mk, mv, mdo, p, (int)dq_items);
+  if (p.splits > 1) {
+    const long n = (long)p.rows * p.Hkv * p.D;
+    packed_join_kernel<<<(unsigned)((2 * n / 8 + 255) / 256), 256, 0, stream>>>(p.partial, p.dk, p.dv, n, p.splits);
+  }
+  return (int)cudaGetLastError();
+}
+
+}  // namespace slab
+
+// Into how many parts a group's heads are cut for dk and dv: a key tile's steps are a serial chain, and the longest, of
+// tiles * G steps, should be no more than half of what an SM does in all, tiles (tiles + 1) / 2 * Hq / SMs.
+extern "C" int slab_packed_attn_splits(int rows, int hq, int hkv) {
+  if (rows <= 0 || hkv <= 0 || hq % hkv) return -10;
+  const long tiles = ((long)rows + slab::PA_TILE - 1) / slab::PA_TILE;
+  const int group = hq / hkv;
+  const long want = (4l * slab::sm_count() + (tiles + 1) * hkv - 1) / ((tiles + 1) * hkv);
+  int s = want < group ? (int)want : group;
+  while (group % s) ++s;
+  return s;
+}
+
+// q, k, v, dout with token and head strides as in slab_packed_attn_fwd; out, dq, dk, dv contiguous; lse from the forward pass,
+// delta [Hq, tiles * 128] scratch; partial: scratch of splits * 2 * rows * Hkv * D floats where splits > 1.
+extern "C" int slab_packed_attn_bwd(const void* q, const void* k, const void* v, const void* out, const void* dout, const void* lse,
+                                    const void* plan, void* dq, void* dk, void* dv, void* delta, void* partial, int splits,
+                                    int rows, int hq, int hkv, int d, long q_ts, long q_hs, long k_ts, long k_hs, long v_ts,
+                                    long v_hs, long do_ts, long do_hs, int window, float scale, void* status, void* stream) {
+  using namespace slab;
+  if (rows <= 0 || hq <= 0 || hkv <= 0 || hq % hkv || d <= 0 || d > 128 || d % 8 || window < 0 || !(scale > 0.f)) return -10;
+  if ((q_ts | q_hs | k_ts | k_hs | v_ts | v_hs | do_ts | do_hs) & 7) return -11;
+  if (splits < 1 || splits > hq / hkv || (splits > 1 && !partial)) return -13;
+  static thread_local bool ctx_ready = false;
+  if (!ctx_ready) { cudaFree(0); ctx_ready = true; }
+  CUtensorMap mq, mk, mv, mdo;
+  int rc;
+  if ((rc = pa_make_map(&mq, q, rows, hq, d, q_ts, q_hs)) != 0) return rc;
+  if ((rc = pa_make_map(&mk, k, rows, hkv, d, k_ts, k_hs)) != 0) return rc;
+  if ((rc = pa_make_map(&mv, v, rows, hkv, d, v_ts, v_hs)) != 0) return rc;
+  if ((rc = pa_make_map(&mdo, dout, rows, hq, d, do_ts, do_hs)) != 0) return rc;
+  cudaStream_t st = (cudaStream_t)stream;
+  const int padded = (rows + PA_TILE - 1) / PA_TILE * PA_TILE;
+  const long units = (long)padded * hq;
+  packed_delta_kernel<<<(unsigned)((units + 15) / 16), 256, 0, st>>>((const __nv_bfloat16*)out, (const __nv_bfloat16*)dout,
+                                                                     (float*)delta, rows, padded, hq, d, do_ts, do_hs);
+  PackedBwdParams p;
+  p.dq = (__nv_bfloat16*)dq;
+  p.dk = (__nv_bfloat16*)dk;
+  p.dv = (__nv_bfloat16*)dv;
+  p.partial = (float*)partial;
+  p.lse = (const float*)lse;
+  p.delta = (const float*)delta;
+  p.plan = (const int*)plan;
+  p.q = {(const __nv_bfloat16*)q, q_ts, q_hs};
+  p.k = {(const __nv_bfloat16*)k, k_ts, k_hs};
+  p.v = {(const __nv_bfloat16*)v, v_ts, v_hs};
+  p.dout = {(const __nv_bfloat16*)dout, do_ts, do_hs};
+  p.rows = rows; p.Hq = hq; p.Hkv = hkv; p.D = d;
+  p.window = window;
+  p.splits = splits;
+  p.scale = scale;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.status = (int*)status;
+  return d <= 64 ? packed_bwd_launch<64>(mq, mk, mv, mdo, p, st) : packed_bwd_launch<128>(mq, mk, mv, mdo, p, st);
+}

@@ -154,6 +154,32 @@ def causal_attention(q, k, v, scale=None, window=0):
     return ref.causal_attention(q, k, v, scale, window)
 
 
+def pack_documents(cu_seqlens, rows):
+    """Plan of a buffer of ``rows`` rows that holds document ``s`` at rows ``cu_seqlens[s] .. cu_seqlens[s + 1] - 1``, for
+    :func:`packed_attention`: made once per batch, used by every layer's forward and backward pass."""
+    from . import packed as pa
+    return pa.pack_documents(cu_seqlens, rows)
+
+
+def documents_from_tokens(tokens, end_token):
+    """The same plan for token rows ``[B, S]`` seen as one buffer of ``B * S`` rows: a document ends behind every
+    ``end_token`` and with every row."""
+    from . import packed as pa
+    return pa.documents_from_tokens(tokens, end_token)
+
+
+def packed_attention(q, k, v, documents, scale=None, window=0):
+    """Causal attention inside each of the packed ``documents``: ``q [rows, heads, d]``, ``k`` and ``v [rows, groups, d]``
+    with any strides -> ``[rows, heads, d]``.  ``window > 0`` restricts a row to the last ``window`` keys.  Rows of no
+    document give zeros (and get zero gradients); nothing that one document holds reaches another.  The kernels take bf16
+    and ``d`` a multiple of 8 up to 128; other types and widths run on the oracle."""
+    from . import packed as pa
+    scale = pa.check(q, k, v, documents, scale, window)
+    if use_kernels(q) and pa.supports(q, k, v):
+        return pa.attention(q, k, v, documents, scale, int(window))
+    return ref.packed_attention(q, k, v, documents.doc_lo, documents.doc_hi, scale, int(window))
+
+
 def linear_cross_entropy(h, weight, targets):
     if use_kernels(h):
         return _cuda().linear_cross_entropy(h, weight, targets)

@@ -1,0 +1,206 @@
+"""Causal attention over packed documents (``csrc/packed_attention.cu``): documents of any lengths lie one behind the other
+in one buffer of rows, and a row attends to its own document only (and, with ``window``, to the last ``window`` keys of it).
+
+:func:`pack_documents` (from offsets) or :func:`documents_from_tokens` (from token ids and an end-of-document id) makes
+the plan of a batch once; every layer's forward and backward pass uses it.  Nothing is read back to the host.
+
+The kernels take bf16 and head widths that are multiples of 8 up to 128, with any token and head strides (slices of a
+packed projection are read where they lie).  Everything else is refused on the GPU: the dense oracle would need memory
+that grows with the square of the length.  CPU tensors take the oracle (``reference.packed_attention``).
+
+Reference: the packed fine-tuning batches of ``notes/mlperf-llama/2026-04-29_llama2_70b_lora_baseline_trace_breakdown.md``.
+"""
+from __future__ import annotations
+
+import contextlib
+import math
+
+import torch
+
+from . import cuda
+
+cuda.register("slab_packed_plan", "piippp")
+cuda.register("slab_packed_plan_tokens", "piilppp")
+cuda.register("slab_packed_attn_fwd", "pppppp" + "iiii" + "llllll" + "if" + "pp")
+cuda.register("slab_packed_attn_splits", "iii")
+cuda.register("slab_packed_attn_bwd", "p" * 12 + "i" + "iiii" + "llllllll" + "if" + "pp")
+cuda._KERNELS_PER_CALL.update({"slab_packed_plan": 2, "slab_packed_plan_tokens": 3, "slab_packed_attn_bwd": 3})
+cuda._STATUS_NAMES.update({40: "PACKED_ATTN_Q", 41: "PACKED_ATTN_KV_FULL", 42: "PACKED_ATTN_EMPTY", 43: "PACKED_ATTN_S",
+                           44: "PACKED_ATTN_P", 45: "PACKED_ATTN_OUT"})
+
+TILE = 128
+
+
+class PackedDocuments:
+    """The documents of one packed buffer of ``rows`` rows.  ``plan`` (CUDA): per row the first row of its document and one
+    past its last, per tile of 128 rows their range, and the orders in which the kernels visit tiles; ``doc_lo`` /
+    ``doc_hi`` are its first two parts.  A row of no document has an empty range, ``doc_lo = row + 1``, ``doc_hi = row``."""
+
+    def __init__(self, rows: int, plan: torch.Tensor):
+        self.rows, self.plan = rows, plan
+
+    @property
+    def device(self):
+        return self.plan.device
+
+    @property
+    def doc_lo(self) -> torch.Tensor:
+        return self.plan[:self.rows]
+
+    @property
+    def doc_hi(self) -> torch.Tensor:
+        return self.plan[self.rows:2 * self.rows]
+
+
+def _plan_words(rows: int) -> int:
+    tiles = (rows + TILE - 1) // TILE
+    return 2 * rows + 4 * tiles + (tiles + 1) // 2
+
+
+def on_device(t: torch.Tensor):
+    """Kernels run on the current device's stream: make the tensor's device the current one where it is not."""
+    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def pack_documents(cu_seqlens: torch.Tensor, rows: int) -> PackedDocuments:
+    """Plan of ``rows`` rows that hold documents ``s`` at ``cu_seqlens[s] .. cu_seqlens[s + 1] - 1`` (starting at 0, not
+    falling, documents may be empty; rows behind the last one belong to none).  Offsets on the GPU are checked there:
+    bad ones set the status word (``cuda.check_status``) and never lead a kernel out of the buffer."""
+    if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1 or cu_seqlens.dtype not in (torch.int32, torch.int64):
+        raise ValueError("cu_seqlens has to be a one-dimensional int32 or int64 tensor of document offsets")
+    if not 0 < rows < 2 ** 31 - 256:
+        raise ValueError(f"{rows} rows")
+    if not cu_seqlens.is_cuda:
+        cu = cu_seqlens.long()
+        if int(cu[0]) != 0 or int(cu[-1]) > rows or bool((cu[1:] < cu[:-1]).any()):
+            raise ValueError("cu_seqlens has to start at 0, not fall and not pass the buffer's rows")
+        i = torch.arange(rows)
+        s = torch.searchsorted(cu[1:].contiguous(), i, right=True)
+        inside = s < cu.numel() - 1
+        s = s.clamp_max(max(cu.numel() - 2, 0))
+        lo = torch.where(inside, cu[s], i + 1)
+        hi = torch.where(inside, cu[(s + 1).clamp_max(cu.numel() - 1)], i)
+        return PackedDocuments(rows, torch.cat([lo, hi]).int())
+    cu = cu_seqlens.to(torch.int32).contiguous()
+    plan = torch.empty(_plan_words(rows), dtype=torch.int32, device=cu.device)
+    with on_device(cu):
+        cuda.call("slab_packed_plan", cu, cu.numel() - 1, rows, plan, cuda.status_word(cu.device), cuda.stream())
+    return PackedDocuments(rows, plan)
+
+
+def documents_from_tokens(tokens: torch.Tensor, end_token: int) -> PackedDocuments:
+    """Plan of a batch of token rows ``[B, S]`` (int64) seen as one buffer of ``B * S`` rows: a document ends behind every
+    ``end_token`` and with every row of the batch."""
+    if tokens.dim() != 2 or tokens.numel() == 0 or tokens.dtype != torch.int64:
+        raise ValueError("tokens has to be a non-empty [B, S] int64 tensor")
+    b, s = tokens.shape
+    rows = b * s
+    if rows >= 2 ** 31 - 256:
+        raise ValueError(f"{rows} rows")
+    tok = tokens.contiguous()
+    if not tok.is_cuda:
+        i = torch.arange(rows)
+        start = torch.ones(rows, dtype=torch.bool)
+        start[1:] = (tok.reshape(-1)[:-1] == end_token) | (i[1:] % s == 0)
+        lo = torch.where(start, i, 0).cummax(0).values
+        ends = torch.where(torch.cat([start[1:], torch.ones(1, dtype=torch.bool)]), i + 1, rows)
+        hi = ends.flip(0).cummin(0).values.flip(0)
+        return PackedDocuments(rows, torch.cat([lo, hi]).int())
+    plan = torch.empty(_plan_words(rows), dtype=torch.int32, device=tok.device)
+    starts = torch.empty(2 * ((rows + TILE - 1) // TILE), dtype=torch.int32, device=tok.device)
+    with on_device(tok):
+        cuda.call("slab_packed_plan_tokens", tok, rows, s, int(end_token), starts, plan, cuda.stream())
+    return PackedDocuments(rows, plan)
+
+
+def check(q, k, v, documents, scale, window) -> float:
+    """Refuses what neither path computes; returns the softmax scale."""
+    if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape:
+        raise ValueError(f"q [rows, heads, d], k and v [rows, groups, d] wanted, got {tuple(q.shape)}, {tuple(k.shape)}, "
+                         f"{tuple(v.shape)}")
+    rows, hq, d = q.shape
+    if k.shape[0] != rows or k.shape[2] != d or k.shape[1] == 0 or hq % k.shape[1] or hq == 0 or d == 0:
+        raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} do not go together")
+    if documents.rows != rows:
+        raise ValueError(f"the documents' plan is for {documents.rows} rows, not {rows}")
+    if not (q.dtype == k.dtype == v.dtype):
+        raise ValueError(f"q, k and v differ in type: {q.dtype}, {k.dtype}, {v.dtype}")
+    if not (q.device == k.device == v.device == documents.device):
+        raise ValueError("q, k, v and the documents' plan lie on different devices")
+    if window < 0:
+        raise ValueError(f"window {window}")
+    scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
+    if not (0.0 < scale < math.inf):
+        raise ValueError(f"softmax scale {scale}: has to be positive and finite")
+    return scale
+
+
+def supports(q, k, v) -> bool:
+    return q.dtype == k.dtype == v.dtype == torch.bfloat16 and q.shape[-1] % 8 == 0 and q.shape[-1] <= 128
+
+
+def _readable(t):
+    """``t`` where the copy engine can read it as it lies: unit stride inside a head, other strides and the address on 16
+    bytes (any stride counts as such on a dimension of one)."""
+    ts, hs, es = t.stride()
+    ok = (es == 1 or t.shape[2] == 1) and t.data_ptr() % 16 == 0
+    ok = ok and (t.shape[0] == 1 or (ts % 8 == 0 and ts > 0)) and (t.shape[1] == 1 or (hs % 8 == 0 and hs > 0))
+    return t if ok else t.contiguous().clone() if t.is_contiguous() else t.contiguous()
+
+
+def _strides(t):
+    return (t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]), (t.stride(1) if t.shape[1] > 1 else t.shape[2])
+
+
+def forward(q, k, v, documents: PackedDocuments, scale: float, window: int = 0):
+    """``(out [rows, Hq, d], lse [Hq, tiles * 128])``, ``lse`` the base-2 log-sum-exp of the scaled scores."""
+    rows, hq, d = q.shape
+    out = torch.empty((rows, hq, d), dtype=q.dtype, device=q.device)
+    lse = torch.empty((hq, (rows + TILE - 1) // TILE * TILE), dtype=torch.float32, device=q.device)
+    window = min(int(window), rows)
+    with on_device(q):
+        cuda.call("slab_packed_attn_fwd", q, k, v, out, lse, documents.plan, rows, hq, k.shape[1], d, *_strides(q),
+                  *_strides(k), *_strides(v), window, scale, cuda.status_word(q.device), cuda.stream())
+    return out, lse
+
+
+def backward(q, k, v, out, lse, dout, documents: PackedDocuments, scale: float, window: int = 0):
+    """``(dq, dk, dv)`` from the forward pass's inputs, output and log-sum-exp.  Where a group's heads are cut into parts
+    (few key tiles for the SMs), the parts' sums are kept in fp32 and added up in their order."""
+    rows, hq, d = q.shape
+    hkv = k.shape[1]
+    dout = _readable(dout)
+    dq = torch.empty((rows, hq, d), dtype=q.dtype, device=q.device)
+    dk = torch.empty((rows, hkv, d), dtype=q.dtype, device=q.device)
+    dv = torch.empty_like(dk)
+    delta = torch.empty_like(lse)
+    window = min(int(window), rows)
+    with on_device(q):
+        splits = cuda.lib().slab_packed_attn_splits(rows, hq, hkv)
+        partial = torch.empty(splits * 2 * dk.numel(), dtype=torch.float32, device=q.device) if splits > 1 else None
+        cuda.call("slab_packed_attn_bwd", q, k, v, out, dout, lse, documents.plan, dq, dk, dv, delta, partial, splits, rows,
+                  hq, hkv, d, *_strides(q), *_strides(k), *_strides(v), *_strides(dout), window, scale,
+                  cuda.status_word(q.device), cuda.stream())
+        if splits > 1:
+            cuda.LAUNCHES[0] += 1
+    return dq, dk, dv
+
+
+class _PackedAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, documents, scale, window):
+        q, k, v = _readable(q), _readable(k), _readable(v)
+        out, lse = forward(q, k, v, documents, scale, window)
+        ctx.save_for_backward(q, k, v, out, lse)
+        ctx.documents, ctx.scale, ctx.window = documents, scale, window
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        q, k, v, out, lse = ctx.saved_tensors
+        return backward(q, k, v, out, lse, g, ctx.documents, ctx.scale, ctx.window) + (None, None, None)
+
+
+def attention(q, k, v, documents: PackedDocuments, scale: float, window: int = 0):
+    return _PackedAttention.apply(q, k, v, documents, scale, window)

@@ -214,6 +214,38 @@ def causal_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: f
     return out.reshape(b, hq, s, -1).permute(0, 2, 1, 3).to(q.dtype)
 
 
+def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, doc_lo: torch.Tensor, doc_hi: torch.Tensor,
+                     scale: float, window: int = 0) -> torch.Tensor:
+    """Causal attention inside each document of a packed buffer, one document (and 512 query rows) at a time; q: [T,Hq,D],
+    k, v: [T,Hkv,D], document of row i: rows doc_lo[i] .. doc_hi[i] - 1 (none where doc_lo[i] > i)."""
+    t, hq, d = q.shape
+    hkv = k.shape[1]
+    acc = torch.float64 if q.dtype == torch.float64 else torch.float32
+    at, parts = 0, []
+    lo, hi = doc_lo.tolist(), doc_hi.tolist()
+    while at < t:
+        if lo[at] > at:                                            # a row of no document
+            end = at + 1
+            while end < t and lo[end] > end:
+                end += 1
+            parts.append((q[at:end] * 0).nan_to_num(0.0, 0.0, 0.0).to(q.dtype))
+            at = end
+            continue
+        end = min(hi[at], at + 512)
+        f = max(lo[at], at - window + 1) if window else lo[at]
+        qf = q[at:end].to(acc).reshape(end - at, hkv, hq // hkv, d)
+        s = torch.einsum("ihgd,jhd->hgij", qf, k[f:end].to(acc)) * scale
+        i = torch.arange(at, end, device=q.device)[:, None]
+        j = torch.arange(f, end, device=q.device)[None, :]
+        hidden = j > i
+        if window:
+            hidden = hidden | (j <= i - window)
+        p = s.masked_fill(hidden, float("-inf")).softmax(-1)
+        parts.append(torch.einsum("hgij,jhd->ihgd", p, v[f:end].to(acc)).reshape(end - at, hq, d).to(q.dtype))
+        at = end
+    return torch.cat(parts)
+
+
 # ----------------------------------------------------------------------------
 # loss
 # ----------------------------------------------------------------------------
