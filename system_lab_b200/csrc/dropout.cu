@@ -1,0 +1,109 @@
+// Dropout whose mask is a function of (seed, offset, element) and is never stored, with an optional residual:
+//
+//   y_e = keep_e x_e / (1 - p') + r_e,   keep_e = bits_e >= t,   t = round(65536 p),   p' = t / 65536
+//
+// bits_e: 16 of the 128 bits that Philox-4x32 with ten rounds (Salmon, Moraes, Dror and Shaw, "Parallel random numbers: as
+// easy as 1, 2, 3", 2011) makes of key `seed` and counter (e / 8, offset): element e takes half e % 2 of word (e % 8) / 2.
+// Sixteen bits keep an element's share of the ten rounds small (a thread makes one block for eight elements) and set p to
+// within 2^-17; the kept elements are scaled by the probability as it is then, so the mean is exact.  The gradient is the
+// same kernel on dy without the residual.  Bound by memory: x, r and y move once.
+#include "common.cuh"
+
+namespace slab {
+
+__device__ __forceinline__ uint4 philox(uint4 c, uint2 k) {
+#pragma unroll
+  for (int i = 0; i < 10; ++i) {
+    const uint64_t a = (uint64_t)0xD2511F53u * c.x, b = (uint64_t)0xCD9E8D57u * c.z;
+    c = make_uint4((uint32_t)(b >> 32) ^ c.y ^ k.x, (uint32_t)b, (uint32_t)(a >> 32) ^ c.w ^ k.y, (uint32_t)a);
+    k.x += 0x9E3779B9u;
+    k.y += 0xBB67AE85u;
+  }
+  return c;
+}
+
+template <typename T>
+__device__ __forceinline__ void dr_load(const T* p, float (&f)[8]);
+template <>
+__device__ __forceinline__ void dr_load(const __nv_bfloat16* p, float (&f)[8]) { const uint4 v = __ldcs(reinterpret_cast<const uint4*>(p));
+  unpack8(*reinterpret_cast<const bf16x8*>(&v), f);
+}
+template <>
+__device__ __forceinline__ void dr_load(const float* p, float (&f)[8]) {
+  const float4 a = __ldcs(reinterpret_cast<const float4*>(p)), b = __ldcs(reinterpret_cast<const float4*>(p) + 1);
+  f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+}
+__device__ __forceinline__ void dr_store(__nv_bfloat16* p, const float (&f)[8]) { *reinterpret_cast<bf16x8*>(p) = pack8(f); }
+__device__ __forceinline__ void dr_store(float* p, const float (&f)[8]) {
+  reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
+  reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
+}
+__device__ __forceinline__ float dr_get(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+__device__ __forceinline__ float dr_get(const float* p) { return *p; }
+__device__ __forceinline__ void dr_put(__nv_bfloat16* p, float v) { *p = __float2bfloat16(v); }
+__device__ __forceinline__ void dr_put(float* p, float v) { *p = v; }
+
+template <typename T, bool RES>
+__global__ void __launch_bounds__(256)
+dropout_kernel(const T* __restrict__ x, const T* __restrict__ res, T* __restrict__ y, long n, uint32_t t, float scale, uint64_t seed,
+               const long long* __restrict__ seed_dev, uint64_t offset) {
+  const long g = (long)blockIdx.x * 256 + threadIdx.x, e = g * 8;      // a block of eight elements
+  if (e >= n) return;
+  const bool whole = e + 8 <= n;
+  float f[8], r[8];
+  if (whole) {
+    dr_load(x + e, f);
+    if (RES) dr_load(res + e, r);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      f[i] = e + i < n ? dr_get(x + e + i) : 0.f;
+      if (RES) r[i] = e + i < n ? dr_get(res + e + i) : 0.f;
+    }
+  }
+  const uint64_t key = seed_dev ? (uint64_t)*seed_dev : seed;
+  const uint4 w = philox(make_uint4((uint32_t)g, (uint32_t)((uint64_t)g >> 32), (uint32_t)offset, (uint32_t)(offset >> 32)),
+                         make_uint2((uint32_t)key, (uint32_t)(key >> 32)));
+  const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t bits = (i & 1) ? words[i >> 1] >> 16 : words[i >> 1] & 0xffffu;
+    // (a dropped element is zero whatever it was)
+    f[i] = bits >= t ? (RES ? fmaf(f[i], scale, r[i]) : f[i] * scale) : (RES ? r[i] : 0.f);
+  }
+  if (whole) {
+    dr_store(y + e, f);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (e + i < n) dr_put(y + e + i, f[i]);
+  }
+}
+
+template <typename T>
+static int dropout_launch(const void* x, const void* res, void* y, long n, uint32_t t, float scale, uint64_t seed, const void* seed_dev,
+                          uint64_t offset, cudaStream_t st) {
+  const long blocks = (n + 2047) / 2048;
+  if (blocks > 0x7fffffffl) return -12;
+  if (res)
+    dropout_kernel<T, true><<<(unsigned)blocks, 256, 0, st>>>((const T*)x, (const T*)res, (T*)y, n, t, scale, seed,
+                                                              (const long long*)seed_dev, offset);
+  else
+    dropout_kernel<T, false><<<(unsigned)blocks, 256, 0, st>>>((const T*)x, nullptr, (T*)y, n, t, scale, seed,
+                                                               (const long long*)seed_dev, offset);
+  return (int)cudaGetLastError();
+}
+
+}  // namespace slab
+
+// x, res (or null) and y [n], all bf16 or all fp32, on 16 bytes; t: elements whose 16 bits are below it are dropped (< 65536);
+// seed_dev: one int64 on the device that takes the place of `seed`, or null
+extern "C" int slab_dropout(const void* x, const void* res, void* y, int bf16, long n, int t, long seed, const void* seed_dev,
+                            long offset, void* stream) {
+  using namespace slab;
+  if (n <= 0 || t < 0 || t > 65535) return -10;
+  if (((size_t)x | (size_t)res | (size_t)y) & 15) return -11;
+  const float scale = (float)(65536.0 / (65536 - t));
+  return bf16 ? dropout_launch<__nv_bfloat16>(x, res, y, n, (uint32_t)t, scale, (uint64_t)seed, seed_dev, (uint64_t)offset, (cudaStream_t)stream)
+              : dropout_launch<float>(x, res, y, n, (uint32_t)t, scale, (uint64_t)seed, seed_dev, (uint64_t)offset, (cudaStream_t)stream);
+}

@@ -154,6 +154,30 @@ def causal_attention(q, k, v, scale=None, window=0):
     return ref.causal_attention(q, k, v, scale, window)
 
 
+def embedding(tokens, weight, scale=1.0, dtype=None):
+    """``scale * weight[tokens]`` in ``dtype`` (the table's own by default), differentiable in ``weight [V, H]``.  On the
+    GPU the gradient is summed in fp32 by sorted tokens, in the order of the positions; ids outside the table look up zeros,
+    get no gradient and set the status word (``BAD_INDEX``)."""
+    from . import lookup
+    scale = lookup.check(tokens, weight, scale)
+    dtype = weight.dtype if dtype is None else dtype
+    if use_kernels(weight) and lookup.supports(weight, dtype):
+        return lookup.embedding(tokens, weight, scale, dtype)
+    return ref.embedding(tokens, weight, scale, dtype)
+
+
+def dropout(x, p, seed, offset=0, residual=None):
+    """``keep / (1 - p) * x (+ residual)`` with a mask that is a function of ``(seed, offset, element)`` and is never stored:
+    the same call gives the same mask, on the CPU too; another seed or offset gives another.  ``p`` is taken to the next
+    multiple of 2^-16, and kept elements are scaled for that one.  ``seed`` is an integer or an int64 tensor of one element
+    (read when the kernel runs)."""
+    from . import drop
+    drop.check(x, p, seed, offset, residual)
+    if use_kernels(x):
+        return drop.dropout(x, p, seed, offset, residual)
+    return ref.dropout(x, p, seed, offset, residual)
+
+
 def pack_documents(cu_seqlens, rows):
     """Plan of a buffer of ``rows`` rows that holds document ``s`` at rows ``cu_seqlens[s] .. cu_seqlens[s + 1] - 1``, for
     :func:`packed_attention`: made once per batch, used by every layer's forward and backward pass."""

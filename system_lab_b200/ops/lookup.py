@@ -1,0 +1,83 @@
+"""Embedding lookup with scaling and its gradient by sorted tokens (``csrc/embedding.cu``).
+
+The gradient is summed in fp32 in the order of the positions, so it is the same bits every time.  If the table carries
+``main_grad`` (a view of the flat gradient buffer set by the FSDP engine) it is written there, or added to what an earlier
+micro-batch left there, which touches only the rows the batch names; otherwise autograd gets the whole gradient.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import cuda
+from .packed import on_device
+
+cuda.register("slab_embedding_fwd", "ppipiliifps")
+cuda.register("slab_embedding_chunk", "i")
+cuda.register("slab_embedding_bwd", "ppipippiiifis")
+cuda._KERNELS_PER_CALL["slab_embedding_bwd"] = 3
+
+_TYPES = (torch.float32, torch.bfloat16)
+
+
+def check(tokens, weight, scale) -> float:
+    if weight.dim() != 2 or weight.shape[0] == 0 or weight.shape[1] == 0:
+        raise ValueError(f"a table [vocabulary, hidden] wanted, got {tuple(weight.shape)}")
+    if tokens.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"token ids have to be int32 or int64, not {tokens.dtype}")
+    if tokens.device != weight.device:
+        raise ValueError(f"tokens on {tokens.device}, table on {weight.device}")
+    return float(scale)
+
+
+def supports(weight, dtype) -> bool:
+    return weight.dtype in _TYPES and dtype in _TYPES and weight.shape[0] < 2 ** 31 and weight.shape[1] < 2 ** 28
+
+
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, tokens, weight, scale, dtype):
+        tok = tokens.long().contiguous()
+        w = weight.contiguous()
+        v, h = w.shape
+        if tok.numel() >= 2 ** 31 - 1:
+            raise ValueError(f"{tok.numel()} tokens")
+        out = torch.empty(*tokens.shape, h, dtype=dtype, device=w.device)
+        if tok.numel():
+            with on_device(w):
+                cuda.call("slab_embedding_fwd", tok, w, int(w.dtype == torch.bfloat16), out, int(dtype == torch.bfloat16),
+                          tok.numel(), v, h, scale, cuda.status_word(w.device), cuda.stream())
+        ctx.save_for_backward(tok)
+        ctx.w_ref, ctx.scale, ctx.table = weight, scale, (v, h, w.dtype)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        if not ctx.needs_input_grad[1]:
+            return None, None, None, None
+        (tok,) = ctx.saved_tensors
+        v, h, dtype = ctx.table
+        rows = tok.numel()
+        mg = getattr(ctx.w_ref, "main_grad", None)
+        into = mg if mg is not None and mg.dtype in _TYPES and mg.is_contiguous() else None
+        accumulate = into is not None and ctx.w_ref.main_grad_written
+        dw = into if into is not None else torch.empty(v, h, dtype=dtype, device=g.device)
+        if rows == 0:
+            if not accumulate:
+                dw.zero_()
+        else:
+            g = g.contiguous()
+            with on_device(g):
+                chunk = cuda.lib().slab_embedding_chunk(rows)
+                order = torch.empty(rows + 1, dtype=torch.int32, device=g.device)
+                pieces = torch.empty((rows + chunk - 1) // chunk * 2 * h, dtype=torch.float32, device=g.device)
+                cuda.call("slab_embedding_bwd", tok, g, int(g.dtype == torch.bfloat16), dw, int(dw.dtype == torch.bfloat16),
+                          order, pieces, rows, v, h, ctx.scale, int(accumulate), cuda.stream())
+        if into is not None:
+            ctx.w_ref.main_grad_written = True
+            return None, None, None, None
+        return None, dw, None, None
+
+
+def embedding(tokens, weight, scale: float, dtype):
+    return _Embedding.apply(tokens, weight, scale, dtype)

@@ -57,6 +57,56 @@ def rope(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
 
 
 # ----------------------------------------------------------------------------
+# embedding
+# ----------------------------------------------------------------------------
+def embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, dtype=None) -> torch.Tensor:
+    """``scale * weight[tokens]``; the gradient adds up in the table's type or, where that is narrower, in fp32."""
+    w = weight.float() if weight.dtype in (torch.bfloat16, torch.float16) else weight
+    return (F.embedding(tokens.long(), w) * scale).to(dtype if dtype is not None else weight.dtype)
+
+
+# ----------------------------------------------------------------------------
+# dropout from a counter-based generator
+# ----------------------------------------------------------------------------
+def dropout_threshold(p: float) -> int:
+    """Elements whose 16 random bits are below it are dropped."""
+    return math.floor(p * 65536 + 0.5)
+
+
+def _mul_hi_lo(a: int, b: torch.Tensor):
+    # 32 x 32 -> 64 bits in pieces that int64 holds
+    low, high = a * (b & 0xFFFF), a * (b >> 16)
+    mid = high + (low >> 16)
+    return mid >> 16, ((mid & 0xFFFF) << 16) | (low & 0xFFFF)
+
+
+def philox_bits(n: int, seed: int, offset: int, device=None) -> torch.Tensor:
+    """16 random bits for each of ``n`` elements (int64): Philox-4x32 with ten rounds (Salmon, Moraes, Dror and Shaw, 2011),
+    key ``seed``, counter ``(element // 8, offset)``, eight halves of words per block, low half first."""
+    block = torch.arange((n + 7) // 8, dtype=torch.int64, device=device)
+    c = [block & 0xFFFFFFFF, block >> 32, torch.full_like(block, offset & 0xFFFFFFFF),
+         torch.full_like(block, (offset >> 32) & 0xFFFFFFFF)]
+    k0, k1 = seed & 0xFFFFFFFF, (seed >> 32) & 0xFFFFFFFF
+    for _ in range(10):
+        hi0, lo0 = _mul_hi_lo(0xD2511F53, c[0])
+        hi1, lo1 = _mul_hi_lo(0xCD9E8D57, c[2])
+        c = [hi1 ^ c[1] ^ k0, lo1, hi0 ^ c[3] ^ k1, lo0]
+        k0, k1 = (k0 + 0x9E3779B9) & 0xFFFFFFFF, (k1 + 0xBB67AE85) & 0xFFFFFFFF
+    words = torch.stack(c, dim=-1)
+    return torch.stack([words & 0xFFFF, words >> 16], dim=-1).reshape(-1)[:n]
+
+
+def dropout(x: torch.Tensor, p: float, seed, offset: int = 0, residual: torch.Tensor | None = None) -> torch.Tensor:
+    t = dropout_threshold(p)
+    keep = (philox_bits(x.numel(), int(seed), offset, x.device) >= t).view(x.shape)
+    wide = x.dtype if x.dtype == torch.float64 else torch.float32
+    y = torch.where(keep, x.to(wide) * (65536.0 / (65536 - t)), 0.0)
+    if residual is not None:
+        y = y + residual.to(wide)
+    return y.to(x.dtype)
+
+
+# ----------------------------------------------------------------------------
 # activations
 # ----------------------------------------------------------------------------
 def swiglu(gate_up: torch.Tensor) -> torch.Tensor:
