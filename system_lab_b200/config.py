@@ -62,6 +62,12 @@ class ModelConfig:
     norm_epsilon: float = 1e-6
     init_method_std: float = 0.02
     tie_embeddings: bool = False
+    embedding_multiplier: float = 1.0    # the looked-up rows are scaled by this (sqrt(hidden_size) in some model families)
+    hidden_dropout: float = 0.0          # dropout of the embedding and of every block's output on its way into the residual stream (training only)
+    # documents packed into one sequence: with reset_attention_mask a token attends to its own document only; a document
+    # ends behind every eod_token (and with the sequence)
+    reset_attention_mask: bool = False
+    eod_token: int = -1
     # attention flavour: "gqa" (multi/grouped query) or "mla" (DeepSeek latent attention)
     attention_type: str = "gqa"
     q_lora_rank: int = 0
@@ -75,6 +81,7 @@ class ModelConfig:
     lora_rank: int = 0
     lora_alpha: float = 32.0
     lora_targets: str = "attn"
+    lora_dropout: float = 0.0            # dropout of the adapters' input (training only)
     # dense FFN (used by the first `first_k_dense` layers and by non-MoE models)
     ffn_hidden_size: int = 1024
     first_k_dense: int = 0

@@ -294,10 +294,8 @@ static int em_fwd(const void* tokens, const void* w, void* out, long rows, int v
   return (int)cudaGetLastError();
 }
 
-static int em_chunk(int rows) { return rows <= 2048 ? 8 : rows <= 16384 ? 16 : 32; }
-
 template <typename TW, typename TO, int VEC>
-static int em_bwd(const void* tokens, const void* dout, void* dw, int* order, float* pieces, int rows, int vocab, int h, float scale,
+static int em_bwd(const void* tokens, const void* dout, void* dw, int* order, float* pieces, int rows, int chunk, int vocab, int h, float scale,
                   int accumulate, cudaStream_t st) {
   const int sms = em_sms();
   int* valid = order + rows;
@@ -314,7 +312,7 @@ static int em_bwd(const void* tokens, const void* dout, void* dw, int* order, fl
   p.valid = valid;
   p.pieces = pieces;
   p.h = h;
-  p.chunk = em_chunk(rows);
+  p.chunk = chunk;
   p.accumulate = accumulate;
   p.scale = scale;
   const int vecs = h / VEC;
@@ -351,18 +349,15 @@ extern "C" int slab_embedding_fwd(const void* tokens, const void* w, int w_bf16,
   });
 }
 
-// positions per chunk of the sorted list
-extern "C" int slab_embedding_chunk(int rows) { return slab::em_chunk(rows); }
-
 // dw [vocab, h] (all of it written, or added to), dout [rows, h]; order: scratch of rows + 1 int32, pieces: scratch of
-// ceil(rows / chunk) * 2 * h floats
+// ceil(rows / chunk) * 2 * h floats, chunk: positions of the sorted list that a group of threads adds up
 extern "C" int slab_embedding_bwd(const void* tokens, const void* dout, int out_bf16, void* dw, int w_bf16, void* order, void* pieces,
-                                  int rows, int vocab, int h, float scale, int accumulate, void* stream) {
+                                  int rows, int chunk, int vocab, int h, float scale, int accumulate, void* stream) {
   using namespace slab;
-  if (rows <= 0 || h <= 0 || vocab <= 0) return -10;
+  if (rows <= 0 || h <= 0 || vocab <= 0 || chunk <= 0) return -10;
   const bool vec = h % 8 == 0 && (((size_t)dw | (size_t)dout | (size_t)pieces) & 15) == 0;
   return em_types(w_bf16, out_bf16, vec, [&](auto a, auto b, auto v) {
-    return em_bwd<decltype(a), decltype(b), decltype(v)::value>(tokens, dout, dw, (int*)order, (float*)pieces, rows, vocab, h, scale,
+    return em_bwd<decltype(a), decltype(b), decltype(v)::value>(tokens, dout, dw, (int*)order, (float*)pieces, rows, chunk, vocab, h, scale,
                                                                 accumulate, (cudaStream_t)stream);
   });
 }

@@ -24,6 +24,8 @@ from __future__ import annotations
 
 import hashlib
 import math
+from dataclasses import dataclass
+from functools import partial
 
 import torch
 import torch.nn as nn
@@ -69,18 +71,40 @@ def _balance_table(like: torch.Tensor) -> torch.Tensor:
     return _BALANCE_TABLES[key]
 
 
+@dataclass
+class BatchInfo:
+    """What the layers need to know of a micro-batch beside its hidden states.  ``documents``: plan of the documents packed
+    into its rows (None: a row attends to its whole sequence).  ``seed``: of the dropout masks; every place that drops has an
+    offset of its own, so a recomputed block draws the masks of its first run (None: nothing is dropped)."""
+    documents: object = None
+    seed: int | None = None
+
+
+# offsets of the dropout masks: SITES per layer (the embedding comes before the first)
+SITES = 8
+SITE_ATTN, SITE_FFN, SITE_QKV, SITE_O, SITE_W1, SITE_W2 = range(6)
+
+
+def _dropout(x, p: float, batch: BatchInfo | None, offset: int, residual=None):
+    if p <= 0.0 or batch is None or batch.seed is None:
+        return x if residual is None else residual + x
+    return ops.dropout(x, p, batch.seed, offset, residual=residual)
+
+
 class LoRA(nn.Module):
-    """Rank-r update of a frozen projection: ``y += (alpha / r) * (x A^T) B^T`` with ``A ~ N(0, std)`` and ``B = 0``, so
-    the adapted model starts out equal to the base model (the Llama-2-70B LoRA workload of
+    """Rank-r update of a frozen projection: ``y += (alpha / r) * (drop(x) A^T) B^T`` with ``A ~ N(0, std)`` and ``B = 0``,
+    so the adapted model starts out equal to the base model (the Llama-2-70B LoRA workload of
     ``notes/mlperf-llama/2026-04-29_llama2_70b_lora_baseline_trace_breakdown.md``)."""
 
-    def __init__(self, out_features: int, in_features: int, rank: int, alpha: float):
+    def __init__(self, out_features: int, in_features: int, rank: int, alpha: float, dropout: float = 0.0, offset: int = 0):
         super().__init__()
         self.lora_a = nn.Parameter(torch.empty(rank, in_features))
         self.lora_b = nn.Parameter(torch.empty(out_features, rank))
         self.scale = alpha / rank
+        self.dropout, self.offset = dropout, offset
 
-    def forward(self, x):
+    def forward(self, x, batch: BatchInfo | None = None):
+        x = _dropout(x, self.dropout, batch, self.offset)
         return F.linear(F.linear(x, self.lora_a.to(x.dtype)), self.lora_b.to(x.dtype)) * self.scale
 
 
@@ -114,22 +138,25 @@ class GQAttention(nn.Module):
         if cfg.lora_rank > 0:
             if tp is not None:
                 raise ValueError("LoRA adapters are not combined with tensor parallelism")
-            self.qkv_lora = LoRA(self.wqkv.shape[0], h, cfg.lora_rank, cfg.lora_alpha)
-            self.o_lora = LoRA(h, self.wo.shape[1], cfg.lora_rank, cfg.lora_alpha)
+            at = (layer_idx + 1) * SITES
+            self.qkv_lora = LoRA(self.wqkv.shape[0], h, cfg.lora_rank, cfg.lora_alpha, cfg.lora_dropout, at + SITE_QKV)
+            self.o_lora = LoRA(h, self.wo.shape[1], cfg.lora_rank, cfg.lora_alpha, cfg.lora_dropout, at + SITE_O)
 
-    def forward(self, x, cos, sin):
+    def forward(self, x, cos, sin, batch: BatchInfo | None = None):
         if self.tp is not None:
             x = self.tp.enter(x)              # sequence parallel: whole sequences from here to the output projection
         b, s, _ = x.shape
         qkv = ops.linear(x, self.wqkv)
         if self.qkv_lora is not None:
-            qkv = qkv + self.qkv_lora(x)
+            qkv = qkv + self.qkv_lora(x, batch)
         qkv = ops.rope_packed(qkv, cos, sin, self.nq + self.nkv, self.d)      # q and k heads, one pass
         q, k, v = qkv.split([self.nq * self.d, self.nkv * self.d, self.nkv * self.d], dim=-1)
         q = q.unflatten(-1, (self.nq, self.d))
         k = k.unflatten(-1, (self.nkv, self.d))
         v = v.unflatten(-1, (self.nkv, self.d))
-        if self.cp_group is not None:
+        if batch is not None and batch.documents is not None:
+            o = ops.packed_attention(q.flatten(0, 1), k.flatten(0, 1), v.flatten(0, 1), batch.documents, None, self.window)
+        elif self.cp_group is not None:
             from ..parallel.cp import ulysses_attention
             o = ulysses_attention(q, k, v, self.cp_group, window=self.window)
         else:
@@ -139,7 +166,7 @@ class GQAttention(nn.Module):
             return self.tp.linear_leave(o2, self.wo)
         out = ops.linear(o2, self.wo)
         if self.o_lora is not None:
-            out = out + self.o_lora(o2)
+            out = out + self.o_lora(o2, batch)
         return out
 
 
@@ -176,7 +203,9 @@ class MLAttention(nn.Module):
         self.scale = 1.0 / math.sqrt(qk)
         self.cp_group = cp_group
 
-    def forward(self, x, cos, sin):
+    def forward(self, x, cos, sin, batch: BatchInfo | None = None):
+        if batch is not None and batch.documents is not None:
+            raise ValueError("packed documents are implemented for grouped-query attention")
         tp = self.tp
         if tp is not None:
             # the low-rank down projections are repeated on every rank and need whole sequences as well
@@ -209,13 +238,14 @@ class MLAttention(nn.Module):
 
 
 class DenseFFN(nn.Module):
-    def __init__(self, hidden: int, ffn: int, tp=None, lora_rank: int = 0, lora_alpha: float = 32.0):
+    def __init__(self, hidden: int, ffn: int, tp=None, lora_rank: int = 0, lora_alpha: float = 32.0,
+                 lora_dropout: float = 0.0, offset: int = 0):
         super().__init__()
         self.tp = tp
         self.w1_lora = self.w2_lora = None
         if lora_rank > 0 and tp is None:
-            self.w1_lora = LoRA(2 * ffn, hidden, lora_rank, lora_alpha)
-            self.w2_lora = LoRA(hidden, ffn, lora_rank, lora_alpha)
+            self.w1_lora = LoRA(2 * ffn, hidden, lora_rank, lora_alpha, lora_dropout, offset + SITE_W1)
+            self.w2_lora = LoRA(hidden, ffn, lora_rank, lora_alpha, lora_dropout, offset + SITE_W2)
         f = ffn // (tp.size if tp is not None else 1)          # this rank's columns
         self.w1 = nn.Parameter(torch.empty(2 * f, hidden))     # [gate | up]
         self.w2 = nn.Parameter(torch.empty(hidden, f))
@@ -224,18 +254,18 @@ class DenseFFN(nn.Module):
             mark_sharded(self.w1, 0, (2 * ffn, hidden), tp.segments([ffn, ffn]))
             mark_sharded(self.w2, 1, (hidden, ffn), tp.segments([ffn]))
 
-    def forward(self, x):
+    def forward(self, x, batch: BatchInfo | None = None):
         if self.tp is not None:
             x = self.tp.enter(x)
         gu = ops.linear(x, self.w1)
         if self.w1_lora is not None:
-            gu = gu + self.w1_lora(x)
+            gu = gu + self.w1_lora(x, batch)
         act = ops.swiglu(gu)
         if self.tp is not None:
             return self.tp.linear_leave(act, self.w2)
         out = ops.linear(act, self.w2)
         if self.w2_lora is not None:
-            out = out + self.w2_lora(act)
+            out = out + self.w2_lora(act, batch)
         return out
 
 
@@ -446,53 +476,61 @@ class DecoderLayer(nn.Module):
         else:
             mlp_rank = cfg.lora_rank if "mlp" in cfg.lora_targets else 0
             self.ffn = DenseFFN(cfg.hidden_size, cfg.ffn_hidden_size, tp) if tp is not None \
-                else DenseFFN(cfg.hidden_size, cfg.ffn_hidden_size, None, mlp_rank, cfg.lora_alpha)
+                else DenseFFN(cfg.hidden_size, cfg.ffn_hidden_size, None, mlp_rank, cfg.lora_alpha, cfg.lora_dropout,
+                              (layer_idx + 1) * SITES)
         if tp is not None and tp.sequence_parallel:
             # the norms see this rank's part of every sequence only
             self.attn_norm.weight.tp_partial_grad = True
             self.ffn_norm.weight.tp_partial_grad = True
         self.recompute_ffn = False        # set by the engine for recompute_granularity=selective
+        self.dropout, self.offset = cfg.hidden_dropout, (layer_idx + 1) * SITES
 
-    def _ffn_block(self, y, h):
+    def _ffn_block(self, y, h, batch: BatchInfo | None = None):
         if self.tp is not None and self.is_moe and not self.tp.sequence_parallel and not self.expert_tp:
             # MoE under tensor parallelism: every rank of the group routes 1 / tp of the shared tokens through the
             # expert-parallel exchange, then the group reassembles the block's output
             shp = y.shape
             out = self.tp.gather_rows(self.ffn(self.tp.scatter_rows(y.reshape(-1, shp[-1]))))
             return h + out.reshape(shp)
-        return h + self.ffn(y)
+        out = self.ffn(y) if self.is_moe else self.ffn(y, batch)
+        return _dropout(out, self.dropout, batch, self.offset + SITE_FFN, residual=h)
 
-    def _ffn_block_aux(self, y, h):
+    def _ffn_block_aux(self, y, h, batch: BatchInfo | None = None):
         """The block plus the load-balancing loss its router produced, as a second output: inside a recomputed block
         the loss cannot leave through the module attribute (the first run builds no graph), so it travels through
         the recompute node like the block's output does."""
-        out = self._ffn_block(y, h)
+        out = self._ffn_block(y, h, batch)
         aux, self.ffn.aux = self.ffn.aux, None
         if aux is None:
             aux = torch.zeros((), dtype=torch.float32, device=out.device)
         return out, aux
 
-    def forward(self, x, cos, sin):
-        a = self.attn(self.attn_norm(x), cos, sin)
-        y, h = ops.rmsnorm_residual(a, x, self.ffn_norm.weight, self.eps)
+    def forward(self, x, cos, sin, batch: BatchInfo | None = None):
+        a = self.attn(self.attn_norm(x), cos, sin, batch)
+        if self.dropout > 0 and batch is not None and batch.seed is not None:
+            h = _dropout(a, self.dropout, batch, self.offset + SITE_ATTN, residual=x)
+            y = self.ffn_norm(h)
+        else:
+            y, h = ops.rmsnorm_residual(a, x, self.ffn_norm.weight, self.eps)
         if self.recompute_ffn and torch.is_grad_enabled():
             # selective recompute: attention activations are kept, the feed-forward block (for MoE layers the
             # dispatch, both grouped GEMMs and the combine) is re-run in backward
             if self.is_moe and self.ffn.aux_enabled():
-                out, aux = _Recompute.apply(self._ffn_block_aux, y, h)
+                out, aux = _Recompute.apply(partial(self._ffn_block_aux, batch=batch), y, h)
                 self.ffn.aux = aux            # picked up by the engine and added to the objective
                 return out
-            return _Recompute.apply(self._ffn_block, y, h)
-        return self._ffn_block(y, h)
+            return _Recompute.apply(partial(self._ffn_block, batch=batch), y, h)
+        return self._ffn_block(y, h, batch)
 
 
 class Embedding(nn.Module):
     def __init__(self, cfg: ModelConfig):
         super().__init__()
         self.weight = nn.Parameter(torch.empty(cfg.vocab_size, cfg.hidden_size))
+        self.scale, self.dropout = cfg.embedding_multiplier, cfg.hidden_dropout
 
-    def forward(self, tokens, dtype):
-        return F.embedding(tokens, self.weight).to(dtype)
+    def forward(self, tokens, dtype, batch: BatchInfo | None = None):
+        return _dropout(ops.embedding(tokens, self.weight, self.scale, dtype), self.dropout, batch, 0)
 
 
 class Head(nn.Module):
@@ -557,6 +595,15 @@ class SimpleMoE(nn.Module):
                                                     offset=self.cp_rank * seq_local)
         return self._rope_cache[key]
 
+    def batch_info(self, tokens, seed: int | None = None) -> BatchInfo | None:
+        """The micro-batch's documents (``reset_attention_mask``) and the seed of its dropout masks; None if the layers need
+        neither."""
+        cfg = self.cfg
+        documents = ops.documents_from_tokens(tokens, cfg.eod_token) if cfg.reset_attention_mask else None
+        if cfg.hidden_dropout <= 0 and cfg.lora_dropout <= 0:
+            seed = None
+        return BatchInfo(documents, seed) if documents is not None or seed is not None else None
+
     @torch.no_grad()
     def init_weights(self, seed: int) -> None:
         """N(0, init_method_std) for matrices, ones for norm gains.  Expert tensors are filled one
@@ -581,12 +628,14 @@ class SimpleMoE(nn.Module):
             parts[1] = str(self.layers[int(parts[1])].layer_idx)
         return ".".join(parts)
 
-    def forward(self, tokens_or_hidden, targets=None, dtype=torch.float32):
+    def forward(self, tokens_or_hidden, targets=None, dtype=torch.float32, batch: BatchInfo | None = None):
         """Plain (engine-less) forward for tests and small runs: tokens -> loss or hidden."""
-        x = self.embed(tokens_or_hidden, dtype) if self.embed is not None else tokens_or_hidden
+        if batch is None and self.embed is not None:
+            batch = self.batch_info(tokens_or_hidden)
+        x = self.embed(tokens_or_hidden, dtype, batch) if self.embed is not None else tokens_or_hidden
         cos, sin = self.rope_tables(x.shape[1], x.device)
         for layer in self.layers:
-            x = layer(x, cos, sin)
+            x = layer(x, cos, sin, batch)
         if self.head is None:
             return x
         return self.head(x, targets) if targets is not None else self.head.logits(x)

@@ -5,7 +5,9 @@ silent fallback.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
+import functools
 import os
 from pathlib import Path
 
@@ -111,6 +113,26 @@ def stream() -> int:
     if _raw_stream is not None and _raw_device is not None:
         return _raw_stream(_raw_device())
     return torch.cuda.current_stream().cuda_stream
+
+
+_HERE = contextlib.nullcontext()
+
+
+def on_device(t):
+    """Kernels run on the current device's stream: a context that makes the tensor's device the current one where it is not."""
+    i = t.device.index
+    return _HERE if i is None or i == torch.cuda.current_device() else torch.cuda.device(i)
+
+
+def first_order(fn):
+    """Backward of a Function whose gradients cannot be differentiated again: plain, unless a graph of the backward pass is
+    asked for, and then with an error in its place."""
+    guarded = torch.autograd.function.once_differentiable(fn)
+
+    @functools.wraps(fn)
+    def backward(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else fn(ctx, *grads)
+    return backward
 
 
 _STATUS = {}

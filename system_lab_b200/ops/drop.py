@@ -12,7 +12,6 @@ import torch
 
 from . import cuda
 from . import reference as ref
-from .packed import on_device
 
 cuda.register("slab_dropout", "pppililpls")
 
@@ -47,7 +46,7 @@ def _run(x, res, p, seed, offset):
     y = torch.empty_like(x)
     if x.numel():
         dev = seed if isinstance(seed, torch.Tensor) else None
-        with on_device(x):
+        with cuda.on_device(x):
             cuda.call("slab_dropout", x, res, y, int(x.dtype == torch.bfloat16), x.numel(), ref.dropout_threshold(p),
                       0 if dev is not None else _signed(seed), dev, _signed(offset), cuda.stream())
     return y
@@ -62,10 +61,11 @@ class _Dropout(torch.autograd.Function):
         return _run(x, residual, p, seed, offset)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         p, seed, offset = ctx.args
-        dx = _run(g, None, p, seed, offset) if ctx.needs_input_grad[0] else None
+        dx = None
+        if ctx.needs_input_grad[0]:                # the mask's product again, itself differentiable where that is asked for
+            dx = _Dropout.apply(g, None, p, seed, offset) if torch.is_grad_enabled() else _run(g, None, p, seed, offset)
         return dx, (g if ctx.needs_input_grad[1] else None), None, None, None
 
 

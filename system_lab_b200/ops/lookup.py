@@ -9,14 +9,18 @@ from __future__ import annotations
 import torch
 
 from . import cuda
-from .packed import on_device
 
 cuda.register("slab_embedding_fwd", "ppipiliifps")
-cuda.register("slab_embedding_chunk", "i")
-cuda.register("slab_embedding_bwd", "ppipippiiifis")
+cuda.register("slab_embedding_bwd", "ppipippiiiifis")
 cuda._KERNELS_PER_CALL["slab_embedding_bwd"] = 3
 
 _TYPES = (torch.float32, torch.bfloat16)
+
+
+def _chunk(rows: int) -> int:
+    """Sorted positions that one group of threads adds up: few where there are few, so that the SMs have work; no more than
+    32, so that a frequent token's run is shared by many."""
+    return 8 if rows <= 2048 else 16 if rows <= 16384 else 32
 
 
 def check(tokens, weight, scale) -> float:
@@ -43,7 +47,7 @@ class _Embedding(torch.autograd.Function):
             raise ValueError(f"{tok.numel()} tokens")
         out = torch.empty(*tokens.shape, h, dtype=dtype, device=w.device)
         if tok.numel():
-            with on_device(w):
+            with cuda.on_device(w):
                 cuda.call("slab_embedding_fwd", tok, w, int(w.dtype == torch.bfloat16), out, int(dtype == torch.bfloat16),
                           tok.numel(), v, h, scale, cuda.status_word(w.device), cuda.stream())
         ctx.save_for_backward(tok)
@@ -51,7 +55,7 @@ class _Embedding(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @cuda.first_order
     def backward(ctx, g):
         if not ctx.needs_input_grad[1]:
             return None, None, None, None
@@ -67,12 +71,13 @@ class _Embedding(torch.autograd.Function):
                 dw.zero_()
         else:
             g = g.contiguous()
-            with on_device(g):
-                chunk = cuda.lib().slab_embedding_chunk(rows)
-                order = torch.empty(rows + 1, dtype=torch.int32, device=g.device)
-                pieces = torch.empty((rows + chunk - 1) // chunk * 2 * h, dtype=torch.float32, device=g.device)
+            with cuda.on_device(g):
+                chunk = _chunk(rows)
+                at = (rows + 4) // 4 * 4                         # the sorted positions and their number, then the pieces
+                scratch = torch.empty(at + (rows + chunk - 1) // chunk * 2 * h, dtype=torch.int32, device=g.device)
+                base = scratch.data_ptr()
                 cuda.call("slab_embedding_bwd", tok, g, int(g.dtype == torch.bfloat16), dw, int(dw.dtype == torch.bfloat16),
-                          order, pieces, rows, v, h, ctx.scale, int(accumulate), cuda.stream())
+                          base, base + 4 * at, rows, chunk, v, h, ctx.scale, int(accumulate), cuda.stream())
         if into is not None:
             ctx.w_ref.main_grad_written = True
             return None, None, None, None

@@ -12,7 +12,6 @@ Reference: the packed fine-tuning batches of ``notes/mlperf-llama/2026-04-29_lla
 """
 from __future__ import annotations
 
-import contextlib
 import math
 
 import torch
@@ -57,11 +56,6 @@ def _plan_words(rows: int) -> int:
     return 2 * rows + 4 * tiles + (tiles + 1) // 2
 
 
-def on_device(t: torch.Tensor):
-    """Kernels run on the current device's stream: make the tensor's device the current one where it is not."""
-    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
-
-
 def pack_documents(cu_seqlens: torch.Tensor, rows: int) -> PackedDocuments:
     """Plan of ``rows`` rows that hold documents ``s`` at ``cu_seqlens[s] .. cu_seqlens[s + 1] - 1`` (starting at 0, not
     falling, documents may be empty; rows behind the last one belong to none).  Offsets on the GPU are checked there:
@@ -83,7 +77,7 @@ def pack_documents(cu_seqlens: torch.Tensor, rows: int) -> PackedDocuments:
         return PackedDocuments(rows, torch.cat([lo, hi]).int())
     cu = cu_seqlens.to(torch.int32).contiguous()
     plan = torch.empty(_plan_words(rows), dtype=torch.int32, device=cu.device)
-    with on_device(cu):
+    with cuda.on_device(cu):
         cuda.call("slab_packed_plan", cu, cu.numel() - 1, rows, plan, cuda.status_word(cu.device), cuda.stream())
     return PackedDocuments(rows, plan)
 
@@ -108,7 +102,7 @@ def documents_from_tokens(tokens: torch.Tensor, end_token: int) -> PackedDocumen
         return PackedDocuments(rows, torch.cat([lo, hi]).int())
     plan = torch.empty(_plan_words(rows), dtype=torch.int32, device=tok.device)
     starts = torch.empty(2 * ((rows + TILE - 1) // TILE), dtype=torch.int32, device=tok.device)
-    with on_device(tok):
+    with cuda.on_device(tok):
         cuda.call("slab_packed_plan_tokens", tok, rows, s, int(end_token), starts, plan, cuda.stream())
     return PackedDocuments(rows, plan)
 
@@ -158,7 +152,7 @@ def forward(q, k, v, documents: PackedDocuments, scale: float, window: int = 0):
     out = torch.empty((rows, hq, d), dtype=q.dtype, device=q.device)
     lse = torch.empty((hq, (rows + TILE - 1) // TILE * TILE), dtype=torch.float32, device=q.device)
     window = min(int(window), rows)
-    with on_device(q):
+    with cuda.on_device(q):
         cuda.call("slab_packed_attn_fwd", q, k, v, out, lse, documents.plan, rows, hq, k.shape[1], d, *_strides(q),
                   *_strides(k), *_strides(v), window, scale, cuda.status_word(q.device), cuda.stream())
     return out, lse
@@ -175,7 +169,7 @@ def backward(q, k, v, out, lse, dout, documents: PackedDocuments, scale: float, 
     dv = torch.empty_like(dk)
     delta = torch.empty_like(lse)
     window = min(int(window), rows)
-    with on_device(q):
+    with cuda.on_device(q):
         splits = cuda.lib().slab_packed_attn_splits(rows, hq, hkv)
         partial = torch.empty(splits * 2 * dk.numel(), dtype=torch.float32, device=q.device) if splits > 1 else None
         cuda.call("slab_packed_attn_bwd", q, k, v, out, dout, lse, documents.plan, dq, dk, dv, delta, partial, splits, rows,
@@ -196,7 +190,7 @@ class _PackedAttention(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @cuda.first_order
     def backward(ctx, g):
         q, k, v, out, lse = ctx.saved_tensors
         return backward(q, k, v, out, lse, g, ctx.documents, ctx.scale, ctx.window) + (None, None, None)

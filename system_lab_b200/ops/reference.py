@@ -61,6 +61,9 @@ def rope(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
 # ----------------------------------------------------------------------------
 def embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, dtype=None) -> torch.Tensor:
     """``scale * weight[tokens]``; the gradient adds up in the table's type or, where that is narrower, in fp32."""
+    if scale == 1.0:
+        out = F.embedding(tokens.long(), weight)
+        return out if dtype is None else out.to(dtype)
     w = weight.float() if weight.dtype in (torch.bfloat16, torch.float16) else weight
     return (F.embedding(tokens.long(), w) * scale).to(dtype if dtype is not None else weight.dtype)
 

@@ -291,8 +291,10 @@ class Engine:
     def run_unit(self, unit: Unit, x: torch.Tensor, *extra):
         return _UnitFn.apply(self.anchor, self, unit, x, *extra)
 
-    def stage_forward(self, inp: torch.Tensor, targets: torch.Tensor | None, chunk: int | None = None):
-        """First stage: ``inp`` are token ids ``[B, S]``; later stages: hidden ``[B, S, H]``.
+    def stage_forward(self, inp: torch.Tensor, targets: torch.Tensor | None, chunk: int | None = None,
+                      seed: int | None = None):
+        """First stage: ``inp`` are token ids ``[B, S]``; later stages: hidden ``[B, S, H]``.  ``seed``: of this
+        micro-batch's dropout masks (none in forward-only passes).
         Returns ``(output, aux_losses)`` where output is the scalar loss on the last stage.  ``chunk`` selects one
         of this rank's virtual pipeline stages (None: all local layers, the non-interleaved case)."""
         aux_all = []
@@ -300,10 +302,12 @@ class Engine:
         first_chunk = chunk is None or chunk == 0
         last_chunk = chunk is None or chunk == self.vpp - 1
         sp = self.tp.size if self.tp is not None and self.tp.sequence_parallel else 1
+        batch = None
         if self.embed_unit is not None and first_chunk:
+            batch = self.model.batch_info(x, None if self.inference else seed)
             if sp > 1:
                 x = self.tp.local_seq(x)          # every rank of the group got the same token ids
-            x = self.run_unit(self.embed_unit, x, self.compute_dtype)
+            x = self.run_unit(self.embed_unit, x, self.compute_dtype, batch)
         cos, sin = self.model.rope_tables(x.shape[1] * sp, x.device)     # attention sees whole sequences
         if chunk is None:
             units = self.layer_units
@@ -311,7 +315,7 @@ class Engine:
             per = len(self.layer_units) // self.vpp
             units = self.layer_units[chunk * per:(chunk + 1) * per]
         for u in units:
-            out = self.run_unit(u, x, cos, sin)
+            out = self.run_unit(u, x, cos, sin, batch)
             if isinstance(out, tuple):
                 x, aux = out
                 aux_all.append(aux)

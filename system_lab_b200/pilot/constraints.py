@@ -48,6 +48,22 @@ def check_config(cfg: Any, world_size: int | None = None) -> list[dict]:
             out.append(_p("lora_excludes_tp", "LoRA adapters are not combined with tensor parallelism"))
         if m.lora_targets not in ("attn", "attn+mlp"):
             out.append(_p("lora_targets", f"lora_targets={m.lora_targets!r}: use 'attn' or 'attn+mlp'"))
+    if m.reset_attention_mask:
+        # every stage's attention needs the batch's document boundaries, over whole sequences
+        if m.eod_token < 0 or m.eod_token >= m.vocab_size:
+            out.append(_p("packing_needs_eod", f"reset_attention_mask needs an eod_token in the vocabulary, not {m.eod_token}"))
+        if m.attention_type != "gqa":
+            out.append(_p("packing_needs_gqa", "reset_attention_mask is implemented for attention_type=gqa"))
+        if pp > 1 or cp > 1:
+            out.append(_p("packing_excludes_pp_cp", "reset_attention_mask is not combined with pipeline or context parallelism"))
+    for name in ("hidden_dropout", "lora_dropout"):
+        rate = getattr(m, name)
+        if not 0.0 <= rate <= 0.999:
+            out.append(_p("dropout_rate", f"{name}={rate}: has to be between 0 and 0.999"))
+        elif rate > 0 and (tp > 1 or pp > 1):
+            out.append(_p("dropout_excludes_tp_pp", f"{name} is not combined with tensor or pipeline parallelism"))
+    if m.lora_dropout > 0 and m.lora_rank == 0:
+        out.append(_p("lora_dropout_needs_rank", "lora_dropout needs lora_rank > 0"))
     if getattr(p, "sequence_parallel", False):
         if tp <= 1:
             out.append(_p("sp_needs_tp", "sequence_parallel needs tensor_model_parallel_size > 1",

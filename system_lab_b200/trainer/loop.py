@@ -12,6 +12,7 @@ tokens/s/GPU, lm loss, grad norm, NaN/skipped iterations, device memory.
 """
 from __future__ import annotations
 
+import hashlib
 import os
 
 import json
@@ -172,8 +173,8 @@ class Trainer:
             from ..parallel.pp import pipeline_1f1b
             loss_sum = pipeline_1f1b(self.engine, mesh, dev_batches, scale, cfg)
         else:
-            for tok, tgt in dev_batches:
-                loss, aux = self.engine.stage_forward(tok, tgt)
+            for i, (tok, tgt) in enumerate(dev_batches):
+                loss, aux = self.engine.stage_forward(tok, tgt, seed=self._dropout_seed(step, i))
                 total = loss * scale
                 for a in aux:
                     total = total + a * scale
@@ -201,6 +202,12 @@ class Trainer:
         if self.heartbeat is not None:
             self.heartbeat.beat(step)
         return {"loss": loss_mean, "grad_norm": grad_norm, "lr": lr, "status_any": status_any}
+
+    def _dropout_seed(self, step: int, micro: int) -> int:
+        """Seed of a micro-batch's dropout masks: a function of the run's seed, the step, the micro-batch and the rank (which
+        holds tokens of its own), so a resumed run draws what it would have drawn."""
+        h = hashlib.sha256(f"{self.cfg.train.seed}:{step}:{micro}:{self.mesh.rank}".encode()).digest()
+        return int.from_bytes(h[:8], "little")
 
     # ---- reading a step's numbers without stalling the launch of the next step -------------------------
     def begin_loss_read(self, out: dict):
@@ -268,8 +275,8 @@ class Trainer:
 
     @torch.no_grad()
     def evaluate(self, iters: int | None = None) -> float:
-        """Mean loss over ``iters`` held-out global batches (forward only, no dropout in this model family so no
-        mode switch is needed); identical on every rank."""
+        """Mean loss over ``iters`` held-out global batches (forward only; the engine gives such passes no dropout seed);
+        identical on every rank."""
         cfg, mesh, dev = self.cfg, self.mesh, self.device
         iters = iters if iters is not None else max(cfg.train.eval_iters, 1)
         offset = 0 if self.eval_data is not self.data else self.EVAL_STEP_OFFSET
