@@ -151,6 +151,7 @@ __global__ void packed_order_kernel(int rows, int* base) {
 
 // ================================================================ forward
 constexpr int PF_THREADS = 384;
+constexpr int PF_EVERY = 8;                   // of that many pairs of exponentials, one is made on the multiply-add units
 constexpr float PF_SLACK = 8.f;              // a row's maximum may be this far (log2) below the true one
 
 struct PackedFwdParams {
@@ -165,11 +166,13 @@ struct PackedFwdParams {
   int* status;
 };
 
+// A stage holds the V tile of a step and the K tile of the next one (of the next item, where the step is an item's last): they are
+// used in one go and freed together.
 template <int DP>
 struct PackedFwdSmem {
   static constexpr int TILE = PA_TILE * DP * 2;
-  static constexpr int STAGES = DP == 128 ? 5 : 8;         // key and value tiles in turn
-  static constexpr int Q_OFF = 1024, KV_OFF = Q_OFF + 2 * TILE, TOTAL = KV_OFF + STAGES * TILE;
+  static constexpr int STAGES = DP == 128 ? 2 : 4;
+  static constexpr int Q_OFF = 1024, KV_OFF = Q_OFF + 2 * TILE, TOTAL = KV_OFF + STAGES * 2 * TILE;
   static_assert(TOTAL <= 232448, "shared memory budget");
 };
 
@@ -238,6 +241,125 @@ __device__ __noinline__ void pf_redo(const PackedFwdParams& p, int row, int head
   if ((threadIdx.x & 31) == 0) p.lse[(size_t)head * padded + row] = pa_nan(inv) ? bad : m + log2f(l);
 }
 
+// A row's running sums come to a maximum that has grown by more than the slack.  All rows of a warp together.
+template <int DP>
+__device__ __forceinline__ void pf_raise(uint32_t o_addr, float top, float& m, float2& la, float2& lb) {
+  if (m == -INFINITY) m = top;                 // nothing has been added yet
+  const bool grow = top > m + PF_SLACK;
+  if (!__any_sync(0xffffffffu, grow)) return;
+  float alpha = 1.f;
+  if (grow) {
+    alpha = pa_exp2(m - top);
+    m = top;
+  }
+  la = pa_mul2(la, make_float2(alpha, alpha));
+  lb = pa_mul2(lb, make_float2(alpha, alpha));
+#pragma unroll 1
+  for (int c = 0; c < DP; c += 16) {
+    uint32_t o[16];
+    pa_tmem_ld_16(o_addr + c, o);
+    tmem_ld_wait();
+#pragma unroll
+    for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+    tmem_st_32x16(o_addr + c, o);
+  }
+}
+__device__ __forceinline__ void pf_arrive(uint64_t* bar) {
+  tmem_st_wait();
+  tc_fence_before();
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
+
+// One step of a row: scores to probabilities, which go back over them as bf16; p_full is told.  m:
+// maximum (log2 units) that the sums la + lb and the output are relative to.  This form: all rows of the warp see all keys.
+template <int DP>
+__device__ __forceinline__ void pf_whole(uint32_t s_addr, uint32_t o_addr, float scale_log2, float& m, float2& la, float2& lb,
+                                         uint64_t* p_full) {
+  float s[128];
+#pragma unroll
+  for (int c = 0; c < 128; c += 32) tmem_ld_32x32(s_addr + c, *reinterpret_cast<uint32_t(*)[32]>(&s[c]));
+  tmem_ld_wait();
+  float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+  for (int k = 4; k < 124; k += 8) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) mx[e] = pa_max3(mx[e], s[k + 2 * e], s[k + 2 * e + 1]);
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], s[124 + e]);
+  pf_raise<DP>(o_addr, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale_log2, m, la, lb);
+  const float base = m == -INFINITY ? 0.f : -m;
+  const float2 c2 = make_float2(scale_log2, scale_log2), b2 = make_float2(base, base);
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    uint32_t packed[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      float2 x = pa_fma2(make_float2(s[32 * c + 2 * k], s[32 * c + 2 * k + 1]), c2, b2);
+      if (k % PF_EVERY == PF_EVERY - 1) {
+        x = pa_exp2_fma(x);
+        lb = pa_add2(lb, x);
+      } else {
+        x.x = pa_exp2(x.x);
+        x.y = pa_exp2(x.y);
+        la = pa_add2(la, x);
+      }
+      packed[k] = pa_pack(x.x, x.y);
+    }
+    tmem_st_32x16(s_addr + c * 16, packed);
+  }
+  pf_arrive(p_full);
+}
+
+// The other form: a row sees keys first .. lastk (none where first > lastk); chunks of 32 that no row of the warp sees (not in
+// vis) are left out.  Two passes over the scores, a chunk at a time: few registers, short code.
+template <int DP>
+__device__ __forceinline__ void pf_part(uint32_t s_addr, uint32_t o_addr, float scale_log2, uint32_t vis, int first, int lastk,
+                                        float& m, float2& la, float2& lb, uint64_t* p_full) {
+  const uint32_t span = first > lastk ? 0u : (uint32_t)(lastk - first);
+  if (first > lastk) first = 1 << 20;
+  float top = -INFINITY;
+#pragma unroll 1
+  for (int c = 0; c < 4; ++c) {
+    if (!(vis >> c & 1u)) continue;
+    float s[32];
+    tmem_ld_32x32(s_addr + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
+    tmem_ld_wait();
+    float mx[2] = {top, -INFINITY};
+#pragma unroll
+    for (int k = 0; k < 32; k += 2)
+      mx[(k >> 1) & 1] = pa_max3(mx[(k >> 1) & 1], (uint32_t)(32 * c + k - first) <= span ? s[k] : -INFINITY,
+                                 (uint32_t)(32 * c + k + 1 - first) <= span ? s[k + 1] : -INFINITY);
+    top = fmaxf(mx[0], mx[1]);
+  }
+  pf_raise<DP>(o_addr, top * scale_log2, m, la, lb);
+  const float base = m == -INFINITY ? 0.f : -m;
+  const float2 c2 = make_float2(scale_log2, scale_log2), b2 = make_float2(base, base);
+#pragma unroll 1
+  for (int c = 0; c < 4; ++c) {
+    uint32_t packed[16];
+    if (vis >> c & 1u) {
+      float s[32];
+      tmem_ld_32x32(s_addr + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
+      tmem_ld_wait();
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        float2 x = pa_fma2(make_float2(s[2 * k], s[2 * k + 1]), c2, b2);
+        x.x = (uint32_t)(32 * c + 2 * k - first) <= span ? pa_exp2(x.x) : 0.f;
+        x.y = (uint32_t)(32 * c + 2 * k + 1 - first) <= span ? pa_exp2(x.y) : 0.f;
+        la = pa_add2(la, x);
+        packed[k] = pa_pack(x.x, x.y);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 16; ++k) packed[k] = 0u;
+    }
+    tmem_st_32x16(s_addr + c * 16, packed);    // (over scores that have been read)
+  }
+  pf_arrive(p_full);
+}
+
 template <int DP>
 __global__ void __launch_bounds__(PF_THREADS, 1)
 packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
@@ -293,9 +415,21 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   if (warp >= 8) {
     reg_dec<72>();
     if (warp == 9) {
-      // ------------------------------------------------------------ copies: Q, Q, then K, V, K, V ...
-      int pos = 0, done = 0;                   // tiles put into the ring, items before this one
+      // ------------------------------------------------------------ copies
+      int st = 0, done = 0;                    // stage, items before this one
+      uint32_t ph = 1;
       bool ok = true;
+      int v_row = -1, v_head = 0;              // V tile of the step before, the stage's other half
+      auto load_stage = [&](int k_row, int k_head) {             // (no K behind the last item's last step)
+        ok = ok && pa_wait(&kv_empty[st], ph, abort_flag, p.status, ST_PATTN_EMPTY);
+        if (ok && elect_one()) {
+          uint8_t* to = kv_s + st * 2 * L::TILE;
+          mbar_arrive_expect_tx(&kv_full[st], (v_row >= 0 ? L::TILE : 0) + (k_row >= 0 ? L::TILE : 0));
+          if (v_row >= 0) pa_load_tile<DP>(to, &map_v, &kv_full[st], v_head, v_row);
+          if (k_row >= 0) pa_load_tile<DP>(to + L::TILE, &map_k, &kv_full[st], k_head, k_row);
+        }
+        if (++st == NST) { st = 0; ph ^= 1; }
+      };
       for (int r = 0; ok; ++r) {
         const int idx = pa_item(r);
         if (r * (int)gridDim.x >= items) break;
@@ -303,97 +437,114 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         PackedFwdItem it = pf_item(p, plan, idx);
         pf_uniform(it);
         if (it.n == 0) continue;
-        auto load_q = [&](int g) {
-          ok = ok && mbar_wait_warp(&q_empty[g], (done & 1) ^ 1, abort_flag, p.status, ST_PATTN_EMPTY);
+        load_stage(it.j0 * PA_TILE, it.hk);
+        for (int g = 0; g < 2; ++g) {
+          ok = ok && pa_wait(&q_empty[g], (done & 1) ^ 1, abort_flag, p.status, ST_PATTN_EMPTY);
           if (ok && elect_one()) {
             mbar_arrive_expect_tx(&q_full[g], L::TILE);
             pa_load_tile<DP>(q_s + g * L::TILE, &map_q, &q_full[g], it.head[g], it.row[g]);
           }
-        };
-        auto load_kv = [&](const CUtensorMap* map, int j) {
-          const int s = pos % NST;
-          ok = ok && mbar_wait_warp(&kv_empty[s], ((pos / NST) & 1) ^ 1, abort_flag, p.status, ST_PATTN_EMPTY);
-          if (ok && elect_one()) {
-            mbar_arrive_expect_tx(&kv_full[s], L::TILE);
-            pa_load_tile<DP>(kv_s + s * L::TILE, map, &kv_full[s], it.hk, j * PA_TILE);
-          }
-          ++pos;
-        };
-        load_q(0);
-        load_kv(&map_k, it.j0);
-        load_q(1);
+        }
+        v_head = it.hk;
         for (int i = 0; ok && i < it.n; ++i) {
-          load_kv(&map_v, it.j0 + i);
-          if (i + 1 < it.n) load_kv(&map_k, it.j0 + i + 1);
+          v_row = (it.j0 + i) * PA_TILE;
+          if (i + 1 < it.n) load_stage(v_row + PA_TILE, it.hk);
         }
         ++done;
       }
+      if (ok && v_row >= 0) load_stage(-1, 0);
     } else if (warp == 8) {
       // ------------------------------------------------------------ MMAs
       constexpr uint32_t idesc_qk = make_idesc(1, 1, 0, 0, PA_TILE, PA_TILE);
       constexpr uint32_t idesc_pv = make_idesc(1, 1, 0, 1, PA_TILE, DP);
-      const uint64_t qd = make_smem_desc(smem_u32(q_s), 16, 1024, 2);
-      const uint64_t kd = make_smem_desc(smem_u32(kv_s), 16, 1024, 2);
-      const uint64_t vd = make_smem_desc(smem_u32(kv_s), 16384, 1024, 2);     // the same bytes, key rows as the reduction
       constexpr uint32_t STEP = L::TILE >> 4;
-      int r = 0, left = 0;                     // steps of the item whose scores were issued last that are still to issue
-      int n_item = 0, items_seen = 0, step = 0;
-      bool ok = true, more = true;
-      auto next_item = [&]() {                 // length of the next item that has keys; more = false behind the last
-        while (true) {
-          if (r * (int)gridDim.x >= items) { more = false; return; }
+      const uint64_t qd = make_smem_desc(smem_u32(q_s), 16, 1024, 2);
+      const uint64_t vd = make_smem_desc(smem_u32(kv_s), 16384, 1024, 2);               // key rows as the reduction
+      const uint64_t kd = make_smem_desc(smem_u32(kv_s + L::TILE), 16, 1024, 2);
+      int r = 0;
+      auto next_len = [&]() {                  // key tiles of the next item that has any, 0 behind the last
+        while (r * (int)gridDim.x < items) {
           const int idx = pa_item(r++);
           if (idx >= items) continue;
           const int n = warp_uniform(pf_item(p, plan, idx).n);
-          if (n > 0) { left = n; n_item = n; ++items_seen; return; }
+          if (n > 0) return n;
         }
+        return 0;
       };
-      // ring positions: K of step s at 2 s, V at 2 s + 1
-      auto wait_tile = [&](int pos) {
-        ok = ok && mbar_wait_warp(&kv_full[pos % NST], (pos / NST) & 1, abort_flag, p.status, ST_PATTN_KV_FULL);
-      };
-      auto scores = [&](int g, int st) {       // scores of step st for tile g
-        if (g == 0) wait_tile(2 * st);
-        if (left == n_item) ok = ok && mbar_wait_warp(&q_full[g], (items_seen - 1) & 1, abort_flag, p.status, ST_PATTN_Q);
-        if (!ok) return;
-        tc_fence_after();
-        const int s = (2 * st) % NST;
-        if (elect_one()) {
-          pa_mma_ss<DP>(tmem + g * 128, qd + g * STEP, kd + s * STEP, idesc_qk);
-          umma_commit(&s_full[g]);
-          if (g == 1) umma_commit(&kv_empty[s]);
-          if (left == 1) umma_commit(&q_empty[g]);
-        }
-      };
-      next_item();
-      if (more) {
-        scores(0, 0);
-        scores(1, 0);
-      }
-      int i = 0, n = n_item;                   // the step whose P V comes next, of n
-      while (ok && more) {
-        // what follows this step: the item's next one, or the first of the next item
-        const bool last = i == n - 1;
-        --left;
-        if (last) next_item();
+      // This warp's own instructions bound a step once its waits (some 250 cycles each beside the softmax warps) follow one
+      // another: what the next step needs is waited for and counted up before the second tile's probabilities are.  (Stages
+      // and parities are counted, not computed: what the issued instructions take has to be plainly the same in all lanes,
+      // see elect_one.)
+      int st = 0;
+      uint32_t ph = 0, pph = 0, qph = 0;
+      int n = next_len(), i = 0;               // the step whose P V comes next: i of n
+      bool ok = true;
+      bool last = n == 1;
+      int after = last ? next_len() : n;       // length of the item that the step behind it belongs to
+      if (n > 0) {                             // scores of the first step
+        ok = pa_wait(&kv_full[0], 0, abort_flag, p.status, ST_PATTN_KV_FULL);
+#pragma unroll
         for (int g = 0; g < 2; ++g) {
-          ok = ok && mbar_wait_warp(&p_full[g], step & 1, abort_flag, p.status, ST_PATTN_P);
-          if (g == 0) wait_tile(2 * step + 1);
+          ok = ok && pa_wait(&q_full[g], 0, abort_flag, p.status, ST_PATTN_Q);
           if (!ok) break;
           tc_fence_after();
-          const int s = (2 * step + 1) % NST;
           if (elect_one()) {
-#pragma unroll
-            for (int kk = 0; kk < PA_TILE / 16; ++kk)
-              umma_f16_ts(tmem + 256 + g * 128, tmem + g * 128 + kk * 8, vd + s * STEP + kk * (2048 >> 4), idesc_pv,
-                          (i | kk) != 0 ? 1u : 0u);
-            if (last) umma_commit(&o_full[g]);
-            if (g == 1) umma_commit(&kv_empty[s]);
+            pa_mma_ss<DP>(tmem + g * 128, qd + g * STEP, kd, idesc_qk);
+            umma_commit(&s_full[g]);
+            if (g == 1) umma_commit(&kv_empty[0]);
+            if (last) umma_commit(&q_empty[g]);
           }
-          if (!last || more) scores(g, step + 1);
         }
-        ++step;
-        if (last) { i = 0; n = n_item; } else ++i;
+        qph = 1;
+        st = 1 % NST;
+        if (st == 0) ph ^= 1;
+        ok = ok && pa_wait(&kv_full[st], ph, abort_flag, p.status, ST_PATTN_KV_FULL);
+      }
+      while (ok && n > 0) {
+        const bool more = after > 0, was = last;
+        const bool ends = last ? after == 1 : i + 2 == n;        // whether the next step is its item's last
+        const uint64_t v0 = vd + (uint32_t)(st * 2 * STEP), k0 = kd + (uint32_t)(st * 2 * STEP);
+        const uint32_t fresh = i != 0 ? 1u : 0u;
+        const int s0 = st;
+        if (more && last) ok = pa_wait(&q_full[0], qph, abort_flag, p.status, ST_PATTN_Q);
+        ok = ok && pa_wait(&p_full[0], pph, abort_flag, p.status, ST_PATTN_P);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int k4 = 0; k4 < 8; ++k4)
+            umma_f16_ts(tmem + 256, tmem + k4 * 8, v0 + k4 * (2048 >> 4), idesc_pv, k4 != 0 ? 1u : fresh);
+          if (was) umma_commit(&o_full[0]);
+          if (more) {
+            pa_mma_ss<DP>(tmem, qd, k0, idesc_qk);
+            umma_commit(&s_full[0]);
+            if (ends) umma_commit(&q_empty[0]);
+          }
+        }
+        if (more && last) ok = pa_wait(&q_full[1], qph, abort_flag, p.status, ST_PATTN_Q);
+        if (last) qph ^= 1;
+        i = last ? 0 : i + 1;
+        n = after;
+        last = i == n - 1;
+        after = last ? next_len() : n;
+        if (++st == NST) { st = 0; ph ^= 1; }
+        if (n > 0) ok = ok && pa_wait(&kv_full[st], ph, abort_flag, p.status, ST_PATTN_KV_FULL);
+        ok = ok && pa_wait(&p_full[1], pph, abort_flag, p.status, ST_PATTN_P);
+        pph ^= 1;
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int k4 = 0; k4 < 8; ++k4)
+            umma_f16_ts(tmem + 384, tmem + 128 + k4 * 8, v0 + k4 * (2048 >> 4), idesc_pv, k4 != 0 ? 1u : fresh);
+          if (was) umma_commit(&o_full[1]);
+          if (more) {
+            pa_mma_ss<DP>(tmem + 128, qd + STEP, k0, idesc_qk);
+            umma_commit(&s_full[1]);
+            if (ends) umma_commit(&q_empty[1]);
+          }
+          umma_commit(&kv_empty[s0]);
+        }
       }
     }
   } else {
@@ -419,79 +570,32 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       }
       const bool sees = lo <= row;
       float m = -INFINITY;                     // maximum (log2 units) that the sums are relative to
-      float2 l2 = make_float2(0.f, 0.f);
+      float2 la = make_float2(0.f, 0.f), lb = la;
       for (int i = 0; i < it.n; ++i, ++step) {
         const int kv0 = (it.j0 + i) * PA_TILE;
-        ok = mbar_wait_warp(&s_full[g], step & 1, abort_flag, p.status, ST_PATTN_S);
+        ok = pa_wait(&s_full[g], step & 1, abort_flag, p.status, ST_PATTN_S);
         if (!ok) break;
         tc_fence_after();
-        float s[128];
+        // keys first .. lastk of this tile are visible to this row
+        const int first = max(lo - kv0, 0), lastk = sees ? min(row - kv0, 127) : -1;
+        uint32_t vis = 0u;                     // 32-key chunks of the tile that some row of the warp sees
+        const bool part = __any_sync(0xffffffffu, first > 0 || lastk < 127);
+        if (part) {
+          const bool none = first > lastk;
+          const int from = __reduce_min_sync(0xffffffffu, none ? 128 : first), to = __reduce_max_sync(0xffffffffu, none ? -1 : lastk);
 #pragma unroll
-        for (int c = 0; c < 128; c += 32) tmem_ld_32x32(s_addr + c, *reinterpret_cast<uint32_t(*)[32]>(&s[c]));
-        tmem_ld_wait();
-        // keys first .. first + span of this tile are visible
-        int first = max(lo - kv0, 0);
-        const int lastk = min(row - kv0, 127);
-        const bool part = !sees || first > 0 || lastk < 127;
-        if (__any_sync(0xffffffffu, part)) {
-          const bool none = !sees || first > lastk;
-          if (none) first = 1 << 20;
-          const uint32_t span = none ? 0u : (uint32_t)(lastk - first);
-#pragma unroll
-          for (int c = 0; c < 128; ++c) s[c] = (uint32_t)(c - first) <= span ? s[c] : -INFINITY;
+          for (int c = 0; c < 4; ++c) vis |= from <= 32 * c + 31 && to >= 32 * c ? 1u << c : 0u;
         }
-        float mx[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-        for (int c = 4; c < 128; c += 8) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], c + 4 + k < 128 ? fmaxf(s[c + k], s[c + 4 + k]) : s[c + k]);
-        }
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
-        if (m == -INFINITY) m = top;           // nothing has been added yet: no product to bring to this maximum
-        const float old = m;
-        const bool grow = top > m + PF_SLACK;
-        if (__any_sync(0xffffffffu, grow)) {
-          float alpha = 1.f;
-          if (grow) {
-            alpha = pa_exp2(old - top);
-            m = top;
-          }
-          l2 = pa_mul2(l2, make_float2(alpha, alpha));
-#pragma unroll
-          for (int c = 0; c < DP; c += 32) {
-            uint32_t o[32];
-            tmem_ld_32x32(o_addr + c, o);
-            tmem_ld_wait();
-#pragma unroll
-            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
-            tmem_st_32x32(o_addr + c, o);
-          }
-        }
-        const float base = m == -INFINITY ? 0.f : -m;
-        const float2 c2 = make_float2(p.scale_log2, p.scale_log2), b2 = make_float2(base, base);
-#pragma unroll
-        for (int c = 0; c < 128; c += 32) {
-          uint32_t packed[16];
-#pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            float2 x = pa_fma2(make_float2(s[c + 2 * k], s[c + 2 * k + 1]), c2, b2);
-            x.x = pa_exp2(x.x);
-            x.y = pa_exp2(x.y);
-            l2 = pa_add2(l2, x);
-            packed[k] = pa_pack(x.x, x.y);
-          }
-          tmem_st_32x16(s_addr + c / 2, packed);
-        }
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[g]);
+        if (!part)
+          pf_whole<DP>(s_addr, o_addr, p.scale_log2, m, la, lb, &p_full[g]);
+        else
+          pf_part<DP>(s_addr, o_addr, p.scale_log2, vis, first, lastk, m, la, lb, &p_full[g]);
       }
       if (!ok) break;
-      const float l = l2.x + l2.y;
+      const float l = (la.x + la.y) + (lb.x + lb.y);
       const float inv = 1.f / l;               // (a row that sees nothing gets zeros)
       if (it.n > 0) {
-        ok = mbar_wait_warp(&o_full[g], done & 1, abort_flag, p.status, ST_PATTN_OUT);
+        ok = pa_wait(&o_full[g], done & 1, abort_flag, p.status, ST_PATTN_OUT);
         if (!ok) break;
         tc_fence_after();
         ++done;

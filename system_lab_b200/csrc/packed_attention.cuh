@@ -78,11 +78,25 @@ __device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&r
       "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
+__device__ __forceinline__ void pa_tmem_ld_16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void reg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
 __device__ __forceinline__ void reg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// mbar_wait_warp, shorter where the barrier has completed already
+__device__ __forceinline__ bool pa_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  return mbar_wait_warp(bar, parity, abort_flag, status, code);
+}
 
 __device__ __forceinline__ uint32_t pa_pack(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
@@ -147,6 +161,30 @@ __device__ __forceinline__ void pa_put4(__nv_bfloat16* to, int d, const float4& 
 }
 __device__ __forceinline__ bool pa_finite(float v) { return (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u; }
 __device__ __forceinline__ bool pa_nan(float v) { return (__float_as_uint(v) & 0x7fffffffu) > 0x7f800000u; }
+
+// Largest of three in one instruction
+__device__ __forceinline__ float pa_max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// 2^x for two numbers on the multiply-add units: x = n + f with n whole (adding 1.5 * 2^23 rounds it into the mantissa's low
+// bits) and |f| <= 1/2; a cubic in f, fitted to 2^f for the least largest relative error (7.5e-5; probabilities are then
+// rounded to bf16, 3.9e-3); n goes into the exponent.  Below -126 the result is 2^-126: only for
+// keys that are seen, never for masked ones, whose probability has to be zero.
+__device__ __forceinline__ float2 pa_exp2_fma(float2 x) {
+  const float2 magic = make_float2(12582912.f, 12582912.f);
+  x.x = fmaxf(x.x, -126.f);
+  x.y = fmaxf(x.y, -126.f);
+  const float2 t = pa_add2(x, magic);
+  const float2 n = pa_add2(t, make_float2(-12582912.f, -12582912.f));
+  const float2 f = pa_fma2(n, make_float2(-1.f, -1.f), x);
+  float2 p = pa_fma2(f, make_float2(0.05517167f, 0.05517167f), make_float2(0.24261113f, 0.24261113f));
+  p = pa_fma2(p, f, make_float2(0.69326097f, 0.69326097f));
+  p = pa_fma2(p, f, make_float2(0.99992806f, 0.99992806f));
+  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
+                     __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
+}
 
 // Tile of 128 rows x DP columns of one head, as boxes of 64 columns ([128 rows][128 bytes], 128-byte swizzle).  Columns at
 // or beyond the head's width and rows at or beyond the buffer's end read as zero.

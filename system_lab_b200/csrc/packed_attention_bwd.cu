@@ -240,7 +240,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       int pos = 0, done = 0;
       bool ok = true;
       auto load = [&](uint8_t* dst, const CUtensorMap* map, uint64_t* full, uint64_t* empty, uint32_t parity, int head, int row) {
-        ok = ok && mbar_wait_warp(empty, parity, abort_flag, p.status, ST_PATTN_EMPTY);
+        ok = ok && pa_wait(empty, parity, abort_flag, p.status, ST_PATTN_EMPTY);
         if (ok && elect_one()) {
           mbar_arrive_expect_tx(full, L::TILE);
           pa_load_tile<DP>(dst, map, full, head, row);
@@ -272,58 +272,75 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         while (r * (int)gridDim.x < items) {
           const int idx = pa_item(r++);
           if (idx >= items) continue;
-          const int n = pb_dq_item(p, plan, idx).n;
+          const int n = warp_uniform(pb_dq_item(p, plan, idx).n);
           if (n > 0) return n;
         }
         return 0;
       };
-      StepWalk<decltype(lens)> ws(lens), wp(lens), wq(lens);                  // scores run two steps ahead, dP one
+      // Scores run two steps ahead, dP one; each walk counts its item's steps, stages and parities (counted, not computed: see
+      // elect_one).  What a product needs beside ds is waited for while others run.
+      StepWalk<decltype(lens)> ws(lens), wp(lens), wq(lens);
+      int sk = 0, sq = 0, sv = 0;              // stages of K for the scores, of K for dq, of V
+      uint32_t kph = 0, vph = 0, buf = 0, qbuf = 0, dsph = 0;
       auto scores = [&]() {
         if (!ok || !ws.more) return;
-        const int s = ws.step % KST;
-        ok = mbar_wait_warp(&k_full[s], (ws.step / KST) & 1, abort_flag, p.status, ST_PATTN_KV_FULL);
-        if (ws.first()) ok = ok && mbar_wait_warp(q_full, ws.item_parity(), abort_flag, p.status, ST_PATTN_Q);
+        ok = pa_wait(&k_full[sk], kph, abort_flag, p.status, ST_PATTN_KV_FULL);
+        if (ws.first()) ok = ok && pa_wait(q_full, ws.item_parity(), abort_flag, p.status, ST_PATTN_Q);
         if (!ok) return;
         tc_fence_after();
+        const uint64_t k0 = kd + (uint32_t)(sk * STEP);
+        const uint32_t to = tmem + buf * 128;
         if (elect_one()) {
-          pa_mma_ss<DP>(tmem + (ws.step & 1) * 128, qd, kd + s * STEP, idesc_s);
-          umma_commit(&s_full[ws.step & 1]);
+          pa_mma_ss<DP>(to, qd, k0, idesc_s);
+          umma_commit(&s_full[buf]);
           if (ws.last()) umma_commit(q_empty);
         }
         ws.advance();
+        buf ^= 1;
+        if (++sk == KST) { sk = 0; kph ^= 1; }
+      };
+      auto need_v = [&]() {                    // V of the next dP (and its item's dO)
+        if (!ok || !wp.more) return;
+        ok = pa_wait(&v_full[sv], vph, abort_flag, p.status, ST_PATTN_KV_FULL);
+        if (wp.first()) ok = ok && pa_wait(do_full, wp.item_parity(), abort_flag, p.status, ST_PATTN_Q);
       };
       auto dprob = [&]() {
         if (!ok || !wp.more) return;
-        const int s = wp.step % VST;
-        ok = mbar_wait_warp(&v_full[s], (wp.step / VST) & 1, abort_flag, p.status, ST_PATTN_KV_FULL);
-        if (wp.first()) ok = ok && mbar_wait_warp(do_full, wp.item_parity(), abort_flag, p.status, ST_PATTN_Q);
-        if (!ok) return;
-        tc_fence_after();
+        const uint64_t v0 = vd + (uint32_t)(sv * STEP);
         if (elect_one()) {
-          pa_mma_ss<DP>(tmem + 256, dod, vd + s * STEP, idesc_s);
+          pa_mma_ss<DP>(tmem + 256, dod, v0, idesc_s);
           umma_commit(dp_full);
-          umma_commit(&v_empty[s]);
+          umma_commit(&v_empty[sv]);
           if (wp.last()) umma_commit(do_empty);
         }
         wp.advance();
+        if (++sv == VST) { sv = 0; vph ^= 1; }
       };
       scores();
+      need_v();
+      tc_fence_after();
       dprob();
       scores();
+      need_v();
       while (ok && wq.more) {
-        ok = mbar_wait_warp(ds_full, wq.step & 1, abort_flag, p.status, ST_PATTN_P);
-        if (!ok) break;
-        dprob();                               // the softmax has read dP
+        ok = pa_wait(ds_full, dsph, abort_flag, p.status, ST_PATTN_P);
         if (!ok) break;
         tc_fence_after();
-        const int s = wq.step % KST;
+        dprob();                               // first: the softmax has read dP and wants the next one soonest
+        const uint64_t k0 = kt + (uint32_t)(sq * STEP);
+        const uint32_t from = tmem + qbuf * 128;
+        const bool add = !wq.first();
         if (elect_one()) {
-          pb_mma_ts<DP>(tmem + 384, tmem + (wq.step & 1) * 128, kt + s * STEP, idesc_d, !wq.first());
-          umma_commit(&k_empty[s]);
+          pb_mma_ts<DP>(tmem + 384, from, k0, idesc_d, add);
+          umma_commit(&k_empty[sq]);
           if (wq.last()) umma_commit(dq_full);
         }
-        wq.advance();
         scores();
+        need_v();
+        wq.advance();
+        dsph ^= 1;
+        qbuf ^= 1;
+        if (++sq == KST) sq = 0;
       }
     }
   } else {
@@ -348,7 +365,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       const float2 c2 = make_float2(p.scale_log2, p.scale_log2), b2 = make_float2(nlse, nlse), d2 = make_float2(-delta, -delta);
       for (int i = 0; i < it.n; ++i, ++step) {
         const int c0 = (it.j0 + i) * PA_TILE + g * 64;         // first key of this thread's columns
-        ok = mbar_wait_warp(&s_full[step & 1], (step >> 1) & 1, abort_flag, p.status, ST_PATTN_S);
+        ok = pa_wait(&s_full[step & 1], (step >> 1) & 1, abort_flag, p.status, ST_PATTN_S);
         if (!ok) break;
         tc_fence_after();
         const uint32_t s_addr = base + (step & 1) * 128 + g * 64;
@@ -368,7 +385,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         const uint32_t span = none ? 0u : (uint32_t)(lastk - first);
         const bool masked = __any_sync(0xffffffffu, part);
         if (masked) pb_mask(s, first, span);
-        ok = mbar_wait_warp(dp_full, step & 1, abort_flag, p.status, ST_PATTN_S);
+        ok = pa_wait(dp_full, step & 1, abort_flag, p.status, ST_PATTN_S);
         if (!ok) break;
         tc_fence_after();
         float t[64];
@@ -387,7 +404,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       }
       if (!ok) break;
       if (it.n > 0) {
-        ok = mbar_wait_warp(dq_full, done & 1, abort_flag, p.status, ST_PATTN_OUT);
+        ok = pa_wait(dq_full, done & 1, abort_flag, p.status, ST_PATTN_OUT);
         if (!ok) break;
         tc_fence_after();
         ++done;
@@ -539,7 +556,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       bool ok = true;
       auto load = [&](uint8_t* dst, const CUtensorMap* map, uint64_t* full, uint64_t* empty, uint32_t parity, int head, int row,
                       float* stat_dst, const float* stat) {
-        ok = ok && mbar_wait_warp(empty, parity, abort_flag, p.status, ST_PATTN_EMPTY);
+        ok = ok && pa_wait(empty, parity, abort_flag, p.status, ST_PATTN_EMPTY);
         if (ok && elect_one()) {
           mbar_arrive_expect_tx(full, L::TILE + (stat ? PA_TILE * 4 : 0));
           pa_load_tile<DP>(dst, map, full, head, row);
@@ -575,34 +592,37 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         while (r * (int)gridDim.x < items) {
           const int idx = pa_item(r++);
           if (idx >= items) continue;
-          const int n = pb_dkv_item(p, plan, idx).n;
+          const int n = warp_uniform(pb_dkv_item(p, plan, idx).n);
           if (n > 0) return n;
         }
         return 0;
       };
+      // (stages and parities are counted, not computed: see elect_one)
       StepWalk<decltype(lens)> w(lens);        // the step whose scores and dP come next
+      int sa = 0, sb = 0;                      // stage of that step, of the one before
+      uint32_t ph = 0, par = 0;
       auto scores = [&]() {
         if (!ok || !w.more) return;
-        const int s = w.step % ST;
-        ok = mbar_wait_warp(&q_full[s], (w.step / ST) & 1, abort_flag, p.status, ST_PATTN_Q);
-        if (w.first()) ok = ok && mbar_wait_warp(k_full, w.item_parity(), abort_flag, p.status, ST_PATTN_KV_FULL);
+        ok = pa_wait(&q_full[sa], ph, abort_flag, p.status, ST_PATTN_Q);
+        if (w.first()) ok = ok && pa_wait(k_full, w.item_parity(), abort_flag, p.status, ST_PATTN_KV_FULL);
         if (!ok) return;
         tc_fence_after();
+        const uint64_t q0 = qd + (uint32_t)(sa * STEP);
         if (elect_one()) {
-          pa_mma_ss<DP>(tmem, kd, qd + s * STEP, idesc_s);
+          pa_mma_ss<DP>(tmem, kd, q0, idesc_s);
           umma_commit(s_full);
           if (w.last()) umma_commit(k_empty);
         }
       };
       auto dprob = [&]() {
         if (!ok || !w.more) return;
-        const int s = w.step % ST;
-        ok = mbar_wait_warp(&do_full[s], (w.step / ST) & 1, abort_flag, p.status, ST_PATTN_Q);
-        if (w.first()) ok = ok && mbar_wait_warp(v_full, w.item_parity(), abort_flag, p.status, ST_PATTN_KV_FULL);
+        ok = pa_wait(&do_full[sa], ph, abort_flag, p.status, ST_PATTN_Q);
+        if (w.first()) ok = ok && pa_wait(v_full, w.item_parity(), abort_flag, p.status, ST_PATTN_KV_FULL);
         if (!ok) return;
         tc_fence_after();
+        const uint64_t d0 = dod + (uint32_t)(sa * STEP);
         if (elect_one()) {
-          pa_mma_ss<DP>(tmem + 128, vd, dod + s * STEP, idesc_s);
+          pa_mma_ss<DP>(tmem + 128, vd, d0, idesc_s);
           umma_commit(dp_full);
           if (w.last()) umma_commit(v_empty);
         }
@@ -610,27 +630,29 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       scores();
       dprob();
       while (ok && w.more) {
-        const int s = w.step % ST;
-        const uint32_t parity = w.step & 1;
-        const bool first = w.first(), last = w.last();
+        const bool add = !w.first(), last = w.last();
         w.advance();                           // now at the step behind this one
-        ok = mbar_wait_warp(p_full, parity, abort_flag, p.status, ST_PATTN_P);
+        sb = sa;
+        if (++sa == ST) { sa = 0; ph ^= 1; }
+        const uint64_t d0 = dot + (uint32_t)(sb * STEP), q0 = qt + (uint32_t)(sb * STEP);
+        ok = pa_wait(p_full, par, abort_flag, p.status, ST_PATTN_P);
         if (!ok) break;
         tc_fence_after();
         if (elect_one()) {
-          pb_mma_ts<DP>(tmem + 256, tmem, dot + s * STEP, idesc_d, !first);
-          umma_commit(&do_empty[s]);
+          pb_mma_ts<DP>(tmem + 256, tmem, d0, idesc_d, add);
+          umma_commit(&do_empty[sb]);
         }
         scores();
-        ok = ok && mbar_wait_warp(ds_full, parity, abort_flag, p.status, ST_PATTN_P);
+        ok = ok && pa_wait(ds_full, par, abort_flag, p.status, ST_PATTN_P);
         if (!ok) break;
         tc_fence_after();
         if (elect_one()) {
-          pb_mma_ts<DP>(tmem + 384, tmem + 128, qt + s * STEP, idesc_d, !first);
-          umma_commit(&q_empty[s]);
+          pb_mma_ts<DP>(tmem + 384, tmem + 128, q0, idesc_d, add);
+          umma_commit(&q_empty[sb]);
           if (last) umma_commit(out_full);
         }
         dprob();
+        par ^= 1;
       }
     }
   } else {
@@ -656,8 +678,8 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         if (++t == it.tiles) t = 0;
         const int slot = step % ST;
         const uint32_t slot_parity = (step / ST) & 1;
-        ok = mbar_wait_warp(s_full, step & 1, abort_flag, p.status, ST_PATTN_S) &&
-             mbar_wait_warp(&q_full[slot], slot_parity, abort_flag, p.status, ST_PATTN_Q);
+        ok = pa_wait(s_full, step & 1, abort_flag, p.status, ST_PATTN_S) &&
+             pa_wait(&q_full[slot], slot_parity, abort_flag, p.status, ST_PATTN_Q);
         if (!ok) break;
         tc_fence_after();
         float s[64];
@@ -684,8 +706,8 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(p_full);
-        ok = mbar_wait_warp(dp_full, step & 1, abort_flag, p.status, ST_PATTN_S) &&
-             mbar_wait_warp(&do_full[slot], slot_parity, abort_flag, p.status, ST_PATTN_Q);
+        ok = pa_wait(dp_full, step & 1, abort_flag, p.status, ST_PATTN_S) &&
+             pa_wait(&do_full[slot], slot_parity, abort_flag, p.status, ST_PATTN_Q);
         if (!ok) break;
         tc_fence_after();
         float u[64];
@@ -709,7 +731,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       }
       if (!ok) break;
       if (it.n > 0) {
-        ok = mbar_wait_warp(out_full, done & 1, abort_flag, p.status, ST_PATTN_OUT);
+        ok = pa_wait(out_full, done & 1, abort_flag, p.status, ST_PATTN_OUT);
         if (!ok) break;
         tc_fence_after();
         ++done;
