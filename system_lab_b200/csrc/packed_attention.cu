@@ -163,6 +163,7 @@ struct PackedFwdParams {
   int window;              // 0: whole document
   int head_pairs;          // two heads of a group share a block, else two tiles of rows
   float scale_log2;        // softmax scale * log2(e)
+  int* counter;            // items taken behind the first of every block, zero at launch
   int* status;
 };
 
@@ -179,23 +180,24 @@ struct PackedFwdSmem {
 struct PackedFwdItem {
   int row[2], head[2], hk;
   int j0, n;               // first key tile, key tiles
+  __device__ __forceinline__ explicit PackedFwdItem(const PaItem& i)
+      : row{i.v[0], i.v[1]}, head{i.v[2], i.v[3]}, hk(i.v[4]), j0(i.v[5]), n(i.v[7]) {}
 };
-__device__ __forceinline__ PackedFwdItem pf_item(const PackedFwdParams& p, const PackedPlan& plan, int idx) {
-  PackedFwdItem it;
+__device__ __forceinline__ PaItem pf_item(const PackedFwdParams& p, const PackedPlan& plan, int idx) {
   const int tiles = (p.rows + PA_TILE - 1) / PA_TILE;
-  int lo, last;
+  int lo, last, row0, row1, head0, head1;
   if (p.head_pairs) {
     const int hp = p.Hq >> 1, o = idx / hp, t = plan.q_order[o];
-    it.head[0] = 2 * (idx - o * hp);
-    it.head[1] = it.head[0] + 1;
-    it.row[0] = it.row[1] = t * PA_TILE;
+    head0 = 2 * (idx - o * hp);
+    head1 = head0 + 1;
+    row0 = row1 = t * PA_TILE;
     lo = plan.tile_lo[t];
     last = t;
   } else {
     const int o = idx / p.Hq, t = 2 * plan.pair_order[o];
-    it.head[0] = it.head[1] = idx - o * p.Hq;
-    it.row[0] = t * PA_TILE;
-    it.row[1] = it.row[0] + PA_TILE;
+    head0 = head1 = idx - o * p.Hq;
+    row0 = t * PA_TILE;
+    row1 = row0 + PA_TILE;
     lo = plan.tile_lo[t];
     last = t;
     if (t + 1 < tiles && plan.tile_lo[t + 1] != PA_NONE) {
@@ -203,20 +205,9 @@ __device__ __forceinline__ PackedFwdItem pf_item(const PackedFwdParams& p, const
       last = t + 1;
     }
   }
-  it.hk = it.head[0] / (p.Hq / p.Hkv);
-  const int first = p.window > 0 ? max(lo, it.row[0] - p.window + 1) : lo;
-  it.j0 = lo == PA_NONE ? 0 : first / PA_TILE;
-  it.n = lo == PA_NONE ? 0 : last - it.j0 + 1;
-  return it;
-}
-__device__ __forceinline__ void pf_uniform(PackedFwdItem& it) {
-  it.row[0] = warp_uniform(it.row[0]);
-  it.row[1] = warp_uniform(it.row[1]);
-  it.head[0] = warp_uniform(it.head[0]);
-  it.head[1] = warp_uniform(it.head[1]);
-  it.hk = warp_uniform(it.hk);
-  it.j0 = warp_uniform(it.j0);
-  it.n = warp_uniform(it.n);
+  const int first = p.window > 0 ? max(lo, row0 - p.window + 1) : lo;
+  const int j0 = lo == PA_NONE ? 0 : first / PA_TILE;
+  return {{row0, row1, head0, head1, head0 / (p.Hq / p.Hkv), j0, 0, lo == PA_NONE ? 0 : last - j0 + 1}};
 }
 
 // One row over its visible keys lo .. row alone (a whole warp)
@@ -378,7 +369,12 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   uint64_t* s_full = kv_empty + NST;
   uint64_t* p_full = s_full + 2;
   uint64_t* o_full = p_full + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 2);
+  PaQueue queue;
+  queue.full = o_full + 2;
+  queue.empty = queue.full + PA_SLOTS;
+  queue.want = queue.empty + PA_SLOTS;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(queue.want + 1);
+  queue.slot = reinterpret_cast<int4*>(smem + 512);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   uint8_t* q_s = smem + L::Q_OFF;
   uint8_t* kv_s = smem + L::KV_OFF;
@@ -397,6 +393,11 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       mbar_init(&kv_full[s], 1);
       mbar_init(&kv_empty[s], 1);
     }
+    for (int q = 0; q < PA_SLOTS; ++q) {
+      mbar_init(&queue.full[q], 1);
+      mbar_init(&queue.empty[q], 10);          // softmax warps, issuer, copies
+    }
+    mbar_init(queue.want, 1);
     *abort_flag = 0;
     fence_mbar_init();
     prefetch_tmap(&map_q);
@@ -430,12 +431,11 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         }
         if (++st == NST) { st = 0; ph ^= 1; }
       };
-      for (int r = 0; ok; ++r) {
-        const int idx = pa_item(r);
-        if (r * (int)gridDim.x >= items) break;
-        if (idx >= items) continue;
-        PackedFwdItem it = pf_item(p, plan, idx);
-        pf_uniform(it);
+      PaReader reader;
+      PaItem next;
+      while (ok && reader.next(queue, next, abort_flag, p.status)) {
+        const PackedFwdItem it(next);
+        if (it.n < 0) break;
         if (it.n == 0) continue;
         load_stage(it.j0 * PA_TILE, it.hk);
         for (int g = 0; g < 2; ++g) {
@@ -453,6 +453,8 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         ++done;
       }
       if (ok && v_row >= 0) load_stage(-1, 0);
+    } else if (warp == 11) {
+      pa_schedule(queue, items, p.counter, [&](int idx) { return pf_item(p, plan, idx); }, abort_flag, p.status);
     } else if (warp == 8) {
       // ------------------------------------------------------------ MMAs
       constexpr uint32_t idesc_qk = make_idesc(1, 1, 0, 0, PA_TILE, PA_TILE);
@@ -461,13 +463,14 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       const uint64_t qd = make_smem_desc(smem_u32(q_s), 16, 1024, 2);
       const uint64_t vd = make_smem_desc(smem_u32(kv_s), 16384, 1024, 2);               // key rows as the reduction
       const uint64_t kd = make_smem_desc(smem_u32(kv_s + L::TILE), 16, 1024, 2);
-      int r = 0;
+      PaReader reader;
+      bool ok = true;
       auto next_len = [&]() {                  // key tiles of the next item that has any, 0 behind the last
-        while (r * (int)gridDim.x < items) {
-          const int idx = pa_item(r++);
-          if (idx >= items) continue;
-          const int n = warp_uniform(pf_item(p, plan, idx).n);
-          if (n > 0) return n;
+        PaItem next;
+        while (ok) {
+          ok = reader.next(queue, next, abort_flag, p.status);
+          const int n = warp_uniform(next.v[7]);
+          if (ok && n != 0) return n > 0 ? n : 0;
         }
         return 0;
       };
@@ -478,11 +481,9 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       int st = 0;
       uint32_t ph = 0, pph = 0, qph = 0;
       int n = next_len(), i = 0;               // the step whose P V comes next: i of n
-      bool ok = true;
       bool last = n == 1;
-      int after = last ? next_len() : n;       // length of the item that the step behind it belongs to
       if (n > 0) {                             // scores of the first step
-        ok = pa_wait(&kv_full[0], 0, abort_flag, p.status, ST_PATTN_KV_FULL);
+        ok = ok && pa_wait(&kv_full[0], 0, abort_flag, p.status, ST_PATTN_KV_FULL);
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
           ok = ok && pa_wait(&q_full[g], 0, abort_flag, p.status, ST_PATTN_Q);
@@ -501,13 +502,11 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         ok = ok && pa_wait(&kv_full[st], ph, abort_flag, p.status, ST_PATTN_KV_FULL);
       }
       while (ok && n > 0) {
-        const bool more = after > 0, was = last;
-        const bool ends = last ? after == 1 : i + 2 == n;        // whether the next step is its item's last
+        const bool was = last;
         const uint64_t v0 = vd + (uint32_t)(st * 2 * STEP), k0 = kd + (uint32_t)(st * 2 * STEP);
         const uint32_t fresh = i != 0 ? 1u : 0u;
         const int s0 = st;
-        if (more && last) ok = pa_wait(&q_full[0], qph, abort_flag, p.status, ST_PATTN_Q);
-        ok = ok && pa_wait(&p_full[0], pph, abort_flag, p.status, ST_PATTN_P);
+        ok = pa_wait(&p_full[0], pph, abort_flag, p.status, ST_PATTN_P);
         if (!ok) break;
         tc_fence_after();
         if (elect_one()) {
@@ -515,18 +514,22 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           for (int k4 = 0; k4 < 8; ++k4)
             umma_f16_ts(tmem + 256, tmem + k4 * 8, v0 + k4 * (2048 >> 4), idesc_pv, k4 != 0 ? 1u : fresh);
           if (was) umma_commit(&o_full[0]);
-          if (more) {
-            pa_mma_ss<DP>(tmem, qd, k0, idesc_qk);
-            umma_commit(&s_full[0]);
-            if (ends) umma_commit(&q_empty[0]);
-          }
         }
-        if (more && last) ok = pa_wait(&q_full[1], qph, abort_flag, p.status, ST_PATTN_Q);
+        const int after = was ? next_len() : n;                  // length of the item that the next step belongs to
+        const bool more = after > 0;
+        const bool ends = was ? after == 1 : i + 2 == n;         // whether that step is its item's last
+        if (more && was) ok = ok && pa_wait(&q_full[0], qph, abort_flag, p.status, ST_PATTN_Q);
+        if (!ok) break;
+        if (more && elect_one()) {
+          pa_mma_ss<DP>(tmem, qd, k0, idesc_qk);
+          umma_commit(&s_full[0]);
+          if (ends) umma_commit(&q_empty[0]);
+        }
+        if (more && last) ok = ok && pa_wait(&q_full[1], qph, abort_flag, p.status, ST_PATTN_Q);
         if (last) qph ^= 1;
         i = last ? 0 : i + 1;
         n = after;
         last = i == n - 1;
-        after = last ? next_len() : n;
         if (++st == NST) { st = 0; ph ^= 1; }
         if (n > 0) ok = ok && pa_wait(&kv_full[st], ph, abort_flag, p.status, ST_PATTN_KV_FULL);
         ok = ok && pa_wait(&p_full[1], pph, abort_flag, p.status, ST_PATTN_P);
@@ -557,11 +560,12 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     const int tiles = (p.rows + PA_TILE - 1) / PA_TILE;
     int step = 0, done = 0;
     bool ok = true;
-    for (int r = 0; ok; ++r) {
-      const int idx = pa_item(r);
-      if (r * (int)gridDim.x >= items) break;
-      if (idx >= items) continue;
-      const PackedFwdItem it = pf_item(p, plan, idx);
+    const bool wide = p.D % 16 == 0 && (reinterpret_cast<size_t>(p.out) & 31) == 0;
+    PaReader reader;
+    PaItem next;
+    while (reader.next(queue, next, abort_flag, p.status)) {
+      const PackedFwdItem it(next);
+      if (it.n < 0) break;
       const int row = it.row[g] + r128, head = it.head[g];
       int lo = PA_NONE;                        // first key of this row
       if (row < p.rows) {
@@ -569,10 +573,13 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         if (p.window > 0) lo = max(lo, row - p.window + 1);
       }
       const bool sees = lo <= row;
+      const int tell = max(it.n - PA_EARLY, 0);
+      if (it.n == 0 && threadIdx.x == 0) mbar_arrive(queue.want);
       float m = -INFINITY;                     // maximum (log2 units) that the sums are relative to
       float2 la = make_float2(0.f, 0.f), lb = la;
       for (int i = 0; i < it.n; ++i, ++step) {
         const int kv0 = (it.j0 + i) * PA_TILE;
+        if (i == tell && threadIdx.x == 0) mbar_arrive(queue.want);
         ok = pa_wait(&s_full[g], step & 1, abort_flag, p.status, ST_PATTN_S);
         if (!ok) break;
         tc_fence_after();
@@ -611,20 +618,15 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         }
 #pragma unroll
         for (int k = 0; k < 32; ++k) sum += fabsf(__uint_as_float(o[k]));
-        if (row < p.rows) {
+        if (!sees) {
 #pragma unroll
-          for (int k = 0; k < 32; k += 8) {
-            if (c + k < p.D) {
-              uint4 v = make_uint4(0u, 0u, 0u, 0u);
-              if (sees) {
-                v.x = pa_pack(__uint_as_float(o[k]) * inv, __uint_as_float(o[k + 1]) * inv);
-                v.y = pa_pack(__uint_as_float(o[k + 2]) * inv, __uint_as_float(o[k + 3]) * inv);
-                v.z = pa_pack(__uint_as_float(o[k + 4]) * inv, __uint_as_float(o[k + 5]) * inv);
-                v.w = pa_pack(__uint_as_float(o[k + 6]) * inv, __uint_as_float(o[k + 7]) * inv);
-              }
-              *reinterpret_cast<uint4*>(o_row + c + k) = v;
-            }
-          }
+          for (int k = 0; k < 32; ++k) o[k] = 0u;
+        }
+        if (row < p.rows) {
+          const float f = sees ? inv : 0.f;
+#pragma unroll
+          for (int k = 0; k < 32; k += 16)
+            if (c + k < p.D) pa_put16(o_row + c + k, o, k, f, wide, p.D - c - k);
         }
       }
       if (it.row[g] < tiles * PA_TILE)
@@ -660,6 +662,7 @@ static int packed_fwd_launch(const CUtensorMap& mq, const CUtensorMap& mk, const
   SLAB_CUDA_CHECK(cudaFuncSetAttribute(packed_fwd_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        PackedFwdSmem<DP>::TOTAL));
   const int grid = items < sm_count() ? (int)items : sm_count();
+  if (items > grid) SLAB_CUDA_CHECK(cudaMemsetAsync(p.counter, 0, sizeof(int), stream));
   packed_fwd_kernel<DP><<<grid, PF_THREADS, PackedFwdSmem<DP>::TOTAL, stream>>>(mq, mk, mv, p, (int)items);
   return (int)cudaGetLastError();
 }
@@ -697,10 +700,10 @@ extern "C" int slab_packed_plan_tokens(const void* tokens, int rows, int seq, lo
 }
 
 // q [rows, Hq, D], k and v [rows, Hkv, D] bf16 with the given token and head strides (elements, multiples of 8; bases on 16
-// bytes), out [rows, Hq, D] contiguous, lse [Hq, tiles * 128] fp32.  D a multiple of 8 up to 128.
+// bytes), out [rows, Hq, D] contiguous, lse [Hq, tiles * 128] fp32, counter: scratch, one int32.  D a multiple of 8 up to 128.
 extern "C" int slab_packed_attn_fwd(const void* q, const void* k, const void* v, void* out, void* lse, const void* plan,
                                     int rows, int hq, int hkv, int d, long q_ts, long q_hs, long k_ts, long k_hs, long v_ts,
-                                    long v_hs, int window, float scale, void* status, void* stream) {
+                                    long v_hs, int window, float scale, void* counter, void* status, void* stream) {
   using namespace slab;
   if (rows <= 0 || hq <= 0 || hkv <= 0 || hq % hkv || d <= 0 || d > 128 || d % 8 || window < 0 || !(scale > 0.f)) return -10;
   if ((q_ts | q_hs | k_ts | k_hs | v_ts | v_hs) & 7) return -11;
@@ -722,6 +725,7 @@ extern "C" int slab_packed_attn_fwd(const void* q, const void* k, const void* v,
   p.window = window;
   p.head_pairs = (hq / hkv) % 2 == 0;
   p.scale_log2 = scale * 1.4426950408889634f;
+  p.counter = (int*)counter;
   p.status = (int*)status;
   return d <= 64 ? packed_fwd_launch<64>(mq, mk, mv, p, (cudaStream_t)stream)
                  : packed_fwd_launch<128>(mq, mk, mv, p, (cudaStream_t)stream);

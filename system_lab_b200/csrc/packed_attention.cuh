@@ -15,6 +15,7 @@ enum : int {
   ST_PATTN_S = 43,         // softmax waited for scores
   ST_PATTN_P = 44,         // MMA issuer waited for probabilities (or their gradient)
   ST_PATTN_OUT = 45,       // softmax waited for the finished accumulators
+  ST_PATTN_ITEM = 46,      // waited for the next item, or for room to put it
 };
 
 // The plan of a packed buffer (packed_bounds_kernel), int32:
@@ -43,11 +44,30 @@ inline __host__ __device__ PackedPlan packed_plan(const int* base, int rows) {
   return p;
 }
 
-// Items are listed by falling work; a persistent block takes one of every round, and rounds run forwards and backwards in
-// turn, so that no block has the longest of each.
-__device__ __forceinline__ int pa_item(int round) {
-  return round * (int)gridDim.x + ((round & 1) ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x);
-}
+// ---------------------------------------------------------------- work queue
+// Items are listed by falling work.  A block takes the one of its index first and then, one by one, the first that no block has
+// taken: documents differ, and dealt out beforehand the last block ended a third after the mean (dk and dv, 8192 rows in
+// documents of 700: 458 thousand cycles, mean 341).  A warp of its own takes and decodes them, so that no other role waits for
+// the plan's dependent loads (2 to 3 thousand cycles an item), when the softmax warps are PA_EARLY steps from their item's end:
+// taken as early as there is room, the first three rounds would be dealt out at once (one document of 8192 rows: dk and dv 2101
+// us, 1755 so).  Issuers and copies may be an item ahead of the softmax warps; nobody waits for an item that is given out only
+// once he has done something for the one before.
+constexpr int PA_SLOTS = 2, PA_EARLY = 3;
+struct PaQueue {
+  uint64_t* full;                            // [PA_SLOTS]
+  uint64_t* empty;                           // [PA_SLOTS], one arrival per reading warp
+  uint64_t* want;                            // the softmax warps are near their item's end
+  int4* slot;                                // [PA_SLOTS][2]
+};
+struct PaItem {
+  int v[8];                                  // the last: steps, -1 behind the last item
+};
+// A reader's next item, to all lanes of its warp; false if a wait ran out
+struct PaReader {
+  int s = 0;
+  uint32_t ph = 0;
+  __device__ __forceinline__ bool next(const PaQueue& q, PaItem& it, volatile int* abort_flag, int* status);
+};
 
 // ---------------------------------------------------------------- tensor memory
 // D[tmem] (+)= A[tmem] * B[smem desc]: A as 16-bit pairs, row = lane, 8 columns per 16 of the reduction.
@@ -98,9 +118,61 @@ __device__ __forceinline__ bool pa_wait(uint64_t* bar, uint32_t parity, volatile
   return mbar_wait_warp(bar, parity, abort_flag, status, code);
 }
 
+__device__ __forceinline__ bool PaReader::next(const PaQueue& q, PaItem& it, volatile int* abort_flag, int* status) {
+  if (!pa_wait(&q.full[s], ph, abort_flag, status, ST_PATTN_ITEM)) return false;
+  const int4 a = q.slot[2 * s], b = q.slot[2 * s + 1];
+  it = {{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(&q.empty[s]);
+  if (++s == PA_SLOTS) { s = 0; ph ^= 1; }
+  return true;
+}
+// The taking warp: decode(index) makes an item of the list's index.
+template <typename Decode>
+__device__ __forceinline__ void pa_schedule(const PaQueue& q, int items, int* counter, Decode decode, volatile int* abort_flag,
+                                            int* status) {
+  int s = 0, idx = blockIdx.x;
+  uint32_t ph = 1, want = 0;
+  while (true) {
+    if (!pa_wait(&q.empty[s], ph, abort_flag, status, ST_PATTN_ITEM)) return;
+    PaItem it;
+    it.v[7] = -1;
+    if (idx < items) it = decode(idx);
+    if ((threadIdx.x & 31) == 0) {
+      q.slot[2 * s] = make_int4(it.v[0], it.v[1], it.v[2], it.v[3]);
+      q.slot[2 * s + 1] = make_int4(it.v[4], it.v[5], it.v[6], it.v[7]);
+      mbar_arrive(&q.full[s]);
+    }
+    if (idx >= items) return;
+    if (++s == PA_SLOTS) { s = 0; ph ^= 1; }
+    if (!pa_wait(q.want, want, abort_flag, status, ST_PATTN_ITEM)) return;
+    want ^= 1;
+    if (items > (int)gridDim.x) {
+      if ((threadIdx.x & 31) == 0) idx = (int)gridDim.x + atomicAdd(counter, 1);
+      idx = warp_uniform(idx);
+    } else {
+      idx = items;                           // a block for every item: nothing is counted
+    }
+  }
+}
+
 __device__ __forceinline__ uint32_t pa_pack(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
+}
+// 16 neighbouring bf16 of a row, from fp32: one 32-byte store (a whole sector) where the row allows it, else up to two of 16
+__device__ __forceinline__ void pa_put16(__nv_bfloat16* to, const uint32_t (&o)[32], int k, float f, bool wide, int left) {
+  uint32_t v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = pa_pack(__uint_as_float(o[k + 2 * i]) * f, __uint_as_float(o[k + 2 * i + 1]) * f);
+  if (wide) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+                 "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+  } else {
+    if (left > 0) *reinterpret_cast<uint4*>(to) = make_uint4(v[0], v[1], v[2], v[3]);
+    if (left > 8) *reinterpret_cast<uint4*>(to + 8) = make_uint4(v[4], v[5], v[6], v[7]);
+  }
 }
 // two fp32 lanes in one instruction
 __device__ __forceinline__ float2 pa_fma2(float2 a, float2 b, float2 c) {

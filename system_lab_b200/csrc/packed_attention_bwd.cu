@@ -16,6 +16,7 @@
 namespace slab {
 
 constexpr int PB_THREADS = 384;
+constexpr int PB_EVERY = 8;                  // of that many pairs of exponentials, one is made on the multiply-add units
 
 struct PackedBwdParams {
   __nv_bfloat16 *dq, *dk, *dv;   // [rows, heads, D] contiguous
@@ -27,6 +28,7 @@ struct PackedBwdParams {
   int window;
   int splits;
   float scale, scale_log2;
+  int* counter;                  // [2] items taken behind the first of every block (dk and dv, dq), zero at launch
   int* status;
 };
 
@@ -41,7 +43,8 @@ __device__ __forceinline__ void pb_bulk_load(void* dst, const void* src, uint32_
 // A group of 16 lanes per (row, head); rows behind the buffer's end, up to whole tiles, get zero.
 __global__ void __launch_bounds__(256)
 packed_delta_kernel(const __nv_bfloat16* out, const __nv_bfloat16* dout, float* delta, int rows, int padded, int hq, int d,
-                    long do_ts, long do_hs) {
+                    long do_ts, long do_hs, int* counter) {
+  if (blockIdx.x == 0 && threadIdx.x < 2) counter[threadIdx.x] = 0;    // of the two kernels behind this one
   const long unit = (long)blockIdx.x * 16 + (threadIdx.x >> 4);          // rows fastest: neighbours write side by side
   const int sub = threadIdx.x & 15;
   const int head = (int)(unit / padded), row = (int)(unit - (long)head * padded);
@@ -59,25 +62,138 @@ packed_delta_kernel(const __nv_bfloat16* out, const __nv_bfloat16* dout, float* 
 }
 
 // ================================================================ common to both
-// 64 scores of a row become probabilities: columns first .. first + span are visible.
-__device__ __forceinline__ void pb_mask(float (&s)[64], int first, uint32_t span) {
-#pragma unroll
-  for (int c = 0; c < 64; ++c) s[c] = (uint32_t)(c - first) <= span ? s[c] : 0.f;
+// What a row's scores are reduced by (base-2 log-sum-exp; delta), per column: one value where rows are queries, one each where
+// columns are.
+struct PbRow {
+  float v;
+  __device__ __forceinline__ float4 at(int) const { return make_float4(v, v, v, v); }
+};
+struct PbCols {
+  const float4* p;
+  __device__ __forceinline__ float4 at(int c) const { return p[c >> 2]; }
+};
+__device__ __forceinline__ bool pb_seen(int c, int first, uint32_t span) { return (uint32_t)(c - first) <= span; }
+__device__ __forceinline__ void pb_load(uint32_t taddr, float* s) {
+  tmem_ld_32x32(taddr, *reinterpret_cast<uint32_t(*)[32]>(s));
 }
-__device__ __forceinline__ void pb_load64(uint32_t taddr, float (&s)[64]) {
-  tmem_ld_32x32(taddr, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
-  tmem_ld_32x32(taddr + 32, *reinterpret_cast<uint32_t(*)[32]>(&s[32]));
-  tmem_ld_wait();
+// 32 values to bf16, over the first 16 columns of where `to` points
+__device__ __forceinline__ void pb_store(uint32_t to, const float* s) {
+  uint32_t v[16];
+#pragma unroll
+  for (int k = 0; k < 16; ++k) v[k] = pa_pack(s[2 * k], s[2 * k + 1]);
+  tmem_st_32x16(to, v);
 }
-__device__ __forceinline__ void pb_store64(uint32_t taddr, const float (&s)[64]) {
+// 32 scores to probabilities; one pair in PB_EVERY is made on the multiply-add units where nothing is masked
+template <bool PART, typename Stat>
+__device__ __forceinline__ void pb_probs(float* s, int c0, const Stat& lse, float2 c2, int first, uint32_t span) {
 #pragma unroll
-  for (int c = 0; c < 64; c += 32) {
-    uint32_t v[16];
+  for (int c = 0; c < 32; c += 4) {
+    const float4 b = lse.at(c0 + c);
 #pragma unroll
-    for (int k = 0; k < 16; ++k) v[k] = pa_pack(s[c + 2 * k], s[c + 2 * k + 1]);
-    tmem_st_32x16(taddr + c / 2, v);
+    for (int e = 0; e < 4; e += 2) {
+      float2 x = pa_fma2(make_float2(s[c + e], s[c + e + 1]), c2, e ? make_float2(-b.z, -b.w) : make_float2(-b.x, -b.y));
+      if (!PART && ((c + e) / 2) % PB_EVERY == PB_EVERY - 1) {
+        x = pa_exp2_fma(x);
+      } else {
+        x.x = pa_exp2(x.x);
+        x.y = pa_exp2(x.y);
+      }
+      s[c + e] = !PART || pb_seen(c0 + c + e, first, span) ? x.x : 0.f;
+      s[c + e + 1] = !PART || pb_seen(c0 + c + e + 1, first, span) ? x.y : 0.f;
+    }
   }
+}
+// 32 probabilities times (dP - delta).  (Zero times what a hidden row holds may be no number: masked again.)
+template <bool PART, typename Stat>
+__device__ __forceinline__ void pb_dscores(float* s, const float* t, int c0, const Stat& delta, int first, uint32_t span) {
+#pragma unroll
+  for (int c = 0; c < 32; c += 4) {
+    const float4 b = delta.at(c0 + c);
+#pragma unroll
+    for (int e = 0; e < 4; e += 2) {
+      const float2 x = pa_mul2(make_float2(s[c + e], s[c + e + 1]),
+                               pa_add2(make_float2(t[c + e], t[c + e + 1]), e ? make_float2(-b.z, -b.w) : make_float2(-b.x, -b.y)));
+      s[c + e] = !PART || pb_seen(c0 + c + e, first, span) ? x.x : 0.f;
+      s[c + e + 1] = !PART || pb_seen(c0 + c + e + 1, first, span) ? x.y : 0.f;
+    }
+  }
+}
+// What of a thread's 64 columns its row and its warp see.  The warp sees all (whole), or 32-column chunks in vis.
+struct PbView {
+  int first;
+  uint32_t span, vis;
+  bool whole;
+  __device__ __forceinline__ PbView(int from, int to) {      // columns from .. to of 0 .. 63
+    from = max(from, 0);
+    to = min(to, 63);
+    const bool none = from > to;
+    first = none ? 1 << 20 : from;
+    span = none ? 0u : (uint32_t)(to - from);
+    whole = !__any_sync(0xffffffffu, from > 0 || to < 63);
+    vis = 3u;
+    if (!whole) {
+      const int lo = __reduce_min_sync(0xffffffffu, none ? 64 : from), hi = __reduce_max_sync(0xffffffffu, none ? -1 : to);
+      vis = (lo < 32 && hi >= 0 ? 1u : 0u) | (hi >= 32 ? 2u : 0u);
+    }
+  }
+};
+// Scores at `from` to probabilities s.  STORE: as bf16 over the scores too.
+template <bool STORE, typename Stat>
+__device__ __forceinline__ void pb_step_p(uint32_t from, float (&s)[64], const PbView& v, const Stat& lse, float2 c2) {
+  if (v.whole) {
+    pb_load(from, &s[0]);
+    pb_load(from + 32, &s[32]);
+    tmem_ld_wait();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      pb_probs<false>(&s[32 * h], 32 * h, lse, c2, 0, 0u);
+      if (STORE) pb_store(from + 16 * h, &s[32 * h]);
+    }
+    return;
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    if (v.vis >> h & 1u) {
+      pb_load(from + 32 * h, &s[32 * h]);
+      tmem_ld_wait();
+      pb_probs<true>(&s[32 * h], 32 * h, lse, c2, v.first, v.span);
+    } else {
+#pragma unroll
+      for (int c = 0; c < 32; ++c) s[32 * h + c] = 0.f;
+    }
+    if (STORE) pb_store(from + 16 * h, &s[32 * h]);
+  }
+}
+// dP at `from` and probabilities s to the scores' gradient, as bf16 at `to`
+template <typename Stat>
+__device__ __forceinline__ void pb_step_ds(uint32_t from, uint32_t to, float (&s)[64], const PbView& v, const Stat& delta) {
+  float t[64];
+  if (v.whole) {
+    pb_load(from, &t[0]);
+    pb_load(from + 32, &t[32]);
+    tmem_ld_wait();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      pb_dscores<false>(&s[32 * h], &t[32 * h], 32 * h, delta, 0, 0u);
+      pb_store(to + 16 * h, &s[32 * h]);
+    }
+    return;
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    if (v.vis >> h & 1u) {
+      pb_load(from + 32 * h, &t[32 * h]);
+      tmem_ld_wait();
+      pb_dscores<true>(&s[32 * h], &t[32 * h], 32 * h, delta, v.first, v.span);
+    }
+    pb_store(to + 16 * h, &s[32 * h]);
+  }
+}
+__device__ __forceinline__ void pb_arrive(uint64_t* bar) {
   tmem_st_wait();
+  tc_fence_before();
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
 }
 // A from tensor memory: 128 rows x 128 of the reduction, the left 64 at a, the right ones 64 columns on
 template <int DP>
@@ -99,44 +215,24 @@ struct PackedDqSmem {
 
 struct PackedDqItem {
   int row, head, hk, j0, n;
+  __device__ __forceinline__ explicit PackedDqItem(const PaItem& i) : row(i.v[0]), head(i.v[1]), hk(i.v[2]), j0(i.v[3]), n(i.v[7]) {}
 };
-__device__ __forceinline__ PackedDqItem pb_dq_item(const PackedBwdParams& p, const PackedPlan& plan, int idx) {
-  PackedDqItem it;
+__device__ __forceinline__ PaItem pb_dq_item(const PackedBwdParams& p, const PackedPlan& plan, int idx) {
   const int o = idx / p.Hq, t = plan.q_order[o], lo = plan.tile_lo[t];
-  it.head = idx - o * p.Hq;
-  it.hk = it.head / (p.Hq / p.Hkv);
-  it.row = t * PA_TILE;
-  const int first = p.window > 0 ? max(lo, it.row - p.window + 1) : lo;
-  it.j0 = lo == PA_NONE ? 0 : first / PA_TILE;
-  it.n = lo == PA_NONE ? 0 : t - it.j0 + 1;
-  it.row = warp_uniform(it.row);
-  it.head = warp_uniform(it.head);
-  it.hk = warp_uniform(it.hk);
-  it.j0 = warp_uniform(it.j0);
-  it.n = warp_uniform(it.n);
-  return it;
+  const int head = idx - o * p.Hq, row = t * PA_TILE;
+  const int first = p.window > 0 ? max(lo, row - p.window + 1) : lo;
+  const int j0 = lo == PA_NONE ? 0 : first / PA_TILE;
+  return {{row, head, head / (p.Hq / p.Hkv), j0, 0, 0, 0, lo == PA_NONE ? 0 : t - j0 + 1}};
 }
 
-// A walk over an issuer's steps (key tiles of item after item), which may run ahead of another one.
-template <typename NextLen>
-struct StepWalk {
-  NextLen next;            // length of the next item with steps, 0 behind the last
-  int n = 0, i = 0, seen = 0, step = 0;
-  bool more = true;
-  __device__ __forceinline__ explicit StepWalk(NextLen f) : next(f) { fetch(); }
-  __device__ __forceinline__ void fetch() {
-    n = next();
-    i = 0;
-    more = n > 0;
-    ++seen;
-  }
-  __device__ __forceinline__ void advance() {
-    ++step;
-    if (++i == n) fetch();
-  }
+// An issuer's place in the steps of item after item
+struct PbWalk {
+  int n = 0, i = 0, items = 0;                 // length of the current item, steps of it done, items begun
+  __device__ __forceinline__ bool due() const { return i == n; }
+  __device__ __forceinline__ void begin(int len) { n = len; i = 0; ++items; }
   __device__ __forceinline__ bool first() const { return i == 0; }
   __device__ __forceinline__ bool last() const { return i == n - 1; }
-  __device__ __forceinline__ uint32_t item_parity() const { return (seen - 1) & 1; }
+  __device__ __forceinline__ uint32_t parity() const { return (items - 1) & 1; }
 };
 
 // p and ds of one pair of rows (a whole warp)
@@ -210,14 +306,22 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   uint64_t* k_empty = k_full + KST;
   uint64_t* v_full = k_empty + KST;
   uint64_t* v_empty = v_full + VST;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_empty + VST);
+  PaQueue queue;
+  queue.full = v_empty + VST;
+  queue.empty = queue.full + PA_SLOTS;
+  queue.want = queue.empty + PA_SLOTS;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(queue.want + 1);
+  queue.slot = reinterpret_cast<int4*>(smem + 512);
+  int* lens = reinterpret_cast<int*>(smem + 768);              // [4] the issuer's items in flight
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   uint8_t *q_s = smem + L::Q_OFF, *do_s = smem + L::DO_OFF, *k_s = smem + L::K_OFF, *v_s = smem + L::V_OFF;
   const int warp = warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const PackedPlan plan = packed_plan(p.plan, p.rows);
 
   if (threadIdx.x == 0) {
-    for (uint64_t* b = q_full; b < v_empty + VST; ++b) mbar_init(b, b == ds_full ? 8 : 1);
+    for (uint64_t* b = q_full; b < queue.empty; ++b) mbar_init(b, b == ds_full ? 8 : 1);
+    for (int q = 0; q < PA_SLOTS; ++q) mbar_init(&queue.empty[q], 10);           // softmax warps, issuer, copies
+    mbar_init(queue.want, 1);
     *abort_flag = 0;
     fence_mbar_init();
     prefetch_tmap(&map_q);
@@ -246,10 +350,11 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           pa_load_tile<DP>(dst, map, full, head, row);
         }
       };
-      for (int r = 0; ok && r * (int)gridDim.x < items; ++r) {
-        const int idx = pa_item(r);
-        if (idx >= items) continue;
-        const PackedDqItem it = pb_dq_item(p, plan, idx);
+      PaReader reader;
+      PaItem next;
+      while (ok && reader.next(queue, next, abort_flag, p.status)) {
+        const PackedDqItem it(next);
+        if (it.n < 0) break;
         if (it.n == 0) continue;
         load(q_s, &map_q, q_full, q_empty, (done & 1) ^ 1, it.head, it.row);
         for (int i = 0; ok && i < it.n; ++i, ++pos) {
@@ -260,6 +365,8 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         }
         ++done;
       }
+    } else if (warp == 11) {
+      pa_schedule(queue, items, p.counter + 1, [&](int idx) { return pb_dq_item(p, plan, idx); }, abort_flag, p.status);
     } else if (warp == 8) {
       constexpr uint32_t idesc_s = make_idesc(1, 1, 0, 0, PA_TILE, PA_TILE);
       constexpr uint32_t idesc_d = make_idesc(1, 1, 0, 1, PA_TILE, DP);
@@ -267,25 +374,28 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       const uint64_t qd = make_smem_desc(smem_u32(q_s), 16, 1024, 2), dod = make_smem_desc(smem_u32(do_s), 16, 1024, 2);
       const uint64_t kd = make_smem_desc(smem_u32(k_s), 16, 1024, 2), vd = make_smem_desc(smem_u32(v_s), 16, 1024, 2);
       const uint64_t kt = make_smem_desc(smem_u32(k_s), 16384, 1024, 2);      // K with its rows as the reduction
-      bool ok = true;
-      auto lens = [&, r = 0]() mutable {
-        while (r * (int)gridDim.x < items) {
-          const int idx = pa_item(r++);
-          if (idx >= items) continue;
-          const int n = warp_uniform(pb_dq_item(p, plan, idx).n);
-          if (n > 0) return n;
-        }
-        return 0;
-      };
+      bool ok = true, more = true;             // more: the queue has not ended
+      PaReader reader;
       // Scores run two steps ahead, dP one; each walk counts its item's steps, stages and parities (counted, not computed: see
       // elect_one).  What a product needs beside ds is waited for while others run.
-      StepWalk<decltype(lens)> ws(lens), wp(lens), wq(lens);
+      PbWalk ws, wp, wq;
       int sk = 0, sq = 0, sv = 0;              // stages of K for the scores, of K for dq, of V
       uint32_t kph = 0, vph = 0, buf = 0, qbuf = 0, dsph = 0;
       auto scores = [&]() {
-        if (!ok || !ws.more) return;
+        while (ok && more && ws.due()) {
+          PaItem next;
+          ok = reader.next(queue, next, abort_flag, p.status);
+          const int n = warp_uniform(next.v[7]);
+          more = ok && n >= 0;
+          if (more && n > 0) {
+            if (lane == 0) lens[ws.items & 3] = n;
+            __syncwarp();
+            ws.begin(n);
+          }
+        }
+        if (!ok || !more) return;
         ok = pa_wait(&k_full[sk], kph, abort_flag, p.status, ST_PATTN_KV_FULL);
-        if (ws.first()) ok = ok && pa_wait(q_full, ws.item_parity(), abort_flag, p.status, ST_PATTN_Q);
+        if (ws.first()) ok = ok && pa_wait(q_full, ws.parity(), abort_flag, p.status, ST_PATTN_Q);
         if (!ok) return;
         tc_fence_after();
         const uint64_t k0 = kd + (uint32_t)(sk * STEP);
@@ -295,17 +405,24 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           umma_commit(&s_full[buf]);
           if (ws.last()) umma_commit(q_empty);
         }
-        ws.advance();
+        ++ws.i;
         buf ^= 1;
         if (++sk == KST) { sk = 0; kph ^= 1; }
       };
-      auto need_v = [&]() {                    // V of the next dP (and its item's dO)
-        if (!ok || !wp.more) return;
+      // the other walks follow the scores' items; false where there is none
+      auto follow = [&](PbWalk& w) {
+        if (w.due() && w.items < ws.items) w.begin(warp_uniform(lens[w.items & 3]));
+        return !w.due();
+      };
+      bool have_p = false;                     // V of the next dP (and its item's dO) is here
+      auto need_v = [&]() {
+        have_p = ok && follow(wp);
+        if (!have_p) return;
         ok = pa_wait(&v_full[sv], vph, abort_flag, p.status, ST_PATTN_KV_FULL);
-        if (wp.first()) ok = ok && pa_wait(do_full, wp.item_parity(), abort_flag, p.status, ST_PATTN_Q);
+        if (wp.first()) ok = ok && pa_wait(do_full, wp.parity(), abort_flag, p.status, ST_PATTN_Q);
       };
       auto dprob = [&]() {
-        if (!ok || !wp.more) return;
+        if (!ok || !have_p) return;
         const uint64_t v0 = vd + (uint32_t)(sv * STEP);
         if (elect_one()) {
           pa_mma_ss<DP>(tmem + 256, dod, v0, idesc_s);
@@ -313,7 +430,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           umma_commit(&v_empty[sv]);
           if (wp.last()) umma_commit(do_empty);
         }
-        wp.advance();
+        ++wp.i;
         if (++sv == VST) { sv = 0; vph ^= 1; }
       };
       scores();
@@ -322,22 +439,24 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       dprob();
       scores();
       need_v();
-      while (ok && wq.more) {
+      while (ok && follow(wq)) {
         ok = pa_wait(ds_full, dsph, abort_flag, p.status, ST_PATTN_P);
         if (!ok) break;
         tc_fence_after();
-        dprob();                               // first: the softmax has read dP and wants the next one soonest
         const uint64_t k0 = kt + (uint32_t)(sq * STEP);
         const uint32_t from = tmem + qbuf * 128;
-        const bool add = !wq.first();
+        const bool add = !wq.first(), last = wq.last();
+        // the softmax has read dP and wants the next one soonest, unless it waits for the item's dq
+        if (!last) dprob();
         if (elect_one()) {
           pb_mma_ts<DP>(tmem + 384, from, k0, idesc_d, add);
           umma_commit(&k_empty[sq]);
-          if (wq.last()) umma_commit(dq_full);
+          if (last) umma_commit(dq_full);
         }
+        if (last) dprob();
         scores();
         need_v();
-        wq.advance();
+        ++wq.i;
         dsph ^= 1;
         qbuf ^= 1;
         if (++sq == KST) sq = 0;
@@ -350,10 +469,12 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     const int padded = (p.rows + PA_TILE - 1) / PA_TILE * PA_TILE;
     int step = 0, done = 0;
     bool ok = true;
-    for (int r = 0; ok && r * (int)gridDim.x < items; ++r) {
-      const int idx = pa_item(r);
-      if (idx >= items) continue;
-      const PackedDqItem it = pb_dq_item(p, plan, idx);
+    const bool wide = p.D % 16 == 0 && (reinterpret_cast<size_t>(p.dq) & 31) == 0;
+    PaReader reader;
+    PaItem next;
+    while (reader.next(queue, next, abort_flag, p.status)) {
+      const PackedDqItem it(next);
+      if (it.n < 0) break;
       const int row = it.row + lg * 32 + lane;
       int lo = PA_NONE;
       if (row < p.rows) {
@@ -361,46 +482,25 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         if (p.window > 0) lo = max(lo, row - p.window + 1);
       }
       const bool sees = lo <= row;
-      const float nlse = -p.lse[(size_t)it.head * padded + row], delta = p.delta[(size_t)it.head * padded + row];
-      const float2 c2 = make_float2(p.scale_log2, p.scale_log2), b2 = make_float2(nlse, nlse), d2 = make_float2(-delta, -delta);
+      const PbRow lse = {p.lse[(size_t)it.head * padded + row]}, delta = {p.delta[(size_t)it.head * padded + row]};
+      const float2 c2 = make_float2(p.scale_log2, p.scale_log2);
+      const int tell = max(it.n - PA_EARLY, 0);
+      if (it.n == 0 && threadIdx.x == 0) mbar_arrive(queue.want);
       for (int i = 0; i < it.n; ++i, ++step) {
         const int c0 = (it.j0 + i) * PA_TILE + g * 64;         // first key of this thread's columns
+        if (i == tell && threadIdx.x == 0) mbar_arrive(queue.want);
         ok = pa_wait(&s_full[step & 1], (step >> 1) & 1, abort_flag, p.status, ST_PATTN_S);
         if (!ok) break;
         tc_fence_after();
+        const PbView view(lo - c0, sees ? row - c0 : -1);
         const uint32_t s_addr = base + (step & 1) * 128 + g * 64;
         float s[64];
-        pb_load64(s_addr, s);
-#pragma unroll
-        for (int c = 0; c < 64; c += 2) {
-          const float2 x = pa_fma2(make_float2(s[c], s[c + 1]), c2, b2);
-          s[c] = pa_exp2(x.x);
-          s[c + 1] = pa_exp2(x.y);
-        }
-        int first = max(lo - c0, 0);
-        const int lastk = min(row - c0, 63);
-        const bool none = !sees || first > lastk;
-        const bool part = none || first > 0 || lastk < 63;
-        if (none) first = 1 << 20;
-        const uint32_t span = none ? 0u : (uint32_t)(lastk - first);
-        const bool masked = __any_sync(0xffffffffu, part);
-        if (masked) pb_mask(s, first, span);
+        pb_step_p<false>(s_addr, s, view, lse, c2);
         ok = pa_wait(dp_full, step & 1, abort_flag, p.status, ST_PATTN_S);
         if (!ok) break;
         tc_fence_after();
-        float t[64];
-        pb_load64(base + 256 + g * 64, t);
-#pragma unroll
-        for (int c = 0; c < 64; c += 2) {
-          const float2 x = pa_mul2(make_float2(s[c], s[c + 1]), pa_add2(make_float2(t[c], t[c + 1]), d2));
-          s[c] = x.x;
-          s[c + 1] = x.y;
-        }
-        if (masked) pb_mask(s, first, span);   // zero times what a hidden key holds may be no number
-        pb_store64(s_addr, s);
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(ds_full);
+        pb_step_ds(base + 256 + g * 64, s_addr, s, view, delta);
+        pb_arrive(ds_full);
       }
       if (!ok) break;
       if (it.n > 0) {
@@ -421,20 +521,14 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         }
 #pragma unroll
         for (int e = 0; e < 32; ++e) sum += fabsf(__uint_as_float(o[e]));
+        if (!sees) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0u;
+        }
         if (row < p.rows) {
 #pragma unroll
-          for (int e = 0; e < 32; e += 8) {
-            if (c + e < p.D) {
-              uint4 v = make_uint4(0u, 0u, 0u, 0u);
-              if (sees) {
-                v.x = pa_pack(__uint_as_float(o[e]) * p.scale, __uint_as_float(o[e + 1]) * p.scale);
-                v.y = pa_pack(__uint_as_float(o[e + 2]) * p.scale, __uint_as_float(o[e + 3]) * p.scale);
-                v.z = pa_pack(__uint_as_float(o[e + 4]) * p.scale, __uint_as_float(o[e + 5]) * p.scale);
-                v.w = pa_pack(__uint_as_float(o[e + 6]) * p.scale, __uint_as_float(o[e + 7]) * p.scale);
-              }
-              *reinterpret_cast<uint4*>(dq_row + c + e) = v;
-            }
-          }
+          for (int e = 0; e < 32; e += 16)
+            if (c + e < p.D) pa_put16(dq_row + c + e, o, e, p.scale, wide, p.D - c - e);
         }
       }
       for (uint32_t m = __ballot_sync(0xffffffffu, sees && !pa_finite(sum)); m; m &= m - 1) {
@@ -472,29 +566,17 @@ struct PackedDkvItem {
   int tile, row, hk, part;
   int h0, heads;           // query heads of this part of the group
   int tiles, n;            // query tiles of each, steps over all
+  __device__ __forceinline__ explicit PackedDkvItem(const PaItem& i)
+      : tile(i.v[0]), row(i.v[0] * PA_TILE), hk(i.v[1]), part(i.v[2]), h0(i.v[3]), heads(i.v[4]), tiles(i.v[5]), n(i.v[7]) {}
 };
-__device__ __forceinline__ PackedDkvItem pb_dkv_item(const PackedBwdParams& p, const PackedPlan& plan, int idx) {
-  PackedDkvItem it;
+__device__ __forceinline__ PaItem pb_dkv_item(const PackedBwdParams& p, const PackedPlan& plan, int idx) {
   const int per = p.Hkv * p.splits, o = idx / per, rest = idx - o * per, G = p.Hq / p.Hkv;
-  it.tile = plan.k_order[o];
-  it.hk = rest / p.splits;
-  it.part = rest - it.hk * p.splits;
-  const int a = it.part * G / p.splits, b = (it.part + 1) * G / p.splits;
-  it.h0 = it.hk * G + a;
-  it.heads = b - a;
-  it.row = it.tile * PA_TILE;
-  int hi = plan.tile_hi[it.tile];
-  if (p.window > 0) hi = min(hi, it.row + PA_TILE - 1 + p.window);
-  it.tiles = hi <= 0 ? 0 : (hi - 1) / PA_TILE - it.tile + 1;
-  it.tile = warp_uniform(it.tile);
-  it.row = warp_uniform(it.row);
-  it.hk = warp_uniform(it.hk);
-  it.part = warp_uniform(it.part);
-  it.h0 = warp_uniform(it.h0);
-  it.heads = warp_uniform(it.heads);
-  it.tiles = warp_uniform(it.tiles);
-  it.n = it.tiles * it.heads;
-  return it;
+  const int tile = plan.k_order[o], hk = rest / p.splits, part = rest - hk * p.splits;
+  const int a = part * G / p.splits, b = (part + 1) * G / p.splits;
+  int hi = plan.tile_hi[tile];
+  if (p.window > 0) hi = min(hi, tile * PA_TILE + PA_TILE - 1 + p.window);
+  const int tiles = hi <= 0 ? 0 : (hi - 1) / PA_TILE - tile + 1;
+  return {{tile, hk, part, hk * G + a, b - a, tiles, 0, tiles * (b - a)}};
 }
 
 template <int DP>
@@ -522,7 +604,12 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   uint64_t* q_empty = q_full + ST;
   uint64_t* do_full = q_empty + ST;
   uint64_t* do_empty = do_full + ST;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(do_empty + ST);
+  PaQueue queue;
+  queue.full = do_empty + ST;
+  queue.empty = queue.full + PA_SLOTS;
+  queue.want = queue.empty + PA_SLOTS;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(queue.want + 1);
+  queue.slot = reinterpret_cast<int4*>(smem + 512);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   float* lse_s = reinterpret_cast<float*>(smem + L::STAT_OFF);
   float* delta_s = lse_s + ST * PA_TILE;
@@ -532,7 +619,9 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   const int padded = (p.rows + PA_TILE - 1) / PA_TILE * PA_TILE;
 
   if (threadIdx.x == 0) {
-    for (uint64_t* b = k_full; b < do_empty + ST; ++b) mbar_init(b, b == p_full || b == ds_full ? 8 : 1);
+    for (uint64_t* b = k_full; b < queue.empty; ++b) mbar_init(b, b == p_full || b == ds_full ? 8 : 1);
+    for (int q = 0; q < PA_SLOTS; ++q) mbar_init(&queue.empty[q], 10);           // softmax warps, issuer, copies
+    mbar_init(queue.want, 1);
     *abort_flag = 0;
     fence_mbar_init();
     prefetch_tmap(&map_q);
@@ -563,10 +652,11 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           if (stat) pb_bulk_load(stat_dst, stat + (size_t)head * padded + row, PA_TILE * 4, full);
         }
       };
-      for (int r = 0; ok && r * (int)gridDim.x < items; ++r) {
-        const int idx = pa_item(r);
-        if (idx >= items) continue;
-        const PackedDkvItem it = pb_dkv_item(p, plan, idx);
+      PaReader reader;
+      PaItem next;
+      while (ok && reader.next(queue, next, abort_flag, p.status)) {
+        const PackedDkvItem it(next);
+        if (it.n < 0) break;
         if (it.n == 0) continue;
         load(k_s, &map_k, k_full, k_empty, (done & 1) ^ 1, it.hk, it.row, nullptr, nullptr);
         int head = it.h0, t = 0;
@@ -580,6 +670,8 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         }
         ++done;
       }
+    } else if (warp == 11) {
+      pa_schedule(queue, items, p.counter, [&](int idx) { return pb_dkv_item(p, plan, idx); }, abort_flag, p.status);
     } else if (warp == 8) {
       constexpr uint32_t idesc_s = make_idesc(1, 1, 0, 0, PA_TILE, PA_TILE);
       constexpr uint32_t idesc_d = make_idesc(1, 1, 0, 1, PA_TILE, DP);
@@ -587,24 +679,26 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       const uint64_t kd = make_smem_desc(smem_u32(k_s), 16, 1024, 2), vd = make_smem_desc(smem_u32(v_s), 16, 1024, 2);
       const uint64_t qd = make_smem_desc(smem_u32(q_s), 16, 1024, 2), dod = make_smem_desc(smem_u32(do_s), 16, 1024, 2);
       const uint64_t qt = make_smem_desc(smem_u32(q_s), 16384, 1024, 2), dot = make_smem_desc(smem_u32(do_s), 16384, 1024, 2);
-      bool ok = true;
-      auto lens = [&, r = 0]() mutable {
-        while (r * (int)gridDim.x < items) {
-          const int idx = pa_item(r++);
-          if (idx >= items) continue;
-          const int n = warp_uniform(pb_dkv_item(p, plan, idx).n);
-          if (n > 0) return n;
-        }
-        return 0;
-      };
+      bool ok = true, more = true;             // more: the queue has not ended
+      PaReader reader;
       // (stages and parities are counted, not computed: see elect_one)
-      StepWalk<decltype(lens)> w(lens);        // the step whose scores and dP come next
+      PbWalk w;                                // the step whose scores and dP come next
+      auto fetch = [&]() {
+        while (ok && more && w.due()) {
+          PaItem next;
+          ok = reader.next(queue, next, abort_flag, p.status);
+          const int n = warp_uniform(next.v[7]);
+          more = ok && n >= 0;
+          if (more && n > 0) w.begin(n);
+        }
+      };
+      bool done = false;                       // behind the last step
       int sa = 0, sb = 0;                      // stage of that step, of the one before
       uint32_t ph = 0, par = 0;
       auto scores = [&]() {
-        if (!ok || !w.more) return;
+        if (!ok || !more) return;
         ok = pa_wait(&q_full[sa], ph, abort_flag, p.status, ST_PATTN_Q);
-        if (w.first()) ok = ok && pa_wait(k_full, w.item_parity(), abort_flag, p.status, ST_PATTN_KV_FULL);
+        if (w.first()) ok = ok && pa_wait(k_full, w.parity(), abort_flag, p.status, ST_PATTN_KV_FULL);
         if (!ok) return;
         tc_fence_after();
         const uint64_t q0 = qd + (uint32_t)(sa * STEP);
@@ -615,9 +709,9 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         }
       };
       auto dprob = [&]() {
-        if (!ok || !w.more) return;
+        if (!ok || !more) return;
         ok = pa_wait(&do_full[sa], ph, abort_flag, p.status, ST_PATTN_Q);
-        if (w.first()) ok = ok && pa_wait(v_full, w.item_parity(), abort_flag, p.status, ST_PATTN_KV_FULL);
+        if (w.first()) ok = ok && pa_wait(v_full, w.parity(), abort_flag, p.status, ST_PATTN_KV_FULL);
         if (!ok) return;
         tc_fence_after();
         const uint64_t d0 = dod + (uint32_t)(sa * STEP);
@@ -627,11 +721,14 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           if (w.last()) umma_commit(v_empty);
         }
       };
+      fetch();
       scores();
       dprob();
-      while (ok && w.more) {
+      while (ok && w.items > 0 && !done) {
         const bool add = !w.first(), last = w.last();
-        w.advance();                           // now at the step behind this one
+        ++w.i;                                 // now at the step behind this one
+        fetch();
+        done = !more;
         sb = sa;
         if (++sa == ST) { sa = 0; ph ^= 1; }
         const uint64_t d0 = dot + (uint32_t)(sb * STEP), q0 = qt + (uint32_t)(sb * STEP);
@@ -659,13 +756,16 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     reg_inc<216>();
     const int g = warp >> 2, lg = warp & 3;
     const uint32_t base = tmem + (uint32_t(lg * 32) << 16);
-    int step = 0, done = 0;
+    int step = 0, done = 0, slot = 0;
+    uint32_t slot_parity = 0;
     bool ok = true;
     const float2 c2 = make_float2(p.scale_log2, p.scale_log2);
-    for (int r = 0; ok && r * (int)gridDim.x < items; ++r) {
-      const int idx = pa_item(r);
-      if (idx >= items) continue;
-      const PackedDkvItem it = pb_dkv_item(p, plan, idx);
+    const bool wide = p.D % 16 == 0 && ((reinterpret_cast<size_t>(p.dk) | reinterpret_cast<size_t>(p.dv)) & 31) == 0;
+    PaReader reader;
+    PaItem next;
+    while (reader.next(queue, next, abort_flag, p.status)) {
+      const PackedDkvItem it(next);
+      if (it.n < 0) break;
       const int row = it.row + lg * 32 + lane;                 // key row of this thread
       int hi = 0;                                              // one past the last query row that sees it
       if (row < p.rows) {
@@ -673,61 +773,28 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         if (p.window > 0) hi = min(hi, row + p.window);
       }
       int t = 0;
+      const int tell = max(it.n - PA_EARLY, 0);
+      if (it.n == 0 && threadIdx.x == 0) mbar_arrive(queue.want);
       for (int i = 0; i < it.n; ++i, ++step) {
         const int c0 = (it.tile + t) * PA_TILE + g * 64;       // first query row of this thread's columns
         if (++t == it.tiles) t = 0;
-        const int slot = step % ST;
-        const uint32_t slot_parity = (step / ST) & 1;
+        const PbView view(row - c0, hi - 1 - c0);
+        if (i == tell && threadIdx.x == 0) mbar_arrive(queue.want);
         ok = pa_wait(s_full, step & 1, abort_flag, p.status, ST_PATTN_S) &&
              pa_wait(&q_full[slot], slot_parity, abort_flag, p.status, ST_PATTN_Q);
         if (!ok) break;
         tc_fence_after();
         float s[64];
-        pb_load64(base + g * 64, s);
-        const float4* lse4 = reinterpret_cast<const float4*>(lse_s + slot * PA_TILE + g * 64);
-#pragma unroll
-        for (int c = 0; c < 64; c += 4) {
-          const float4 b = lse4[c / 4];
-          const float2 x = pa_fma2(make_float2(s[c], s[c + 1]), c2, make_float2(-b.x, -b.y));
-          const float2 y = pa_fma2(make_float2(s[c + 2], s[c + 3]), c2, make_float2(-b.z, -b.w));
-          s[c] = pa_exp2(x.x);
-          s[c + 1] = pa_exp2(x.y);
-          s[c + 2] = pa_exp2(y.x);
-          s[c + 3] = pa_exp2(y.y);
-        }
-        int first = max(row - c0, 0);
-        const int lastq = min(hi - 1 - c0, 63);
-        const bool none = first > lastq;
-        const bool masked = __any_sync(0xffffffffu, none || first > 0 || lastq < 63);
-        if (none) first = 1 << 20;
-        const uint32_t span = none ? 0u : (uint32_t)(lastq - first);
-        if (masked) pb_mask(s, first, span);
-        pb_store64(base + g * 64, s);
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(p_full);
+        pb_step_p<true>(base + g * 64, s, view, PbCols{reinterpret_cast<const float4*>(lse_s + slot * PA_TILE + g * 64)}, c2);
+        pb_arrive(p_full);
         ok = pa_wait(dp_full, step & 1, abort_flag, p.status, ST_PATTN_S) &&
              pa_wait(&do_full[slot], slot_parity, abort_flag, p.status, ST_PATTN_Q);
         if (!ok) break;
         tc_fence_after();
-        float u[64];
-        pb_load64(base + 128 + g * 64, u);
-        const float4* delta4 = reinterpret_cast<const float4*>(delta_s + slot * PA_TILE + g * 64);
-#pragma unroll
-        for (int c = 0; c < 64; c += 4) {
-          const float4 b = delta4[c / 4];
-          const float2 x = pa_mul2(make_float2(s[c], s[c + 1]), pa_add2(make_float2(u[c], u[c + 1]), make_float2(-b.x, -b.y)));
-          const float2 y = pa_mul2(make_float2(s[c + 2], s[c + 3]), pa_add2(make_float2(u[c + 2], u[c + 3]), make_float2(-b.z, -b.w)));
-          s[c] = x.x;
-          s[c + 1] = x.y;
-          s[c + 2] = y.x;
-          s[c + 3] = y.y;
-        }
-        if (masked) pb_mask(s, first, span);   // zero times what a hidden row holds may be no number
-        pb_store64(base + 128 + g * 64, s);
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(ds_full);
+        pb_step_ds(base + 128 + g * 64, base + 128 + g * 64, s, view,
+                   PbCols{reinterpret_cast<const float4*>(delta_s + slot * PA_TILE + g * 64)});
+        pb_arrive(ds_full);
+        if (++slot == ST) { slot = 0; slot_parity ^= 1; }
       }
       if (!ok) break;
       if (it.n > 0) {
@@ -761,16 +828,8 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
               if (c + e < p.D) *reinterpret_cast<uint4*>(part + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
           } else {
 #pragma unroll
-            for (int e = 0; e < 32; e += 8) {
-              if (c + e < p.D) {
-                uint4 v;
-                v.x = pa_pack(__uint_as_float(o[e]), __uint_as_float(o[e + 1]));
-                v.y = pa_pack(__uint_as_float(o[e + 2]), __uint_as_float(o[e + 3]));
-                v.z = pa_pack(__uint_as_float(o[e + 4]), __uint_as_float(o[e + 5]));
-                v.w = pa_pack(__uint_as_float(o[e + 6]), __uint_as_float(o[e + 7]));
-                *reinterpret_cast<uint4*>(to + c + e) = v;
-              }
-            }
+            for (int e = 0; e < 32; e += 16)
+              if (c + e < p.D) pa_put16(to + c + e, o, e, 1.f, wide, p.D - c - e);
           }
         }
       }
@@ -834,21 +893,22 @@ static int packed_bwd_launch(const CUtensorMap& mq, const CUtensorMap& mk, const
 }  // namespace slab
 
 // Into how many parts a group's heads are cut for dk and dv: a key tile's steps are a serial chain, and the longest, of
-// tiles * G steps, should be no more than half of what an SM does in all, tiles (tiles + 1) / 2 * Hq / SMs.
+// tiles * G steps, should be no more than what an SM does in all, tiles (tiles + 1) / 2 * Hq / SMs.  (8192 rows in documents of
+// 700, 32/4 heads, dk and dv in 1, 2, 4, 8 parts: 346, 275, 276, 334 us; one document, 64/8: 1755, 1789, 1884, 2171.)
 extern "C" int slab_packed_attn_splits(int rows, int hq, int hkv) {
   if (rows <= 0 || hkv <= 0 || hq % hkv) return -10;
   const long tiles = ((long)rows + slab::PA_TILE - 1) / slab::PA_TILE;
   const int group = hq / hkv;
-  const long want = (4l * slab::sm_count() + (tiles + 1) * hkv - 1) / ((tiles + 1) * hkv);
+  const long want = (2l * slab::sm_count() + (tiles + 1) * hkv - 1) / ((tiles + 1) * hkv);
   int s = want < group ? (int)want : group;
   while (group % s) ++s;
   return s;
 }
 
 // q, k, v, dout with token and head strides as in slab_packed_attn_fwd; out, dq, dk, dv contiguous; lse from the forward pass,
-// delta [Hq, tiles * 128] scratch; partial: scratch of splits * 2 * rows * Hkv * D floats where splits > 1.
+// delta [Hq, tiles * 128] and counter [2] int32 scratch; partial: scratch of splits * 2 * rows * Hkv * D floats where splits > 1.
 extern "C" int slab_packed_attn_bwd(const void* q, const void* k, const void* v, const void* out, const void* dout, const void* lse,
-                                    const void* plan, void* dq, void* dk, void* dv, void* delta, void* partial, int splits,
+                                    const void* plan, void* dq, void* dk, void* dv, void* delta, void* counter, void* partial, int splits,
                                     int rows, int hq, int hkv, int d, long q_ts, long q_hs, long k_ts, long k_hs, long v_ts,
                                     long v_hs, long do_ts, long do_hs, int window, float scale, void* status, void* stream) {
   using namespace slab;
@@ -867,7 +927,7 @@ extern "C" int slab_packed_attn_bwd(const void* q, const void* k, const void* v,
   const int padded = (rows + PA_TILE - 1) / PA_TILE * PA_TILE;
   const long units = (long)padded * hq;
   packed_delta_kernel<<<(unsigned)((units + 15) / 16), 256, 0, st>>>((const __nv_bfloat16*)out, (const __nv_bfloat16*)dout,
-                                                                     (float*)delta, rows, padded, hq, d, do_ts, do_hs);
+                                                                     (float*)delta, rows, padded, hq, d, do_ts, do_hs, (int*)counter);
   PackedBwdParams p;
   p.dq = (__nv_bfloat16*)dq;
   p.dk = (__nv_bfloat16*)dk;
@@ -883,6 +943,7 @@ extern "C" int slab_packed_attn_bwd(const void* q, const void* k, const void* v,
   p.rows = rows; p.Hq = hq; p.Hkv = hkv; p.D = d;
   p.window = window;
   p.splits = splits;
+  p.counter = (int*)counter;
   p.scale = scale;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.status = (int*)status;

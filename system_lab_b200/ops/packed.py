@@ -20,12 +20,12 @@ from . import cuda
 
 cuda.register("slab_packed_plan", "piippp")
 cuda.register("slab_packed_plan_tokens", "piilppp")
-cuda.register("slab_packed_attn_fwd", "pppppp" + "iiii" + "llllll" + "if" + "pp")
+cuda.register("slab_packed_attn_fwd", "pppppp" + "iiii" + "llllll" + "if" + "ppp")
 cuda.register("slab_packed_attn_splits", "iii")
-cuda.register("slab_packed_attn_bwd", "p" * 12 + "i" + "iiii" + "llllllll" + "if" + "pp")
+cuda.register("slab_packed_attn_bwd", "p" * 13 + "i" + "iiii" + "llllllll" + "if" + "pp")
 cuda._KERNELS_PER_CALL.update({"slab_packed_plan": 2, "slab_packed_plan_tokens": 3, "slab_packed_attn_bwd": 3})
 cuda._STATUS_NAMES.update({40: "PACKED_ATTN_Q", 41: "PACKED_ATTN_KV_FULL", 42: "PACKED_ATTN_EMPTY", 43: "PACKED_ATTN_S",
-                           44: "PACKED_ATTN_P", 45: "PACKED_ATTN_OUT"})
+                           44: "PACKED_ATTN_P", 45: "PACKED_ATTN_OUT", 46: "PACKED_ATTN_ITEM"})
 
 TILE = 128
 
@@ -147,14 +147,16 @@ def _strides(t):
 
 
 def forward(q, k, v, documents: PackedDocuments, scale: float, window: int = 0):
-    """``(out [rows, Hq, d], lse [Hq, tiles * 128])``, ``lse`` the base-2 log-sum-exp of the scaled scores."""
+    """``(out [rows, Hq, d], lse)``, ``lse`` the base-2 log-sum-exp of the scaled scores, ``[Hq, tiles * 128]`` flat, with the
+    kernel's work counter behind it."""
     rows, hq, d = q.shape
     out = torch.empty((rows, hq, d), dtype=q.dtype, device=q.device)
-    lse = torch.empty((hq, (rows + TILE - 1) // TILE * TILE), dtype=torch.float32, device=q.device)
+    stats = hq * ((rows + TILE - 1) // TILE * TILE)
+    lse = torch.empty(stats + 1, dtype=torch.float32, device=q.device)
     window = min(int(window), rows)
     with cuda.on_device(q):
         cuda.call("slab_packed_attn_fwd", q, k, v, out, lse, documents.plan, rows, hq, k.shape[1], d, *_strides(q),
-                  *_strides(k), *_strides(v), window, scale, cuda.status_word(q.device), cuda.stream())
+                  *_strides(k), *_strides(v), window, scale, lse.data_ptr() + 4 * stats, cuda.status_word(q.device), cuda.stream())
     return out, lse
 
 
@@ -167,12 +169,13 @@ def backward(q, k, v, out, lse, dout, documents: PackedDocuments, scale: float, 
     dq = torch.empty((rows, hq, d), dtype=q.dtype, device=q.device)
     dk = torch.empty((rows, hkv, d), dtype=q.dtype, device=q.device)
     dv = torch.empty_like(dk)
-    delta = torch.empty_like(lse)
+    stats = lse.numel() - 1
+    delta = torch.empty(stats + 2, dtype=torch.float32, device=q.device)
     window = min(int(window), rows)
     with cuda.on_device(q):
         splits = cuda.lib().slab_packed_attn_splits(rows, hq, hkv)
         partial = torch.empty(splits * 2 * dk.numel(), dtype=torch.float32, device=q.device) if splits > 1 else None
-        cuda.call("slab_packed_attn_bwd", q, k, v, out, dout, lse, documents.plan, dq, dk, dv, delta, partial, splits, rows,
+        cuda.call("slab_packed_attn_bwd", q, k, v, out, dout, lse, documents.plan, dq, dk, dv, delta, delta.data_ptr() + 4 * stats, partial, splits, rows,
                   hq, hkv, d, *_strides(q), *_strides(k), *_strides(v), *_strides(dout), window, scale,
                   cuda.status_word(q.device), cuda.stream())
         if splits > 1:
