@@ -40,25 +40,47 @@ __device__ __forceinline__ void pb_bulk_load(void* dst, const void* src, uint32_
 }
 
 // ================================================================ delta
-// A group of 16 lanes per (row, head); rows behind the buffer's end, up to whole tiles, get zero.
+// DP / 8 lanes per head, eight neighbouring rows each, all of whose loads are in flight together; heads fastest, so that a block
+// reads whole lines.  Rows behind the buffer's end, up to whole tiles, get zero.
+template <int DP>
 __global__ void __launch_bounds__(256)
 packed_delta_kernel(const __nv_bfloat16* out, const __nv_bfloat16* dout, float* delta, int rows, int padded, int hq, int d,
                     long do_ts, long do_hs, int* counter) {
   if (blockIdx.x == 0 && threadIdx.x < 2) counter[threadIdx.x] = 0;    // of the two kernels behind this one
-  const long unit = (long)blockIdx.x * 16 + (threadIdx.x >> 4);          // rows fastest: neighbours write side by side
-  const int sub = threadIdx.x & 15;
-  const int head = (int)(unit / padded), row = (int)(unit - (long)head * padded);
-  float sum = 0.f;
-  if (head < hq && row < rows && sub * 8 < d) {
-    float a[8], b[8];
-    unpack8(*reinterpret_cast<const bf16x8*>(out + ((size_t)row * hq + head) * d + sub * 8), a);
-    unpack8(*reinterpret_cast<const bf16x8*>(dout + (size_t)row * do_ts + (size_t)head * do_hs + sub * 8), b);
+  constexpr int LANES = DP / 8, ROWS = 8;
+  const long unit = (long)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+  const int c = (threadIdx.x % LANES) * 8;
+  const int head = (int)(unit % hq), row0 = (int)(unit / hq) * ROWS;
+  if (row0 >= padded) return;                  // (units of a warp end together: 32 / LANES divides ROWS of padded's 128)
+  uint4 o[ROWS], g[ROWS];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum = fmaf(a[i], b[i], sum);
+  for (int i = 0; i < ROWS; ++i) {
+    o[i] = g[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (row0 + i < rows && c < d) {
+      o[i] = __ldg(reinterpret_cast<const uint4*>(out + ((size_t)(row0 + i) * hq + head) * d + c));
+      g[i] = __ldg(reinterpret_cast<const uint4*>(dout + (size_t)(row0 + i) * do_ts + (size_t)head * do_hs + c));
+    }
+  }
+  float sum[ROWS];
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    float x[8], y[8];
+    unpack8(*reinterpret_cast<const bf16x8*>(&o[i]), x);
+    unpack8(*reinterpret_cast<const bf16x8*>(&g[i]), y);
+    sum[i] = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum[i] = fmaf(x[e], y[e], sum[i]);
   }
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (sub == 0 && head < hq) delta[(size_t)head * padded + row] = sum;
+  for (int i = 0; i < ROWS; ++i) {
+#pragma unroll
+    for (int k = LANES / 2; k > 0; k >>= 1) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], k);
+  }
+  if (threadIdx.x % LANES == 0) {
+    float4* to = reinterpret_cast<float4*>(delta + (size_t)head * padded + row0);
+    to[0] = make_float4(sum[0], sum[1], sum[2], sum[3]);
+    to[1] = make_float4(sum[4], sum[5], sum[6], sum[7]);
+  }
 }
 
 // ================================================================ common to both
@@ -925,9 +947,13 @@ extern "C" int slab_packed_attn_bwd(const void* q, const void* k, const void* v,
   if ((rc = pa_make_map(&mdo, dout, rows, hq, d, do_ts, do_hs)) != 0) return rc;
   cudaStream_t st = (cudaStream_t)stream;
   const int padded = (rows + PA_TILE - 1) / PA_TILE * PA_TILE;
-  const long units = (long)padded * hq;
-  packed_delta_kernel<<<(unsigned)((units + 15) / 16), 256, 0, st>>>((const __nv_bfloat16*)out, (const __nv_bfloat16*)dout,
-                                                                     (float*)delta, rows, padded, hq, d, do_ts, do_hs, (int*)counter);
+  const long units = (long)padded / 8 * hq, per = d <= 64 ? 32 : 16;
+  if (d <= 64)
+    packed_delta_kernel<64><<<(unsigned)((units + per - 1) / per), 256, 0, st>>>((const __nv_bfloat16*)out, (const __nv_bfloat16*)dout,
+        (float*)delta, rows, padded, hq, d, do_ts, do_hs, (int*)counter);
+  else
+    packed_delta_kernel<128><<<(unsigned)((units + per - 1) / per), 256, 0, st>>>((const __nv_bfloat16*)out, (const __nv_bfloat16*)dout,
+        (float*)delta, rows, padded, hq, d, do_ts, do_hs, (int*)counter);
   PackedBwdParams p;
   p.dq = (__nv_bfloat16*)dq;
   p.dk = (__nv_bfloat16*)dk;

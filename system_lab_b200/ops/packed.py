@@ -170,14 +170,14 @@ def backward(q, k, v, out, lse, dout, documents: PackedDocuments, scale: float, 
     dk = torch.empty((rows, hkv, d), dtype=q.dtype, device=q.device)
     dv = torch.empty_like(dk)
     stats = lse.numel() - 1
-    delta = torch.empty(stats + 2, dtype=torch.float32, device=q.device)
+    delta = torch.empty(stats + 2, dtype=torch.float32, device=q.device)          # and two work counters
     window = min(int(window), rows)
     with cuda.on_device(q):
         splits = cuda.lib().slab_packed_attn_splits(rows, hq, hkv)
         partial = torch.empty(splits * 2 * dk.numel(), dtype=torch.float32, device=q.device) if splits > 1 else None
-        cuda.call("slab_packed_attn_bwd", q, k, v, out, dout, lse, documents.plan, dq, dk, dv, delta, delta.data_ptr() + 4 * stats, partial, splits, rows,
-                  hq, hkv, d, *_strides(q), *_strides(k), *_strides(v), *_strides(dout), window, scale,
-                  cuda.status_word(q.device), cuda.stream())
+        cuda.call("slab_packed_attn_bwd", q, k, v, out, dout, lse, documents.plan, dq, dk, dv, delta,
+                  delta.data_ptr() + 4 * stats, partial, splits, rows, hq, hkv, d, *_strides(q), *_strides(k), *_strides(v),
+                  *_strides(dout), window, scale, cuda.status_word(q.device), cuda.stream())
         if splits > 1:
             cuda.LAUNCHES[0] += 1
     return dq, dk, dv
@@ -200,4 +200,6 @@ class _PackedAttention(torch.autograd.Function):
 
 
 def attention(q, k, v, documents: PackedDocuments, scale: float, window: int = 0):
+    if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)):
+        return forward(_readable(q), _readable(k), _readable(v), documents, scale, window)[0]
     return _PackedAttention.apply(q, k, v, documents, scale, window)
