@@ -7,8 +7,8 @@
 // tile sees are the tiles from its least lo to its own, whatever documents lie in it, and many short documents share one
 // tile.  Rows of no document get zeros.
 //
-// Roles (384 threads, one persistent block per SM): warps 0-3 and 4-7 softmax, one query tile of 128 rows each, a row per
-// thread; warp 8 issues the MMAs, warp 9 the copies.  The two query tiles share the key and value tiles: two heads of one
+// Roles (512 threads, one persistent block per SM): warps 0-3 and 4-7 softmax, one query tile of 128 rows each, a row per
+// thread; warp 8 issues the MMAs, warp 9 the copies, warp 11 takes items; warps 12-15 store finished rows.  The two query tiles share the key and value tiles: two heads of one
 // group on the same rows where the group is even (nothing is masked for one tile only), else the next 128 rows.
 // S and O live in tensor memory (2 x 128 + 2 x DP columns).  The probabilities go back over the scores they came from, as
 // bf16, and are the A operand of P V from there.  While one tile's softmax runs, the tensor cores do P V of the other
@@ -150,7 +150,7 @@ __global__ void packed_order_kernel(int rows, int* base) {
 }
 
 // ================================================================ forward
-constexpr int PF_THREADS = 384;
+constexpr int PF_THREADS = 512;
 constexpr int PF_EVERY = 8;                   // of that many pairs of exponentials, one is made on the multiply-add units
 constexpr float PF_SLACK = 8.f;              // a row's maximum may be this far (log2) below the true one
 
@@ -173,7 +173,7 @@ template <int DP>
 struct PackedFwdSmem {
   static constexpr int TILE = PA_TILE * DP * 2;
   static constexpr int STAGES = DP == 128 ? 2 : 4;
-  static constexpr int Q_OFF = 1024, KV_OFF = Q_OFF + 2 * TILE, TOTAL = KV_OFF + STAGES * 2 * TILE;
+  static constexpr int STAT_OFF = 1024, Q_OFF = STAT_OFF + 4096, KV_OFF = Q_OFF + 2 * TILE, TOTAL = KV_OFF + STAGES * 2 * TILE;
   static_assert(TOTAL <= 232448, "shared memory budget");
 };
 
@@ -370,12 +370,15 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   uint64_t* p_full = s_full + 2;
   uint64_t* o_full = p_full + 2;
   PaQueue queue;
-  queue.full = o_full + 2;
+  uint64_t* o_empty = o_full + 2;
+  uint64_t* l_full = o_empty + 2;
+  queue.full = l_full + 2;
   queue.empty = queue.full + PA_SLOTS;
   queue.want = queue.empty + PA_SLOTS;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(queue.want + 1);
   queue.slot = reinterpret_cast<int4*>(smem + 512);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  float2* stat_s = reinterpret_cast<float2*>(smem + L::STAT_OFF);       // [2 items][2 tiles][128] sum and maximum of a row
   uint8_t* q_s = smem + L::Q_OFF;
   uint8_t* kv_s = smem + L::KV_OFF;
   const int warp = warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -388,6 +391,8 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       mbar_init(&s_full[g], 1);
       mbar_init(&p_full[g], 4);
       mbar_init(&o_full[g], 1);
+      mbar_init(&o_empty[g], 4);
+      mbar_init(&l_full[g], 4);
     }
     for (int s = 0; s < NST; ++s) {
       mbar_init(&kv_full[s], 1);
@@ -395,7 +400,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     }
     for (int q = 0; q < PA_SLOTS; ++q) {
       mbar_init(&queue.full[q], 1);
-      mbar_init(&queue.empty[q], 10);          // softmax warps, issuer, copies
+      mbar_init(&queue.empty[q], 14);          // softmax warps, output warps, issuer, copies
     }
     mbar_init(queue.want, 1);
     *abort_flag = 0;
@@ -413,8 +418,8 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;            // S of tile g at 128 g, O at 256 + 128 g
 
-  if (warp >= 8) {
-    reg_dec<72>();
+  if (warp >= 8 && warp < 12) {
+    reg_dec<48>();
     if (warp == 9) {
       // ------------------------------------------------------------ copies
       int st = 0, done = 0;                    // stage, items before this one
@@ -479,7 +484,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       // and parities are counted, not computed: what the issued instructions take has to be plainly the same in all lanes,
       // see elect_one.)
       int st = 0;
-      uint32_t ph = 0, pph = 0, qph = 0;
+      uint32_t ph = 0, pph = 0, qph = 0, oph = 1;
       int n = next_len(), i = 0;               // the step whose P V comes next: i of n
       bool last = n == 1;
       if (n > 0) {                             // scores of the first step
@@ -506,7 +511,8 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         const uint64_t v0 = vd + (uint32_t)(st * 2 * STEP), k0 = kd + (uint32_t)(st * 2 * STEP);
         const uint32_t fresh = i != 0 ? 1u : 0u;
         const int s0 = st;
-        ok = pa_wait(&p_full[0], pph, abort_flag, p.status, ST_PATTN_P);
+        if (i == 0) ok = pa_wait(&o_empty[0], oph, abort_flag, p.status, ST_PATTN_OUT);
+        ok = ok && pa_wait(&p_full[0], pph, abort_flag, p.status, ST_PATTN_P);
         if (!ok) break;
         tc_fence_after();
         if (elect_one()) {
@@ -526,6 +532,10 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           if (ends) umma_commit(&q_empty[0]);
         }
         if (more && last) ok = ok && pa_wait(&q_full[1], qph, abort_flag, p.status, ST_PATTN_Q);
+        if (i == 0) {
+          ok = ok && pa_wait(&o_empty[1], oph, abort_flag, p.status, ST_PATTN_OUT);
+          oph ^= 1;
+        }
         if (last) qph ^= 1;
         i = last ? 0 : i + 1;
         n = after;
@@ -550,23 +560,21 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         }
       }
     }
-  } else {
-    reg_inc<216>();
+  } else if (warp < 8) {
+    reg_inc<192>();
     // ------------------------------------------------------------ softmax: a query row per thread
     const int g = warp >> 2, lg = warp & 3;
     const int r128 = lg * 32 + lane;
     const uint32_t s_addr = tmem + g * 128 + (uint32_t(lg * 32) << 16);
     const uint32_t o_addr = tmem + 256 + g * 128 + (uint32_t(lg * 32) << 16);
-    const int tiles = (p.rows + PA_TILE - 1) / PA_TILE;
-    int step = 0, done = 0;
+    int step = 0, buf = 0;
     bool ok = true;
-    const bool wide = p.D % 16 == 0 && (reinterpret_cast<size_t>(p.out) & 31) == 0;
     PaReader reader;
     PaItem next;
     while (reader.next(queue, next, abort_flag, p.status)) {
       const PackedFwdItem it(next);
       if (it.n < 0) break;
-      const int row = it.row[g] + r128, head = it.head[g];
+      const int row = it.row[g] + r128;
       int lo = PA_NONE;                        // first key of this row
       if (row < p.rows) {
         lo = plan.doc_lo[row];
@@ -599,43 +607,81 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           pf_part<DP>(s_addr, o_addr, p.scale_log2, vis, first, lastk, m, la, lb, &p_full[g]);
       }
       if (!ok) break;
-      const float l = (la.x + la.y) + (lb.x + lb.y);
-      const float inv = 1.f / l;               // (a row that sees nothing gets zeros)
-      if (it.n > 0) {
-        ok = pa_wait(&o_full[g], done & 1, abort_flag, p.status, ST_PATTN_OUT);
-        if (!ok) break;
-        tc_fence_after();
-        ++done;
-      }
-      __nv_bfloat16* o_row = p.out + ((size_t)row * p.Hq + head) * p.D;
-      float sum = l;                           // finite if all of the row is (or as good as: else it is made again for nothing)
-#pragma unroll
-      for (int c = 0; c < DP; c += 32) {
-        uint32_t o[32];
-        if (it.n > 0) {
-          tmem_ld_32x32(o_addr + c, o);
-          tmem_ld_wait();
-        }
-#pragma unroll
-        for (int k = 0; k < 32; ++k) sum += fabsf(__uint_as_float(o[k]));
-        if (!sees) {
-#pragma unroll
-          for (int k = 0; k < 32; ++k) o[k] = 0u;
-        }
-        if (row < p.rows) {
-          const float f = sees ? inv : 0.f;
-#pragma unroll
-          for (int k = 0; k < 32; k += 16)
-            if (c + k < p.D) pa_put16(o_row + c + k, o, k, f, wide, p.D - c - k);
-        }
-      }
-      if (it.row[g] < tiles * PA_TILE)
-        p.lse[(size_t)head * tiles * PA_TILE + row] = sees ? m + log2f(l) : INFINITY;
-      for (uint32_t again = __ballot_sync(0xffffffffu, sees && !(pa_finite(sum) && l > 0.f)); again; again &= again - 1) {
-        const int who = __ffs(again) - 1;
+      if (it.n > 0) {                          // (the output warps are done with what the item before the last one left there)
+        stat_s[(buf * 2 + g) * 128 + r128] = make_float2((la.x + la.y) + (lb.x + lb.y), m);
+        buf ^= 1;
         __syncwarp();
-        pf_redo(p, it.row[g] + lg * 32 + who, head, __shfl_sync(0xffffffffu, lo, who));
+        if (lane == 0) mbar_arrive(&l_full[g]);
       }
+    }
+  } else {
+    reg_dec<80>();
+    // ------------------------------------------------------------ output: both tiles of an item, while the softmax warps are at
+    // the next one (the time between an item's last probabilities and its stored rows is some 5 thousand cycles)
+    const int lg = warp & 3, r128 = lg * 32 + lane;
+    const int tiles = (p.rows + PA_TILE - 1) / PA_TILE;
+    const bool wide = p.D % 16 == 0 && (reinterpret_cast<size_t>(p.out) & 31) == 0;
+    int done = 0;
+    bool ok = true;
+    PaReader reader;
+    PaItem next;
+    while (ok && reader.next(queue, next, abort_flag, p.status)) {
+      const PackedFwdItem it(next);
+      if (it.n < 0) break;
+#pragma unroll 1
+      for (int g = 0; g < 2 && ok; ++g) {
+        const int row = (g ? it.row[1] : it.row[0]) + r128, head = g ? it.head[1] : it.head[0];
+        int lo = PA_NONE;                      // first key of this row
+        if (row < p.rows) {
+          lo = plan.doc_lo[row];
+          if (p.window > 0) lo = max(lo, row - p.window + 1);
+        }
+        const bool sees = lo <= row;           // (a row that sees nothing gets zeros)
+        float l = 0.f, m = 0.f;
+        if (it.n > 0) {
+          ok = pa_wait(&l_full[g], done & 1, abort_flag, p.status, ST_PATTN_OUT) &&
+               pa_wait(&o_full[g], done & 1, abort_flag, p.status, ST_PATTN_OUT);
+          if (!ok) break;
+          tc_fence_after();
+          const float2 st = stat_s[((done & 1) * 2 + g) * 128 + r128];
+          l = st.x;
+          m = st.y;
+        }
+        const uint32_t o_addr = tmem + 256 + g * 128 + (uint32_t(lg * 32) << 16);
+        __nv_bfloat16* o_row = p.out + ((size_t)row * p.Hq + head) * p.D;
+        const float f = sees ? 1.f / l : 0.f;
+        float sum = l;                         // finite if all of the row is (or as good as: else it is made again for nothing)
+#pragma unroll 1
+        for (int c = 0; c < DP; c += 32) {
+          uint32_t o[32];
+          if (it.n > 0) {
+            tmem_ld_32x32(o_addr + c, o);
+            tmem_ld_wait();
+            if (c + 32 == DP) {                // all read: the next item's products may come
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&o_empty[g]);
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < 32; ++k) {
+            if (!sees) o[k] = 0u;
+            sum += fabsf(__uint_as_float(o[k]));
+          }
+          if (row < p.rows) {
+#pragma unroll
+            for (int k = 0; k < 32; k += 16)
+              if (c + k < p.D) pa_put16(o_row + c + k, o, k, f, wide, p.D - c - k);
+          }
+        }
+        if (row < tiles * PA_TILE) p.lse[(size_t)head * tiles * PA_TILE + row] = sees ? m + log2f(l) : INFINITY;
+        for (uint32_t again = __ballot_sync(0xffffffffu, sees && !(pa_finite(sum) && l > 0.f)); again; again &= again - 1) {
+          const int who = __ffs(again) - 1;
+          __syncwarp();
+          pf_redo(p, row - lane + who, head, __shfl_sync(0xffffffffu, lo, who));
+        }
+      }
+      if (it.n > 0) ++done;
     }
   }
 

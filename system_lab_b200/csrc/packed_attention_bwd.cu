@@ -7,15 +7,15 @@
 // scores and their gradient again (7 products of 128 x 128 x D a tile pair where one kernel could do with 5), but no sum
 // leaves the tensor cores before it is whole: no atomics, no fp32 copy of dq, and the same bits every time.
 //
-// Roles as in the forward pass (384 threads): warps 0-3 and 4-7 take the left and the right 64 columns of every 128 x 128
-// tile, a row per thread; warp 8 issues the MMAs, warp 9 the copies.  p and ds go back over the scores and products they
+// Roles as in the forward pass (512 threads): warps 0-3 and 4-7 take the left and the right 64 columns of every 128 x 128
+// tile, a row per thread; warp 8 issues the MMAs, warp 9 the copies, warp 11 takes items; warps 12-15 store what is finished.  p and ds go back over the scores and products they
 // came from, as bf16, and are the A operand of the next product from tensor memory.  Statistics, p - delta and all sums
 // are fp32; p and ds are rounded to bf16 once, as operands.
 #include "packed_attention.cuh"
 
 namespace slab {
 
-constexpr int PB_THREADS = 384;
+constexpr int PB_THREADS = 512;
 constexpr int PB_EVERY = 8;                  // of that many pairs of exponentials, one is made on the multiply-add units
 
 struct PackedBwdParams {
@@ -264,8 +264,8 @@ __device__ __forceinline__ float2 pb_pair(const PackedBwdParams& p, int head, in
   const float prob = pa_exp2(fmaf(pa_dot4(q, k), p.scale_log2, -p.lse[at]));
   return make_float2(prob, prob * (pa_dot4(dout, v) - p.delta[at]));
 }
-// Columns c0 .. c0 + cols - 1 of dq of one row, over its visible keys lo .. row alone (a whole warp)
-__device__ __noinline__ void pb_redo_dq(const PackedBwdParams& p, int row, int head, int lo, int c0, int cols) {
+// dq of one row over its visible keys lo .. row alone (a whole warp)
+__device__ __noinline__ void pb_redo_dq(const PackedBwdParams& p, int row, int head, int lo) {
   const int hk = head / (p.Hq / p.Hkv);
   const float4 q = pa_row4(p.q, row, head, p.D), dout = pa_row4(p.dout, row, head, p.D);
   float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -275,8 +275,7 @@ __device__ __noinline__ void pb_redo_dq(const PackedBwdParams& p, int row, int h
     pa_add4(sum, ds, k);
     if (pa_nan(ds)) { sum = make_float4(ds, ds, ds, ds); break; }
   }
-  if ((uint32_t)((threadIdx.x & 31) * 4 - c0) < (uint32_t)cols)
-    pa_put4(p.dq + ((size_t)row * p.Hq + head) * p.D, p.D, sum, p.scale);
+  pa_put4(p.dq + ((size_t)row * p.Hq + head) * p.D, p.D, sum, p.scale);
 }
 // dk or dv of one key row for heads h0 .. h0 + heads - 1 over the queries row .. hi - 1 alone (a whole warp)
 __device__ __noinline__ void pb_redo_dkv(const PackedBwdParams& p, bool dv, int row, int hk, int h0, int heads, int part, int hi) {
@@ -329,7 +328,8 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   uint64_t* v_full = k_empty + KST;
   uint64_t* v_empty = v_full + VST;
   PaQueue queue;
-  queue.full = v_empty + VST;
+  uint64_t* dq_empty = v_empty + VST;
+  queue.full = dq_empty + 1;
   queue.empty = queue.full + PA_SLOTS;
   queue.want = queue.empty + PA_SLOTS;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(queue.want + 1);
@@ -341,8 +341,8 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   const PackedPlan plan = packed_plan(p.plan, p.rows);
 
   if (threadIdx.x == 0) {
-    for (uint64_t* b = q_full; b < queue.empty; ++b) mbar_init(b, b == ds_full ? 8 : 1);
-    for (int q = 0; q < PA_SLOTS; ++q) mbar_init(&queue.empty[q], 10);           // softmax warps, issuer, copies
+    for (uint64_t* b = q_full; b < queue.empty; ++b) mbar_init(b, b == ds_full ? 8 : b == dq_empty ? 4 : 1);
+    for (int q = 0; q < PA_SLOTS; ++q) mbar_init(&queue.empty[q], 14);           // softmax warps, output warps, issuer, copies
     mbar_init(queue.want, 1);
     *abort_flag = 0;
     fence_mbar_init();
@@ -360,8 +360,8 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;            // S at 0 and 128 in turn, dP at 256, dQ at 384
 
-  if (warp >= 8) {
-    reg_dec<72>();
+  if (warp >= 8 && warp < 12) {
+    reg_dec<80>();
     if (warp == 9) {
       int pos = 0, done = 0;
       bool ok = true;
@@ -462,7 +462,8 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       scores();
       need_v();
       while (ok && follow(wq)) {
-        ok = pa_wait(ds_full, dsph, abort_flag, p.status, ST_PATTN_P);
+        if (wq.first()) ok = pa_wait(dq_empty, wq.parity() ^ 1, abort_flag, p.status, ST_PATTN_OUT);
+        ok = ok && pa_wait(ds_full, dsph, abort_flag, p.status, ST_PATTN_P);
         if (!ok) break;
         tc_fence_after();
         const uint64_t k0 = kt + (uint32_t)(sq * STEP);
@@ -484,14 +485,13 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         if (++sq == KST) sq = 0;
       }
     }
-  } else {
-    reg_inc<216>();
+  } else if (warp < 8) {
+    reg_inc<176>();
     const int g = warp >> 2, lg = warp & 3;
     const uint32_t base = tmem + (uint32_t(lg * 32) << 16);
     const int padded = (p.rows + PA_TILE - 1) / PA_TILE * PA_TILE;
-    int step = 0, done = 0;
+    int step = 0;
     bool ok = true;
-    const bool wide = p.D % 16 == 0 && (reinterpret_cast<size_t>(p.dq) & 31) == 0;
     PaReader reader;
     PaItem next;
     while (reader.next(queue, next, abort_flag, p.status)) {
@@ -525,27 +525,49 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         pb_arrive(ds_full);
       }
       if (!ok) break;
+    }
+  } else {
+    reg_dec<80>();
+    // output warps, a row per thread: dq of an item while the softmax warps are at the next one
+    const int lg = warp & 3;
+    const uint32_t base = tmem + 384 + (uint32_t(lg * 32) << 16);
+    const bool wide = p.D % 16 == 0 && (reinterpret_cast<size_t>(p.dq) & 31) == 0;
+    int done = 0;
+    PaReader reader;
+    PaItem next;
+    while (reader.next(queue, next, abort_flag, p.status)) {
+      const PackedDqItem it(next);
+      if (it.n < 0) break;
+      const int row = it.row + lg * 32 + lane;
+      int lo = PA_NONE;
+      if (row < p.rows) {
+        lo = plan.doc_lo[row];
+        if (p.window > 0) lo = max(lo, row - p.window + 1);
+      }
+      const bool sees = lo <= row;
       if (it.n > 0) {
-        ok = pa_wait(dq_full, done & 1, abort_flag, p.status, ST_PATTN_OUT);
-        if (!ok) break;
+        if (!pa_wait(dq_full, done & 1, abort_flag, p.status, ST_PATTN_OUT)) break;
         tc_fence_after();
         ++done;
       }
       __nv_bfloat16* dq_row = p.dq + ((size_t)row * p.Hq + it.head) * p.D;
       float sum = 0.f;
-#pragma unroll
-      for (int k = 0; k < DP / 2; k += 32) {
-        const int c = g * (DP / 2) + k;
+#pragma unroll 1
+      for (int c = 0; c < DP; c += 32) {
         uint32_t o[32];
         if (it.n > 0) {
-          tmem_ld_32x32(base + 384 + c, o);
+          tmem_ld_32x32(base + c, o);
           tmem_ld_wait();
+          if (c + 32 == DP) {                  // all read: the next item's products may come
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(dq_empty);
+          }
         }
 #pragma unroll
-        for (int e = 0; e < 32; ++e) sum += fabsf(__uint_as_float(o[e]));
-        if (!sees) {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = 0u;
+        for (int e = 0; e < 32; ++e) {
+          if (!sees) o[e] = 0u;
+          sum += fabsf(__uint_as_float(o[e]));
         }
         if (row < p.rows) {
 #pragma unroll
@@ -556,7 +578,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       for (uint32_t m = __ballot_sync(0xffffffffu, sees && !pa_finite(sum)); m; m &= m - 1) {
         const int who = __ffs(m) - 1;
         __syncwarp();
-        pb_redo_dq(p, it.row + lg * 32 + who, it.head, __shfl_sync(0xffffffffu, lo, who), g * (DP / 2), DP / 2);
+        pb_redo_dq(p, it.row + lg * 32 + who, it.head, __shfl_sync(0xffffffffu, lo, who));
       }
     }
   }
@@ -627,7 +649,8 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   uint64_t* do_full = q_empty + ST;
   uint64_t* do_empty = do_full + ST;
   PaQueue queue;
-  queue.full = do_empty + ST;
+  uint64_t* out_empty = do_empty + ST;
+  queue.full = out_empty + 1;
   queue.empty = queue.full + PA_SLOTS;
   queue.want = queue.empty + PA_SLOTS;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(queue.want + 1);
@@ -641,8 +664,8 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   const int padded = (p.rows + PA_TILE - 1) / PA_TILE * PA_TILE;
 
   if (threadIdx.x == 0) {
-    for (uint64_t* b = k_full; b < queue.empty; ++b) mbar_init(b, b == p_full || b == ds_full ? 8 : 1);
-    for (int q = 0; q < PA_SLOTS; ++q) mbar_init(&queue.empty[q], 10);           // softmax warps, issuer, copies
+    for (uint64_t* b = k_full; b < queue.empty; ++b) mbar_init(b, b == p_full || b == ds_full ? 8 : b == out_empty ? 4 : 1);
+    for (int q = 0; q < PA_SLOTS; ++q) mbar_init(&queue.empty[q], 14);           // softmax warps, output warps, issuer, copies
     mbar_init(queue.want, 1);
     *abort_flag = 0;
     fence_mbar_init();
@@ -660,8 +683,8 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;            // S^T at 0, dP^T at 128, dV at 256, dK at 384
 
-  if (warp >= 8) {
-    reg_dec<72>();
+  if (warp >= 8 && warp < 12) {
+    reg_dec<80>();
     if (warp == 9) {
       int pos = 0, done = 0;
       bool ok = true;
@@ -748,13 +771,14 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       dprob();
       while (ok && w.items > 0 && !done) {
         const bool add = !w.first(), last = w.last();
+        if (!add) ok = pa_wait(out_empty, w.parity() ^ 1, abort_flag, p.status, ST_PATTN_OUT);
         ++w.i;                                 // now at the step behind this one
         fetch();
         done = !more;
         sb = sa;
         if (++sa == ST) { sa = 0; ph ^= 1; }
         const uint64_t d0 = dot + (uint32_t)(sb * STEP), q0 = qt + (uint32_t)(sb * STEP);
-        ok = pa_wait(p_full, par, abort_flag, p.status, ST_PATTN_P);
+        ok = ok && pa_wait(p_full, par, abort_flag, p.status, ST_PATTN_P);
         if (!ok) break;
         tc_fence_after();
         if (elect_one()) {
@@ -774,15 +798,14 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         par ^= 1;
       }
     }
-  } else {
-    reg_inc<216>();
+  } else if (warp < 8) {
+    reg_inc<176>();
     const int g = warp >> 2, lg = warp & 3;
     const uint32_t base = tmem + (uint32_t(lg * 32) << 16);
-    int step = 0, done = 0, slot = 0;
+    int step = 0, slot = 0;
     uint32_t slot_parity = 0;
     bool ok = true;
     const float2 c2 = make_float2(p.scale_log2, p.scale_log2);
-    const bool wide = p.D % 16 == 0 && ((reinterpret_cast<size_t>(p.dk) | reinterpret_cast<size_t>(p.dv)) & 31) == 0;
     PaReader reader;
     PaItem next;
     while (reader.next(queue, next, abort_flag, p.status)) {
@@ -819,46 +842,77 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         if (++slot == ST) { slot = 0; slot_parity ^= 1; }
       }
       if (!ok) break;
+    }
+  } else {
+    reg_dec<80>();
+    // output warps, a row per thread: dV, then dK of an item while the softmax warps are at the next one
+    const int lg = warp & 3;
+    const uint32_t base = tmem + 256 + (uint32_t(lg * 32) << 16);
+    const bool wide = p.D % 16 == 0 && ((reinterpret_cast<size_t>(p.dk) | reinterpret_cast<size_t>(p.dv)) & 31) == 0;
+    int done = 0;
+    PaReader reader;
+    PaItem next;
+    while (reader.next(queue, next, abort_flag, p.status)) {
+      const PackedDkvItem it(next);
+      if (it.n < 0) break;
+      const int row = it.row + lg * 32 + lane;                 // key row of this thread
+      int hi = 0;                                              // one past the last query row that sees it
+      if (row < p.rows) {
+        hi = plan.doc_hi[row];
+        if (p.window > 0) hi = min(hi, row + p.window);
+      }
+      const bool any = hi > row;
       if (it.n > 0) {
-        ok = pa_wait(out_full, done & 1, abort_flag, p.status, ST_PATTN_OUT);
-        if (!ok) break;
+        if (!pa_wait(out_full, done & 1, abort_flag, p.status, ST_PATTN_OUT)) break;
         tc_fence_after();
         ++done;
       }
-      // the first group of warps writes dV, the second dK
-      const bool any = hi > row;
-      const float f = g == 0 ? 1.f : p.scale;
       const size_t at = ((size_t)row * p.Hkv + it.hk) * p.D;
-      __nv_bfloat16* to = (g == 0 ? p.dv : p.dk) + at;
-      float* part = p.partial + ((size_t)(2 * it.part + (g == 0)) * p.rows * p.Hkv) * p.D + at;
-      float sum = 0.f;
+      float bad[2] = {0.f, 0.f};
 #pragma unroll
-      for (int c = 0; c < DP; c += 32) {
-        uint32_t o[32];
-        if (it.n > 0) {
-          tmem_ld_32x32(base + 256 + (g == 0 ? 0 : 128) + c, o);
-          tmem_ld_wait();
-        }
+      for (int which = 0; which < 2; ++which) {                // dV, dK
+        const float f = which == 0 ? 1.f : p.scale;
+        __nv_bfloat16* to = (which == 0 ? p.dv : p.dk) + at;
+        float* part = p.partial + (size_t)(2 * it.part + (which == 0)) * p.rows * p.Hkv * p.D + at;
+#pragma unroll 1
+        for (int c = 0; c < DP; c += 32) {
+          uint32_t o[32];
+          if (it.n > 0) {
+            tmem_ld_32x32(base + which * 128 + c, o);
+            tmem_ld_wait();
+            if (which == 1 && c + 32 == DP) {                  // all read: the next item's products may come
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(out_empty);
+            }
+          }
 #pragma unroll
-        for (int e = 0; e < 32; ++e) sum += fabsf(__uint_as_float(o[e]));
+          for (int e = 0; e < 32; ++e) {
+            if (!any) o[e] = 0u;
+            bad[which] += fabsf(__uint_as_float(o[e]));
+          }
+          if (row < p.rows) {
+            if (p.splits > 1) {
 #pragma unroll
-        for (int e = 0; e < 32; ++e) o[e] = any ? __float_as_uint(__uint_as_float(o[e]) * f) : 0u;
-        if (row < p.rows) {
-          if (p.splits > 1) {
+              for (int e = 0; e < 32; e += 4)
+                if (c + e < p.D)
+                  *reinterpret_cast<float4*>(part + c + e) = make_float4(__uint_as_float(o[e]) * f, __uint_as_float(o[e + 1]) * f,
+                                                                         __uint_as_float(o[e + 2]) * f, __uint_as_float(o[e + 3]) * f);
+            } else {
 #pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              if (c + e < p.D) *reinterpret_cast<uint4*>(part + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 32; e += 16)
-              if (c + e < p.D) pa_put16(to + c + e, o, e, 1.f, wide, p.D - c - e);
+              for (int e = 0; e < 32; e += 16)
+                if (c + e < p.D) pa_put16(to + c + e, o, e, f, wide, p.D - c - e);
+            }
           }
         }
       }
-      for (uint32_t m = __ballot_sync(0xffffffffu, any && !pa_finite(sum)); m; m &= m - 1) {
-        const int who = __ffs(m) - 1;
-        __syncwarp();
-        pb_redo_dkv(p, g == 0, it.row + lg * 32 + who, it.hk, it.h0, it.heads, it.part, __shfl_sync(0xffffffffu, hi, who));
+#pragma unroll
+      for (int which = 0; which < 2; ++which) {
+        for (uint32_t m = __ballot_sync(0xffffffffu, any && !pa_finite(bad[which])); m; m &= m - 1) {
+          const int who = __ffs(m) - 1;
+          __syncwarp();
+          pb_redo_dkv(p, which == 0, it.row + lg * 32 + who, it.hk, it.h0, it.heads, it.part, __shfl_sync(0xffffffffu, hi, who));
+        }
       }
     }
   }
