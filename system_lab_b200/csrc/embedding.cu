@@ -5,9 +5,8 @@
 // Both are bound by memory.  The gradient is made from sorted tokens: no atomics on values, every row of dW is written
 // once, and the order of the sum is that of the positions whatever the launch.
 //   sort   one block per slice of the vocabulary.  It reads all tokens (they are few and lie in L2), counts those below its
-//          slice - which is where its part of the sorted list begins - and sorts its own by counting: 16 warps own
-//          consecutive parts of the positions and a histogram each, so the order of equal tokens is kept.  Rows of the
-//          slice that no token names are set to zero here, unless the gradient is added to an old one.
+//          slice - which is where its part of the sorted list begins - and sorts its own by counting: 32 warps own
+//          consecutive parts of the positions and a histogram each, so the order of equal tokens is kept.
 //   sum    the sorted list is cut into chunks; a group of threads, one vector of the row each, adds up a chunk's rows and
 //          writes every run of equal tokens that lies in it; a run that reaches over a border leaves its pieces' sums, fp32
 //   join   such runs: their pieces in order
@@ -18,21 +17,27 @@
 
 namespace slab {
 
-constexpr int EM_WARPS = 16;                 // of a sorting block
-constexpr int EM_MAX_SLICE = 768;            // vocabulary rows per sorting block: 16 histograms of 3 KB
+constexpr int EM_WARPS = 32;                 // of a sorting block
+constexpr int EM_BATCH = 8;                  // tokens per lane read together
+constexpr int EM_MAX_SLICE = 1536;           // vocabulary rows per sorting block: 32 histograms of 6 KB
+constexpr int EM_SORT_SMEM = 220 * 1024;     // histograms, and the tokens where they fit beside them
 
+// Vectors of a row as they are in memory (Raw: a quarter of the registers that 32-bit numbers take) and as numbers
 template <typename T, int VEC>
 struct EmVec;
 template <>
 struct EmVec<__nv_bfloat16, 8> {
-  static __device__ __forceinline__ void load(const __nv_bfloat16* p, float (&f)[8]) { unpack8(*reinterpret_cast<const bf16x8*>(p), f); }
+  typedef uint4 Raw;
+  static __device__ __forceinline__ Raw raw(const __nv_bfloat16* p) { return *reinterpret_cast<const uint4*>(p); }
+  static __device__ __forceinline__ void get(const Raw& r, float (&f)[8]) { unpack8(*reinterpret_cast<const bf16x8*>(&r), f); }
   static __device__ __forceinline__ void store(__nv_bfloat16* p, const float (&f)[8]) { *reinterpret_cast<bf16x8*>(p) = pack8(f); }
 };
 template <>
 struct EmVec<float, 8> {
-  static __device__ __forceinline__ void load(const float* p, float (&f)[8]) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+  struct Raw { float4 a, b; };
+  static __device__ __forceinline__ Raw raw(const float* p) { return {reinterpret_cast<const float4*>(p)[0], reinterpret_cast<const float4*>(p)[1]}; }
+  static __device__ __forceinline__ void get(const Raw& r, float (&f)[8]) {
+    f[0] = r.a.x; f[1] = r.a.y; f[2] = r.a.z; f[3] = r.a.w; f[4] = r.b.x; f[5] = r.b.y; f[6] = r.b.z; f[7] = r.b.w;
   }
   static __device__ __forceinline__ void store(float* p, const float (&f)[8]) {
     reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
@@ -41,51 +46,68 @@ struct EmVec<float, 8> {
 };
 template <>
 struct EmVec<__nv_bfloat16, 1> {
-  static __device__ __forceinline__ void load(const __nv_bfloat16* p, float (&f)[1]) { f[0] = __bfloat162float(*p); }
+  typedef __nv_bfloat16 Raw;
+  static __device__ __forceinline__ Raw raw(const __nv_bfloat16* p) { return *p; }
+  static __device__ __forceinline__ void get(const Raw& r, float (&f)[1]) { f[0] = __bfloat162float(r); }
   static __device__ __forceinline__ void store(__nv_bfloat16* p, const float (&f)[1]) { *p = __float2bfloat16(f[0]); }
 };
 template <>
 struct EmVec<float, 1> {
-  static __device__ __forceinline__ void load(const float* p, float (&f)[1]) { f[0] = *p; }
+  typedef float Raw;
+  static __device__ __forceinline__ Raw raw(const float* p) { return *p; }
+  static __device__ __forceinline__ void get(const Raw& r, float (&f)[1]) { f[0] = r; }
   static __device__ __forceinline__ void store(float* p, const float (&f)[1]) { *p = f[0]; }
 };
+template <typename T, int VEC>
+__device__ __forceinline__ void em_load(const T* p, float (&f)[VEC]) { EmVec<T, VEC>::get(EmVec<T, VEC>::raw(p), f); }
 
 // ---------------------------------------------------------------- lookup
+constexpr int EM_ROWS = 4;                   // rows of a thread, whose loads are in flight together
+// block (vectors, row groups): neighbouring threads on neighbouring vectors of a row
 template <typename TW, typename TO, int VEC>
 __global__ void __launch_bounds__(256)
-embedding_fwd_kernel(const long long* __restrict__ tokens, const TW* __restrict__ w, TO* __restrict__ out, long n, int vecs, int h,
-                     int vocab, float scale, int* status) {
-  // `vecs` vectors a row, neighbouring threads on neighbouring ones
-  const long stride = (long)gridDim.x * blockDim.x;
-  for (long i = (long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += stride) {
-    const long row = i / vecs;
-    const int c = (int)(i - row * vecs) * VEC;
-    const long long id = tokens[row];
-    float f[VEC];
-    if (id >= 0 && id < vocab) {
-      EmVec<TW, VEC>::load(w + (size_t)id * h + c, f);
+embedding_fwd_kernel(const long long* __restrict__ tokens, const TW* __restrict__ w, TO* __restrict__ out, long rows, int h, int vocab,
+                     float scale, int* status) {
+  const int c = (blockIdx.y * blockDim.x + threadIdx.x) * VEC;
+  const long row0 = ((long)blockIdx.x * blockDim.y + threadIdx.y) * EM_ROWS;
+  if (c >= h || row0 >= rows) return;
+  long long id[EM_ROWS];
+  float f[EM_ROWS][VEC];
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) f[k] *= scale;
-    } else {
+  for (int i = 0; i < EM_ROWS; ++i) id[i] = row0 + i < rows ? tokens[row0 + i] : -1;
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) f[k] = 0.f;
-      if (c == 0) atomicCAS(status, 0, ST_BAD_INDEX);
-    }
-    EmVec<TO, VEC>::store(out + (size_t)row * h + c, f);
+  for (int i = 0; i < EM_ROWS; ++i) {
+    const bool in = id[i] >= 0 && id[i] < vocab;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) f[i][k] = 0.f;
+    if (in) em_load<TW, VEC>(w + (size_t)id[i] * h + c, f[i]);
+    else if (c == 0 && row0 + i < rows) atomicCAS(status, 0, ST_BAD_INDEX);
+  }
+#pragma unroll
+  for (int i = 0; i < EM_ROWS; ++i) {
+    if (row0 + i >= rows) break;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) f[i][k] *= scale;
+    EmVec<TO, VEC>::store(out + (size_t)(row0 + i) * h + c, f[i]);
   }
 }
 
 // ---------------------------------------------------------------- sort
-// order[0 .. valid): positions of the tokens in the table, by token and then by position; *valid their number
-template <typename TW>
+// place of a token id in the slice from v0 on: negative below it (and for negative ids), at least the slice's width above
+__device__ __forceinline__ int em_bin(long long id, int v0) {
+  return id < 0 ? -1 : id >= 0x7fffffffll ? 0x7fffffff : (int)id - v0;
+}
+// order[0 .. valid): positions of the tokens in the table, by token and then by position; *valid their number; bit v of named: some
+// token is v (slices are multiples of 32 rows)
 __global__ void __launch_bounds__(EM_WARPS * 32)
 embedding_sort_kernel(const long long* __restrict__ tokens, int n, int vocab, int slice, int* __restrict__ order, int* valid,
-                      TW* __restrict__ dw, int h, int fill) {
-  extern __shared__ int hist[];              // [warps][slice], then [slice] totals
+                      uint32_t* __restrict__ named, int keep) {
+  extern __shared__ int hist[];              // [warps][slice], [slice] totals, and with `keep` the tokens for the second pass
   __shared__ int below_s, warp_sums[EM_WARPS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int v0 = blockIdx.x * slice, width = min(slice, vocab - v0);
   int* total = hist + EM_WARPS * slice;
+  int* kept = total + slice;
   for (int i = threadIdx.x; i < EM_WARPS * slice; i += blockDim.x) hist[i] = 0;
   if (threadIdx.x == 0) below_s = 0;
   __syncthreads();
@@ -94,11 +116,17 @@ embedding_sort_kernel(const long long* __restrict__ tokens, int n, int vocab, in
   const int from = min(n, warp * per), to = min(n, from + per);
   int below = 0;
   int* mine = hist + warp * slice;
-#pragma unroll 4
-  for (int i = from + lane; i < to; i += 32) {
-    const long long id = tokens[i];
-    below += id >= 0 && id < v0;
-    if (id >= v0 && id < v0 + width) atomicAdd(&mine[(int)id - v0], 1);
+  for (int i0 = from; i0 < to; i0 += 32 * EM_BATCH) {
+    long long id[EM_BATCH];
+#pragma unroll
+    for (int a = 0; a < EM_BATCH; ++a) id[a] = i0 + 32 * a + lane < to ? tokens[i0 + 32 * a + lane] : -1;
+#pragma unroll
+    for (int a = 0; a < EM_BATCH; ++a) {
+      const int b = em_bin(id[a], v0);
+      below += b < 0 && id[a] >= 0;
+      if (keep && i0 + 32 * a + lane < to) kept[i0 + 32 * a + lane] = b;
+      if ((unsigned)b < (unsigned)width) atomicAdd(&mine[b], 1);
+    }
   }
   below = __reduce_add_sync(0xffffffffu, below);
   if (lane == 0) atomicAdd(&below_s, below);
@@ -115,6 +143,8 @@ embedding_sort_kernel(const long long* __restrict__ tokens, int n, int vocab, in
       }
     }
     total[b] = sum;
+    const uint32_t bits = __ballot_sync(__activemask(), sum > 0);      // (whole warps: slice is a multiple of 32)
+    if ((b & 31) == 0 && b < width) named[(v0 + b) >> 5] = bits;
   }
   __syncthreads();
   // first place of every bin: a thread has neighbouring bins
@@ -142,29 +172,24 @@ embedding_sort_kernel(const long long* __restrict__ tokens, int n, int vocab, in
   }
   __syncthreads();
   if (all > 0) {
-    for (int i0 = from; i0 < to; i0 += 32) {
-      const int i = i0 + lane;
-      const long long id = i < to ? tokens[i] : -1;
-      const bool in = id >= v0 && id < v0 + width;
-      const int b = in ? (int)id - v0 : -1;
-      if (!__any_sync(0xffffffffu, in)) continue;
-      const unsigned peers = __match_any_sync(0xffffffffu, b);
-      if (in) order[mine[b] + __popc(peers & ((1u << lane) - 1u))] = i;
-      __syncwarp();
-      if (in && (peers >> lane) == 1u) mine[b] += __popc(peers);       // the last of the equal ones
-      __syncwarp();
-    }
-  }
-  if (!fill) return;
-  // rows without tokens, a warp each (their bytes are a multiple of 16 where the table's rows are)
-  const long bytes = (long)h * sizeof(TW);
-  for (int b = warp; b < width; b += EM_WARPS) {
-    if (total[b]) continue;
-    char* row = reinterpret_cast<char*>(dw) + (size_t)(v0 + b) * bytes;
-    if (((reinterpret_cast<size_t>(dw) | bytes) & 15) == 0) {
-      for (long i = lane * 16; i < bytes; i += 512) __stcs(reinterpret_cast<uint4*>(row + i), make_uint4(0u, 0u, 0u, 0u));
-    } else {
-      for (int i = lane; i < h; i += 32) reinterpret_cast<TW*>(row)[i] = TW(0.f);
+    for (int i0 = from; i0 < to; i0 += 32 * EM_BATCH) {
+      int bin[EM_BATCH];
+#pragma unroll
+      for (int a = 0; a < EM_BATCH; ++a) {
+        const int i = i0 + 32 * a + lane;
+        bin[a] = i >= to ? -1 : keep ? kept[i] : em_bin(tokens[i], v0);
+      }
+#pragma unroll
+      for (int a = 0; a < EM_BATCH; ++a) {
+        const bool in = (unsigned)bin[a] < (unsigned)width;
+        if (!__any_sync(0xffffffffu, in)) continue;
+        const int b = in ? bin[a] : -1;
+        const unsigned peers = __match_any_sync(0xffffffffu, b);
+        if (in) order[mine[b] + __popc(peers & ((1u << lane) - 1u))] = i0 + 32 * a + lane;
+        __syncwarp();
+        if (in && (peers >> lane) == 1u) mine[b] += __popc(peers);     // the last of the equal ones
+        __syncwarp();
+      }
     }
   }
 }
@@ -175,69 +200,105 @@ struct EmSum {
   const int* order;
   const int* valid;
   float* pieces;             // [chunks][2][h]: the piece of a run that comes from the chunk before, and of one that goes on
+  int2* ends;                // [chunks]: {EM_WHOLE, EM_BEGINS, token of the chunk's last run}
   int h, chunk;              // columns, positions per chunk
   int accumulate;
   float scale;
+  const uint32_t* named;     // rows that some token names
+  int vocab, sum_blocks;
 };
 template <typename TW, int VEC>
 __device__ __forceinline__ void em_write(const EmSum& p, TW* dw, long long id, int c, const float (&sum)[VEC]) {
   TW* to = dw + (size_t)id * p.h + c;
   float f[VEC], old[VEC];
-  if (p.accumulate) EmVec<TW, VEC>::load(to, old);
+  if (p.accumulate) em_load<TW, VEC>(to, old);
 #pragma unroll
   for (int k = 0; k < VEC; ++k) f[k] = p.accumulate ? fmaf(sum[k], p.scale, old[k]) : sum[k] * p.scale;
   EmVec<TW, VEC>::store(to, f);
 }
 
+enum { EM_WHOLE = 1, EM_BEGINS = 2 };        // a chunk lies inside one run that goes on; a run begins in it that goes on
 constexpr int EM_AHEAD = 8;                  // rows in flight per thread
 
 // block (columns / VEC threads, chunks): a row of threads sums one chunk
+// Blocks from sum_blocks on set the rows that no token names to zero, a warp each: writing them is most of the time where the
+// table has many more rows than the batch has tokens, and the sums, which wait for scattered rows, run beside it (8192 tokens,
+// 151936 x 2048: 132 us one after the other).
+template <typename TW>
+__device__ __forceinline__ void em_fill(const uint32_t* named, TW* dw, int vocab, int h, int block, int blocks) {
+  const int threads = blockDim.x * blockDim.y, t = threadIdx.y * blockDim.x + threadIdx.x, lane = t & 31;
+  const long bytes = (long)h * sizeof(TW);
+  const bool vec = ((reinterpret_cast<size_t>(dw) | bytes) & 15) == 0;
+  for (long v = (long)block * (threads >> 5) + (t >> 5); v < vocab; v += (long)blocks * (threads >> 5)) {
+    if (named[v >> 5] >> (v & 31) & 1u) continue;
+    char* row = reinterpret_cast<char*>(dw) + (size_t)v * bytes;
+    if (vec) {
+      for (long i = lane * 16; i < bytes; i += 512) __stcs(reinterpret_cast<uint4*>(row + i), make_uint4(0u, 0u, 0u, 0u));
+    } else {
+      for (int i = lane; i < h; i += 32) reinterpret_cast<TW*>(row)[i] = TW(0.f);
+    }
+  }
+}
 template <typename TW, typename TO, int VEC>
 __global__ void __launch_bounds__(256)
 embedding_sum_kernel(const EmSum p, const TO* __restrict__ dout, TW* __restrict__ dw) {
+  if ((int)blockIdx.x >= p.sum_blocks) {
+    if (blockIdx.y == 0) em_fill(p.named, dw, p.vocab, p.h, blockIdx.x - p.sum_blocks, gridDim.x - p.sum_blocks);
+    return;
+  }
+  // the chunk's part of the list, from the position before it to the one behind it: {position, token}, token -1 beyond the list
+  extern __shared__ int2 list_s[];
   const int chunk = blockIdx.x * blockDim.y + threadIdx.y;
   const int c = (blockIdx.y * blockDim.x + threadIdx.x) * VEC;
   const int valid = *p.valid, from = chunk * p.chunk;
+  int2* list = list_s + threadIdx.y * (p.chunk + 2);
+  for (int i = threadIdx.x; i < p.chunk + 2; i += blockDim.x) {
+    const int at = from - 1 + i;
+    int2 e = make_int2(0, -1);
+    if (at >= 0 && at < valid) {
+      e.x = p.order[at];
+      e.y = (int)p.tokens[e.x];
+    }
+    list[i] = e;
+  }
+  __syncthreads();
   if (c >= p.h || from >= valid) return;
-  const int to = min(valid, from + p.chunk);
+  const int n = min(valid - from, p.chunk);
   float sum[VEC];
 #pragma unroll
   for (int k = 0; k < VEC; ++k) sum[k] = 0.f;
-  long long run = p.tokens[p.order[from]];
-  bool head = from > 0 && p.tokens[p.order[from - 1]] == run;          // this run began in a chunk before
-  for (int i = from; i < to; i += EM_AHEAD) {
-    int pos[EM_AHEAD];
-    long long id[EM_AHEAD];
-    float x[EM_AHEAD][VEC];
+  int run = list[1].y;
+  bool head = from > 0 && list[0].y == run;                            // this run began in a chunk before
+  bool one = true;
+  for (int i = 0; i < n; i += EM_AHEAD) {
+    typename EmVec<TO, VEC>::Raw raw[EM_AHEAD];
 #pragma unroll
-    for (int a = 0; a < EM_AHEAD; ++a) pos[a] = i + a < to ? p.order[i + a] : 0;
-#pragma unroll
-    for (int a = 0; a < EM_AHEAD; ++a) {
-      if (i + a < to) {
-        id[a] = p.tokens[pos[a]];
-        EmVec<TO, VEC>::load(dout + (size_t)pos[a] * p.h + c, x[a]);
-      }
-    }
+    for (int a = 0; a < EM_AHEAD; ++a)
+      if (i + a < n) raw[a] = EmVec<TO, VEC>::raw(dout + (size_t)list[1 + i + a].x * p.h + c);
 #pragma unroll
     for (int a = 0; a < EM_AHEAD; ++a) {
-      if (i + a < to) {
-        if (id[a] != run) {
+      if (i + a < n) {
+        const int id = list[1 + i + a].y;
+        if (id != run) {
           if (head) EmVec<float, VEC>::store(p.pieces + (size_t)(2 * chunk) * p.h + c, sum);
           else em_write<TW, VEC>(p, dw, run, c, sum);
-          head = false;
-          run = id[a];
+          head = one = false;
+          run = id;
 #pragma unroll
           for (int k = 0; k < VEC; ++k) sum[k] = 0.f;
         }
+        float x[VEC];
+        EmVec<TO, VEC>::get(raw[a], x);
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) sum[k] += x[a][k];
+        for (int k = 0; k < VEC; ++k) sum[k] += x[k];
       }
     }
   }
-  const bool on = to < valid && p.tokens[p.order[to]] == run;          // the last run goes on in the next chunk
+  const bool on = from + n < valid && list[1 + n].y == run;            // the last run goes on in the next chunk
   if (head) EmVec<float, VEC>::store(p.pieces + (size_t)(2 * chunk) * p.h + c, sum);
   else if (on) EmVec<float, VEC>::store(p.pieces + (size_t)(2 * chunk + 1) * p.h + c, sum);
   else em_write<TW, VEC>(p, dw, run, c, sum);
+  if (c == 0) p.ends[chunk] = make_int2(!on ? 0 : head && one ? EM_WHOLE : EM_BEGINS, run);
 }
 
 template <typename TW, int VEC>
@@ -245,27 +306,29 @@ __global__ void __launch_bounds__(256)
 embedding_join_kernel(const EmSum p, TW* __restrict__ dw) {
   const int chunk = blockIdx.x * blockDim.y + threadIdx.y;
   const int c = (blockIdx.y * blockDim.x + threadIdx.x) * VEC;
-  const int valid = *p.valid, from = chunk * p.chunk, next = from + p.chunk;
-  if (c >= p.h || next >= valid) return;
-  // runs that begin in this chunk and go on in the next
-  const long long run = p.tokens[p.order[next - 1]];
-  if (p.tokens[p.order[next]] != run || (from > 0 && p.tokens[p.order[from - 1]] == run)) return;
+  const int valid = *p.valid, chunks = (valid + p.chunk - 1) / p.chunk;
+  if (c >= p.h || chunk >= chunks) return;
+  const int2 e = p.ends[chunk];
+  if (!(e.x & EM_BEGINS)) return;
+  const long long run = e.y;
   float sum[VEC];
-  EmVec<float, VEC>::load(p.pieces + (size_t)(2 * chunk + 1) * p.h + c, sum);
-  int end = chunk + 1;                       // chunks chunk + 1 .. end - 1 have a piece: the run's last position, by bisection
-  {
-    int lo = next, hi = valid;               // order[lo] is of the run, order[hi] is not (or behind the list)
-    while (hi - lo > 1) {
-      const int mid = lo + (hi - lo) / 2;
-      if (p.tokens[p.order[mid]] == run) lo = mid; else hi = mid;
+  em_load<float, VEC>(p.pieces + (size_t)(2 * chunk + 1) * p.h + c, sum);
+  int end = chunk + 1;                       // chunks chunk + 1 .. end have a piece: up to the first the run ends in
+  for (bool found = false; !found;) {
+    int w[EM_AHEAD];
+#pragma unroll
+    for (int a = 0; a < EM_AHEAD; ++a) w[a] = end + a < chunks ? p.ends[end + a].x & EM_WHOLE : 0;
+#pragma unroll
+    for (int a = 0; a < EM_AHEAD; ++a) {
+      if (!found) ++end;
+      found = found || !w[a];
     }
-    end = lo / p.chunk + 1;
   }
   for (int k0 = chunk + 1; k0 < end; k0 += EM_AHEAD) {
     float x[EM_AHEAD][VEC];
 #pragma unroll
     for (int a = 0; a < EM_AHEAD; ++a)
-      if (k0 + a < end) EmVec<float, VEC>::load(p.pieces + (size_t)(2 * (k0 + a)) * p.h + c, x[a]);
+      if (k0 + a < end) em_load<float, VEC>(p.pieces + (size_t)(2 * (k0 + a)) * p.h + c, x[a]);
 #pragma unroll
     for (int a = 0; a < EM_AHEAD; ++a) {
       if (k0 + a < end) {
@@ -284,13 +347,22 @@ static int em_sms() {
   cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
   return n > 0 ? n : 1;
 }
+// Threads for rows of `vecs` vectors: up to 256 side by side, in slabs of about one length that end on whole warps (2880 columns
+// are two slabs of 192 threads, not one of 256 and one of 104), the rest of the block for other rows.
+static dim3 em_block(int vecs) {
+  const int slabs = (vecs + 255) / 256, each = (vecs + slabs - 1) / slabs;
+  int tx = 8;
+  if (each > 16) tx = (each + 31) / 32 * 32;
+  else while (tx < each) tx *= 2;
+  return dim3(tx, 256 / tx > 0 ? 256 / tx : 1);
+}
 template <typename TW, typename TO, int VEC>
 static int em_fwd(const void* tokens, const void* w, void* out, long rows, int vocab, int h, float scale, void* status, cudaStream_t st) {
-  const int vecs = h / VEC;
-  const long n = rows * vecs;
-  const long blocks = (n + 255) / 256;
-  embedding_fwd_kernel<TW, TO, VEC><<<(unsigned)(blocks < (1l << 30) ? blocks : (1l << 30)), 256, 0, st>>>(
-      (const long long*)tokens, (const TW*)w, (TO*)out, n, vecs, h, vocab, scale, (int*)status);
+  const dim3 block = em_block(h / VEC);
+  const long groups = (rows + EM_ROWS - 1) / EM_ROWS;
+  const dim3 grid((unsigned)((groups + block.y - 1) / block.y), (h / VEC + block.x - 1) / block.x);
+  embedding_fwd_kernel<TW, TO, VEC><<<grid, block, 0, st>>>((const long long*)tokens, (const TW*)w, (TO*)out, rows, h, vocab, scale,
+                                                            (int*)status);
   return (int)cudaGetLastError();
 }
 
@@ -299,13 +371,18 @@ static int em_bwd(const void* tokens, const void* dout, void* dw, int* order, fl
                   int accumulate, cudaStream_t st) {
   const int sms = em_sms();
   int* valid = order + rows;
-  int slice = (vocab + 2 * sms - 1) / (2 * sms);
-  slice = slice < 1 ? 1 : slice > EM_MAX_SLICE ? EM_MAX_SLICE : slice;
-  const int smem = (EM_WARPS + 1) * slice * 4;
-  SLAB_CUDA_CHECK(cudaFuncSetAttribute(embedding_sort_kernel<TW>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       (EM_WARPS + 1) * EM_MAX_SLICE * 4));
-  embedding_sort_kernel<TW><<<(vocab + slice - 1) / slice, EM_WARPS * 32, smem, st>>>(
-      (const long long*)tokens, rows, vocab, slice, order, valid, (TW*)dw, h, accumulate ? 0 : 1);
+  uint32_t* named = reinterpret_cast<uint32_t*>(valid + 1);
+  // a block per SM: every block reads all tokens, which from L2 is what bounds it (32749 tokens, 32000 rows, two blocks per SM and
+  // both passes from L2: 24 us)
+  int slice = (vocab + sms - 1) / sms;
+  slice = slice > EM_MAX_SLICE ? EM_MAX_SLICE : (slice + 31) / 32 * 32;
+  const int bins = (EM_WARPS + 1) * slice * 4;
+  const bool keep = rows <= (EM_SORT_SMEM - bins) / 4;
+  const int smem = bins + (keep ? rows * 4 : 0);
+  if (smem > 48 * 1024)
+    SLAB_CUDA_CHECK(cudaFuncSetAttribute(embedding_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  embedding_sort_kernel<<<(vocab + slice - 1) / slice, EM_WARPS * 32, smem, st>>>((const long long*)tokens, rows, vocab, slice, order,
+                                                                                  valid, named, keep ? 1 : 0);
   EmSum p;
   p.tokens = (const long long*)tokens;
   p.order = order;
@@ -315,13 +392,15 @@ static int em_bwd(const void* tokens, const void* dout, void* dw, int* order, fl
   p.chunk = chunk;
   p.accumulate = accumulate;
   p.scale = scale;
-  const int vecs = h / VEC;
-  int tx = 8;
-  while (tx < 256 && tx < vecs) tx *= 2;
-  const dim3 block(tx, 256 / tx);
+  const dim3 block = em_block(h / VEC);
   const int chunks = (rows + p.chunk - 1) / p.chunk;
-  const dim3 grid((chunks + block.y - 1) / block.y, (vecs + tx - 1) / tx);
-  embedding_sum_kernel<TW, TO, VEC><<<grid, block, 0, st>>>(p, (const TO*)dout, (TW*)dw);
+  const dim3 grid((chunks + block.y - 1) / block.y, (h / VEC + block.x - 1) / block.x);
+  p.named = named;
+  p.vocab = vocab;
+  p.sum_blocks = (int)grid.x;
+  const int fill_blocks = accumulate ? 0 : (vocab + 7) / 8 < 8 * sms ? (vocab + 7) / 8 : 8 * sms;
+  p.ends = reinterpret_cast<int2*>(pieces + (size_t)chunks * 2 * h);
+  embedding_sum_kernel<TW, TO, VEC><<<dim3(grid.x + fill_blocks, grid.y), block, block.y * (p.chunk + 2) * sizeof(int2), st>>>(p, (const TO*)dout, (TW*)dw);
   if (chunks > 1) embedding_join_kernel<TW, VEC><<<grid, block, 0, st>>>(p, (TW*)dw);
   return (int)cudaGetLastError();
 }
@@ -349,8 +428,8 @@ extern "C" int slab_embedding_fwd(const void* tokens, const void* w, int w_bf16,
   });
 }
 
-// dw [vocab, h] (all of it written, or added to), dout [rows, h]; order: scratch of rows + 1 int32, pieces: scratch of
-// ceil(rows / chunk) * 2 * h floats, chunk: positions of the sorted list that a group of threads adds up
+// dw [vocab, h] (all of it written, or added to), dout [rows, h]; order: scratch of rows + 1 + ceil(vocab / 32) int32, pieces: scratch of
+// ceil(rows / chunk) * (2 * h + 2) floats, chunk: positions of the sorted list that a group of threads adds up
 extern "C" int slab_embedding_bwd(const void* tokens, const void* dout, int out_bf16, void* dw, int w_bf16, void* order, void* pieces,
                                   int rows, int chunk, int vocab, int h, float scale, int accumulate, void* stream) {
   using namespace slab;

@@ -73,8 +73,8 @@ class _Embedding(torch.autograd.Function):
             g = g.contiguous()
             with cuda.on_device(g):
                 chunk = _chunk(rows)
-                at = (rows + 4) // 4 * 4                         # the sorted positions and their number, then the pieces
-                scratch = torch.empty(at + (rows + chunk - 1) // chunk * 2 * h, dtype=torch.int32, device=g.device)
+                at = (rows + 1 + (v + 31) // 32 + 3) // 4 * 4      # the sorted positions, their number, which rows; then the pieces
+                scratch = torch.empty(at + (rows + chunk - 1) // chunk * (2 * h + 2), dtype=torch.int32, device=g.device)
                 base = scratch.data_ptr()
                 cuda.call("slab_embedding_bwd", tok, g, int(g.dtype == torch.bfloat16), dw, int(dw.dtype == torch.bfloat16),
                           base, base + 4 * at, rows, chunk, v, h, ctx.scale, int(accumulate), cuda.stream())
