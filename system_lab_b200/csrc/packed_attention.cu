@@ -183,18 +183,19 @@ struct PackedFwdItem {
   __device__ __forceinline__ explicit PackedFwdItem(const PaItem& i)
       : row{i.v[0], i.v[1]}, head{i.v[2], i.v[3]}, hk(i.v[4]), j0(i.v[5]), n(i.v[7]) {}
 };
-__device__ __forceinline__ PaItem pf_item(const PackedFwdParams& p, const PackedPlan& plan, int idx) {
+// (sorted: the plan's order; not where every item has a block of its own, which spares it a dependent load)
+__device__ __forceinline__ PaItem pf_item(const PackedFwdParams& p, const PackedPlan& plan, int idx, bool sorted) {
   const int tiles = (p.rows + PA_TILE - 1) / PA_TILE;
   int lo, last, row0, row1, head0, head1;
   if (p.head_pairs) {
-    const int hp = p.Hq >> 1, o = idx / hp, t = plan.q_order[o];
+    const int hp = p.Hq >> 1, o = idx / hp, t = sorted ? plan.q_order[o] : o;
     head0 = 2 * (idx - o * hp);
     head1 = head0 + 1;
     row0 = row1 = t * PA_TILE;
     lo = plan.tile_lo[t];
     last = t;
   } else {
-    const int o = idx / p.Hq, t = 2 * plan.pair_order[o];
+    const int o = idx / p.Hq, t = 2 * (sorted ? plan.pair_order[o] : o);
     head0 = head1 = idx - o * p.Hq;
     row0 = t * PA_TILE;
     row1 = row0 + PA_TILE;
@@ -459,7 +460,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       }
       if (ok && v_row >= 0) load_stage(-1, 0);
     } else if (warp == 11) {
-      pa_schedule(queue, items, p.counter, [&](int idx) { return pf_item(p, plan, idx); }, abort_flag, p.status);
+      pa_schedule(queue, items, p.counter, [&](int idx) { return pf_item(p, plan, idx, items > (int)gridDim.x); }, abort_flag, p.status);
     } else if (warp == 8) {
       // ------------------------------------------------------------ MMAs
       constexpr uint32_t idesc_qk = make_idesc(1, 1, 0, 0, PA_TILE, PA_TILE);

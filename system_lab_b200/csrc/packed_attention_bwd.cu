@@ -239,8 +239,9 @@ struct PackedDqItem {
   int row, head, hk, j0, n;
   __device__ __forceinline__ explicit PackedDqItem(const PaItem& i) : row(i.v[0]), head(i.v[1]), hk(i.v[2]), j0(i.v[3]), n(i.v[7]) {}
 };
-__device__ __forceinline__ PaItem pb_dq_item(const PackedBwdParams& p, const PackedPlan& plan, int idx) {
-  const int o = idx / p.Hq, t = plan.q_order[o], lo = plan.tile_lo[t];
+// (sorted: the plan's order; not where every item has a block of its own)
+__device__ __forceinline__ PaItem pb_dq_item(const PackedBwdParams& p, const PackedPlan& plan, int idx, bool sorted) {
+  const int o = idx / p.Hq, t = sorted ? plan.q_order[o] : o, lo = plan.tile_lo[t];
   const int head = idx - o * p.Hq, row = t * PA_TILE;
   const int first = p.window > 0 ? max(lo, row - p.window + 1) : lo;
   const int j0 = lo == PA_NONE ? 0 : first / PA_TILE;
@@ -388,7 +389,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         ++done;
       }
     } else if (warp == 11) {
-      pa_schedule(queue, items, p.counter + 1, [&](int idx) { return pb_dq_item(p, plan, idx); }, abort_flag, p.status);
+      pa_schedule(queue, items, p.counter + 1, [&](int idx) { return pb_dq_item(p, plan, idx, items > (int)gridDim.x); }, abort_flag, p.status);
     } else if (warp == 8) {
       constexpr uint32_t idesc_s = make_idesc(1, 1, 0, 0, PA_TILE, PA_TILE);
       constexpr uint32_t idesc_d = make_idesc(1, 1, 0, 1, PA_TILE, DP);
@@ -613,9 +614,9 @@ struct PackedDkvItem {
   __device__ __forceinline__ explicit PackedDkvItem(const PaItem& i)
       : tile(i.v[0]), row(i.v[0] * PA_TILE), hk(i.v[1]), part(i.v[2]), h0(i.v[3]), heads(i.v[4]), tiles(i.v[5]), n(i.v[7]) {}
 };
-__device__ __forceinline__ PaItem pb_dkv_item(const PackedBwdParams& p, const PackedPlan& plan, int idx) {
+__device__ __forceinline__ PaItem pb_dkv_item(const PackedBwdParams& p, const PackedPlan& plan, int idx, bool sorted) {
   const int per = p.Hkv * p.splits, o = idx / per, rest = idx - o * per, G = p.Hq / p.Hkv;
-  const int tile = plan.k_order[o], hk = rest / p.splits, part = rest - hk * p.splits;
+  const int tile = sorted ? plan.k_order[o] : o, hk = rest / p.splits, part = rest - hk * p.splits;
   const int a = part * G / p.splits, b = (part + 1) * G / p.splits;
   int hi = plan.tile_hi[tile];
   if (p.window > 0) hi = min(hi, tile * PA_TILE + PA_TILE - 1 + p.window);
@@ -716,7 +717,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         ++done;
       }
     } else if (warp == 11) {
-      pa_schedule(queue, items, p.counter, [&](int idx) { return pb_dkv_item(p, plan, idx); }, abort_flag, p.status);
+      pa_schedule(queue, items, p.counter, [&](int idx) { return pb_dkv_item(p, plan, idx, items > (int)gridDim.x); }, abort_flag, p.status);
     } else if (warp == 8) {
       constexpr uint32_t idesc_s = make_idesc(1, 1, 0, 0, PA_TILE, PA_TILE);
       constexpr uint32_t idesc_d = make_idesc(1, 1, 0, 1, PA_TILE, DP);

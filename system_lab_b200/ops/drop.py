@@ -40,36 +40,38 @@ def check(x, p, seed, offset, residual):
                          f"{tuple(x.shape)} {x.dtype} on {x.device}")
 
 
-def _run(x, res, p, seed, offset):
+def _run(x, res, args):
+    """``args``: threshold, seed (signed), seed on the device or None, offset (signed)."""
     x = cuda._aligned16(x.contiguous())
-    res = cuda._aligned16(res.contiguous()) if res is not None else None
+    if res is not None:
+        res = cuda._aligned16(res.contiguous())
     y = torch.empty_like(x)
-    if x.numel():
-        dev = seed if isinstance(seed, torch.Tensor) else None
+    n = x.numel()
+    if n:
         with cuda.on_device(x):
-            cuda.call("slab_dropout", x, res, y, int(x.dtype == torch.bfloat16), x.numel(), ref.dropout_threshold(p),
-                      0 if dev is not None else _signed(seed), dev, _signed(offset), cuda.stream())
+            cuda.call("slab_dropout", x, res, y, int(x.dtype == torch.bfloat16), n, *args, cuda.stream())
     return y
 
 
 class _Dropout(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, residual, p, seed, offset):
-        if isinstance(seed, torch.Tensor):
-            seed = seed.detach().clone()
-        ctx.args = (p, seed, offset)
-        return _run(x, residual, p, seed, offset)
+    def forward(ctx, x, residual, args):
+        ctx.args = args
+        return _run(x, residual, args)
 
     @staticmethod
     def backward(ctx, g):
-        p, seed, offset = ctx.args
         dx = None
         if ctx.needs_input_grad[0]:                # the mask's product again, itself differentiable where that is asked for
-            dx = _Dropout.apply(g, None, p, seed, offset) if torch.is_grad_enabled() else _run(g, None, p, seed, offset)
-        return dx, (g if ctx.needs_input_grad[1] else None), None, None, None
+            dx = _Dropout.apply(g, None, ctx.args) if torch.is_grad_enabled() else _run(g, None, ctx.args)
+        return dx, (g if ctx.needs_input_grad[1] else None), None
 
 
 def dropout(x, p, seed, offset=0, residual=None):
     if x.dtype not in _TYPES:
         return ref.dropout(x, p, seed, offset, residual)
-    return _Dropout.apply(x, residual, p, seed, offset)
+    if isinstance(seed, torch.Tensor):
+        args = (ref.dropout_threshold(p), 0, seed.detach().clone(), _signed(offset))
+    else:
+        args = (ref.dropout_threshold(p), _signed(seed), None, _signed(offset))
+    return _Dropout.apply(x, residual, args)

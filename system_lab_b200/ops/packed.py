@@ -36,11 +36,7 @@ class PackedDocuments:
     ``doc_hi`` are its first two parts.  A row of no document has an empty range, ``doc_lo = row + 1``, ``doc_hi = row``."""
 
     def __init__(self, rows: int, plan: torch.Tensor):
-        self.rows, self.plan = rows, plan
-
-    @property
-    def device(self):
-        return self.plan.device
+        self.rows, self.plan, self.device = rows, plan, plan.device
 
     @property
     def doc_lo(self) -> torch.Tensor:
@@ -109,22 +105,23 @@ def documents_from_tokens(tokens: torch.Tensor, end_token: int) -> PackedDocumen
 
 def check(q, k, v, documents, scale, window) -> float:
     """Refuses what neither path computes; returns the softmax scale."""
-    if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape:
-        raise ValueError(f"q [rows, heads, d], k and v [rows, groups, d] wanted, got {tuple(q.shape)}, {tuple(k.shape)}, "
-                         f"{tuple(v.shape)}")
-    rows, hq, d = q.shape
-    if k.shape[0] != rows or k.shape[2] != d or k.shape[1] == 0 or hq % k.shape[1] or hq == 0 or d == 0:
-        raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} do not go together")
+    qs, ks = q.shape, k.shape
+    if len(qs) != 3 or len(ks) != 3 or v.shape != ks:
+        raise ValueError(f"q [rows, heads, d], k and v [rows, groups, d] wanted, got {tuple(qs)}, {tuple(ks)}, {tuple(v.shape)}")
+    rows, hq, d = qs
+    if ks[0] != rows or ks[2] != d or ks[1] == 0 or hq % ks[1] or hq == 0 or d == 0:
+        raise ValueError(f"q {tuple(qs)} and k {tuple(ks)} do not go together")
     if documents.rows != rows:
         raise ValueError(f"the documents' plan is for {documents.rows} rows, not {rows}")
-    if not (q.dtype == k.dtype == v.dtype):
+    if k.dtype != q.dtype or v.dtype != q.dtype:
         raise ValueError(f"q, k and v differ in type: {q.dtype}, {k.dtype}, {v.dtype}")
-    if not (q.device == k.device == v.device == documents.device):
+    dev = documents.device
+    if q.device != dev or k.device != dev or v.device != dev:
         raise ValueError("q, k, v and the documents' plan lie on different devices")
     if window < 0:
         raise ValueError(f"window {window}")
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
-    if not (0.0 < scale < math.inf):
+    if not 0.0 < scale < math.inf:
         raise ValueError(f"softmax scale {scale}: has to be positive and finite")
     return scale
 
@@ -134,16 +131,17 @@ def supports(q, k, v) -> bool:
 
 
 def _readable(t):
-    """``t`` where the copy engine can read it as it lies: unit stride inside a head, other strides and the address on 16
-    bytes (any stride counts as such on a dimension of one)."""
+    """``(t, token stride, head stride)``, ``t`` copied where the copy engine cannot read it as it lies: unit stride inside a
+    head, other strides and the address on 16 bytes (any stride counts as such on a dimension of one)."""
+    n, h, d = t.shape
     ts, hs, es = t.stride()
-    ok = (es == 1 or t.shape[2] == 1) and t.data_ptr() % 16 == 0
-    ok = ok and (t.shape[0] == 1 or (ts % 8 == 0 and ts > 0)) and (t.shape[1] == 1 or (hs % 8 == 0 and hs > 0))
-    return t if ok else t.contiguous().clone() if t.is_contiguous() else t.contiguous()
-
-
-def _strides(t):
-    return (t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]), (t.stride(1) if t.shape[1] > 1 else t.shape[2])
+    if n == 1:
+        ts = h * d
+    if h == 1:
+        hs = d
+    if (es == 1 or d == 1) and ts % 8 == 0 and ts > 0 and hs % 8 == 0 and hs > 0 and t.data_ptr() % 16 == 0:
+        return t, ts, hs
+    return t.clone(memory_format=torch.contiguous_format), h * d, d
 
 
 def forward(q, k, v, documents: PackedDocuments, scale: float, window: int = 0):
@@ -153,10 +151,12 @@ def forward(q, k, v, documents: PackedDocuments, scale: float, window: int = 0):
     out = torch.empty((rows, hq, d), dtype=q.dtype, device=q.device)
     stats = hq * ((rows + TILE - 1) // TILE * TILE)
     lse = torch.empty(stats + 1, dtype=torch.float32, device=q.device)
-    window = min(int(window), rows)
+    q, qt, qh = _readable(q)
+    k, kt, kh = _readable(k)
+    v, vt, vh = _readable(v)
     with cuda.on_device(q):
-        cuda.call("slab_packed_attn_fwd", q, k, v, out, lse, documents.plan, rows, hq, k.shape[1], d, *_strides(q),
-                  *_strides(k), *_strides(v), window, scale, lse.data_ptr() + 4 * stats, cuda.status_word(q.device), cuda.stream())
+        cuda.call("slab_packed_attn_fwd", q, k, v, out, lse, documents.plan, rows, hq, k.shape[1], d, qt, qh, kt, kh, vt, vh,
+                  min(window, rows), scale, lse.data_ptr() + 4 * stats, cuda.status_word(q.device), cuda.stream())
     return out, lse
 
 
@@ -165,19 +165,21 @@ def backward(q, k, v, out, lse, dout, documents: PackedDocuments, scale: float, 
     (few key tiles for the SMs), the parts' sums are kept in fp32 and added up in their order."""
     rows, hq, d = q.shape
     hkv = k.shape[1]
-    dout = _readable(dout)
     dq = torch.empty((rows, hq, d), dtype=q.dtype, device=q.device)
     dk = torch.empty((rows, hkv, d), dtype=q.dtype, device=q.device)
     dv = torch.empty_like(dk)
     stats = lse.numel() - 1
     delta = torch.empty(stats + 2, dtype=torch.float32, device=q.device)          # and two work counters
-    window = min(int(window), rows)
+    q, qt, qh = _readable(q)
+    k, kt, kh = _readable(k)
+    v, vt, vh = _readable(v)
+    dout, gt, gh = _readable(dout)
     with cuda.on_device(q):
         splits = cuda.lib().slab_packed_attn_splits(rows, hq, hkv)
         partial = torch.empty(splits * 2 * dk.numel(), dtype=torch.float32, device=q.device) if splits > 1 else None
         cuda.call("slab_packed_attn_bwd", q, k, v, out, dout, lse, documents.plan, dq, dk, dv, delta,
-                  delta.data_ptr() + 4 * stats, partial, splits, rows, hq, hkv, d, *_strides(q), *_strides(k), *_strides(v),
-                  *_strides(dout), window, scale, cuda.status_word(q.device), cuda.stream())
+                  delta.data_ptr() + 4 * stats, partial, splits, rows, hq, hkv, d, qt, qh, kt, kh, vt, vh, gt, gh,
+                  min(window, rows), scale, cuda.status_word(q.device), cuda.stream())
         if splits > 1:
             cuda.LAUNCHES[0] += 1
     return dq, dk, dv
@@ -186,7 +188,7 @@ def backward(q, k, v, out, lse, dout, documents: PackedDocuments, scale: float, 
 class _PackedAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, documents, scale, window):
-        q, k, v = _readable(q), _readable(k), _readable(v)
+        q, k, v = (_readable(t)[0] for t in (q, k, v))         # copied once, if at all, for both passes
         out, lse = forward(q, k, v, documents, scale, window)
         ctx.save_for_backward(q, k, v, out, lse)
         ctx.documents, ctx.scale, ctx.window = documents, scale, window
@@ -201,5 +203,5 @@ class _PackedAttention(torch.autograd.Function):
 
 def attention(q, k, v, documents: PackedDocuments, scale: float, window: int = 0):
     if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)):
-        return forward(_readable(q), _readable(k), _readable(v), documents, scale, window)[0]
+        return forward(q, k, v, documents, scale, window)[0]
     return _PackedAttention.apply(q, k, v, documents, scale, window)
