@@ -309,8 +309,6 @@ __device__ __forceinline__ void pf_whole(uint32_t s_addr, uint32_t o_addr, float
 template <int DP>
 __device__ __forceinline__ void pf_part(uint32_t s_addr, uint32_t o_addr, float scale_log2, uint32_t vis, int first, int lastk,
                                         float& m, float2& la, float2& lb, uint64_t* p_full) {
-  const uint32_t span = first > lastk ? 0u : (uint32_t)(lastk - first);
-  if (first > lastk) first = 1 << 20;
   float top = -INFINITY;
 #pragma unroll 1
   for (int c = 0; c < 4; ++c) {
@@ -318,11 +316,11 @@ __device__ __forceinline__ void pf_part(uint32_t s_addr, uint32_t o_addr, float 
     float s[32];
     tmem_ld_32x32(s_addr + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
     tmem_ld_wait();
+    const uint32_t seen = pa_bits(first, lastk, 32 * c);
     float mx[2] = {top, -INFINITY};
 #pragma unroll
     for (int k = 0; k < 32; k += 2)
-      mx[(k >> 1) & 1] = pa_max3(mx[(k >> 1) & 1], (uint32_t)(32 * c + k - first) <= span ? s[k] : -INFINITY,
-                                 (uint32_t)(32 * c + k + 1 - first) <= span ? s[k + 1] : -INFINITY);
+      mx[(k >> 1) & 1] = pa_max3(mx[(k >> 1) & 1], seen >> k & 1u ? s[k] : -INFINITY, seen >> (k + 1) & 1u ? s[k + 1] : -INFINITY);
     top = fmaxf(mx[0], mx[1]);
   }
   pf_raise<DP>(o_addr, top * scale_log2, m, la, lb);
@@ -335,11 +333,12 @@ __device__ __forceinline__ void pf_part(uint32_t s_addr, uint32_t o_addr, float 
       float s[32];
       tmem_ld_32x32(s_addr + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
       tmem_ld_wait();
+      const uint32_t seen = pa_bits(first, lastk, 32 * c);
 #pragma unroll
       for (int k = 0; k < 16; ++k) {
         float2 x = pa_fma2(make_float2(s[2 * k], s[2 * k + 1]), c2, b2);
-        x.x = (uint32_t)(32 * c + 2 * k - first) <= span ? pa_exp2(x.x) : 0.f;
-        x.y = (uint32_t)(32 * c + 2 * k + 1 - first) <= span ? pa_exp2(x.y) : 0.f;
+        x.x = seen >> (2 * k) & 1u ? pa_exp2(x.x) : 0.f;
+        x.y = seen >> (2 * k + 1) & 1u ? pa_exp2(x.y) : 0.f;
         la = pa_add2(la, x);
         packed[k] = pa_pack(x.x, x.y);
       }

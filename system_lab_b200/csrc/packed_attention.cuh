@@ -156,6 +156,12 @@ __device__ __forceinline__ void pa_schedule(const PaQueue& q, int items, int* co
   }
 }
 
+// Bits of the columns from .. to (any values; none where from > to) among c0 .. c0 + 31
+__device__ __forceinline__ uint32_t pa_bits(int from, int to, int c0) {
+  from = max(from - c0, 0);
+  to = min(to - c0, 31);
+  return from > to ? 0u : (0xffffffffu << from) & (0xffffffffu >> (31 - to));
+}
 __device__ __forceinline__ uint32_t pa_pack(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);

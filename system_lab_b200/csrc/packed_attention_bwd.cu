@@ -94,7 +94,6 @@ struct PbCols {
   const float4* p;
   __device__ __forceinline__ float4 at(int c) const { return p[c >> 2]; }
 };
-__device__ __forceinline__ bool pb_seen(int c, int first, uint32_t span) { return (uint32_t)(c - first) <= span; }
 __device__ __forceinline__ void pb_load(uint32_t taddr, float* s) {
   tmem_ld_32x32(taddr, *reinterpret_cast<uint32_t(*)[32]>(s));
 }
@@ -107,7 +106,7 @@ __device__ __forceinline__ void pb_store(uint32_t to, const float* s) {
 }
 // 32 scores to probabilities; one pair in PB_EVERY is made on the multiply-add units where nothing is masked
 template <bool PART, typename Stat>
-__device__ __forceinline__ void pb_probs(float* s, int c0, const Stat& lse, float2 c2, int first, uint32_t span) {
+__device__ __forceinline__ void pb_probs(float* s, int c0, const Stat& lse, float2 c2, uint32_t seen) {
 #pragma unroll
   for (int c = 0; c < 32; c += 4) {
     const float4 b = lse.at(c0 + c);
@@ -120,14 +119,14 @@ __device__ __forceinline__ void pb_probs(float* s, int c0, const Stat& lse, floa
         x.x = pa_exp2(x.x);
         x.y = pa_exp2(x.y);
       }
-      s[c + e] = !PART || pb_seen(c0 + c + e, first, span) ? x.x : 0.f;
-      s[c + e + 1] = !PART || pb_seen(c0 + c + e + 1, first, span) ? x.y : 0.f;
+      s[c + e] = !PART || (seen >> (c + e) & 1u) ? x.x : 0.f;
+      s[c + e + 1] = !PART || (seen >> (c + e + 1) & 1u) ? x.y : 0.f;
     }
   }
 }
 // 32 probabilities times (dP - delta).  (Zero times what a hidden row holds may be no number: masked again.)
 template <bool PART, typename Stat>
-__device__ __forceinline__ void pb_dscores(float* s, const float* t, int c0, const Stat& delta, int first, uint32_t span) {
+__device__ __forceinline__ void pb_dscores(float* s, const float* t, int c0, const Stat& delta, uint32_t seen) {
 #pragma unroll
   for (int c = 0; c < 32; c += 4) {
     const float4 b = delta.at(c0 + c);
@@ -135,27 +134,27 @@ __device__ __forceinline__ void pb_dscores(float* s, const float* t, int c0, con
     for (int e = 0; e < 4; e += 2) {
       const float2 x = pa_mul2(make_float2(s[c + e], s[c + e + 1]),
                                pa_add2(make_float2(t[c + e], t[c + e + 1]), e ? make_float2(-b.z, -b.w) : make_float2(-b.x, -b.y)));
-      s[c + e] = !PART || pb_seen(c0 + c + e, first, span) ? x.x : 0.f;
-      s[c + e + 1] = !PART || pb_seen(c0 + c + e + 1, first, span) ? x.y : 0.f;
+      s[c + e] = !PART || (seen >> (c + e) & 1u) ? x.x : 0.f;
+      s[c + e + 1] = !PART || (seen >> (c + e + 1) & 1u) ? x.y : 0.f;
     }
   }
 }
 // What of a thread's 64 columns its row and its warp see.  The warp sees all (whole), or 32-column chunks in vis.
 struct PbView {
-  int first;
-  uint32_t span, vis;
+  uint32_t seen[2], vis;                                     // what the row sees of the chunks; seen only where not whole
   bool whole;
   __device__ __forceinline__ PbView(int from, int to) {      // columns from .. to of 0 .. 63
     from = max(from, 0);
     to = min(to, 63);
     const bool none = from > to;
-    first = none ? 1 << 20 : from;
-    span = none ? 0u : (uint32_t)(to - from);
+    seen[0] = seen[1] = 0u;
     whole = !__any_sync(0xffffffffu, from > 0 || to < 63);
     vis = 3u;
     if (!whole) {
       const int lo = __reduce_min_sync(0xffffffffu, none ? 64 : from), hi = __reduce_max_sync(0xffffffffu, none ? -1 : to);
       vis = (lo < 32 && hi >= 0 ? 1u : 0u) | (hi >= 32 ? 2u : 0u);
+      seen[0] = pa_bits(from, to, 0);
+      seen[1] = pa_bits(from, to, 32);
     }
   }
 };
@@ -168,7 +167,7 @@ __device__ __forceinline__ void pb_step_p(uint32_t from, float (&s)[64], const P
     tmem_ld_wait();
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      pb_probs<false>(&s[32 * h], 32 * h, lse, c2, 0, 0u);
+      pb_probs<false>(&s[32 * h], 32 * h, lse, c2, 0u);
       if (STORE) pb_store(from + 16 * h, &s[32 * h]);
     }
     return;
@@ -178,7 +177,7 @@ __device__ __forceinline__ void pb_step_p(uint32_t from, float (&s)[64], const P
     if (v.vis >> h & 1u) {
       pb_load(from + 32 * h, &s[32 * h]);
       tmem_ld_wait();
-      pb_probs<true>(&s[32 * h], 32 * h, lse, c2, v.first, v.span);
+      pb_probs<true>(&s[32 * h], 32 * h, lse, c2, v.seen[h]);
     } else {
 #pragma unroll
       for (int c = 0; c < 32; ++c) s[32 * h + c] = 0.f;
@@ -196,7 +195,7 @@ __device__ __forceinline__ void pb_step_ds(uint32_t from, uint32_t to, float (&s
     tmem_ld_wait();
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      pb_dscores<false>(&s[32 * h], &t[32 * h], 32 * h, delta, 0, 0u);
+      pb_dscores<false>(&s[32 * h], &t[32 * h], 32 * h, delta, 0u);
       pb_store(to + 16 * h, &s[32 * h]);
     }
     return;
@@ -206,7 +205,7 @@ __device__ __forceinline__ void pb_step_ds(uint32_t from, uint32_t to, float (&s
     if (v.vis >> h & 1u) {
       pb_load(from + 32 * h, &t[32 * h]);
       tmem_ld_wait();
-      pb_dscores<true>(&s[32 * h], &t[32 * h], 32 * h, delta, v.first, v.span);
+      pb_dscores<true>(&s[32 * h], &t[32 * h], 32 * h, delta, v.seen[h]);
     }
     pb_store(to + 16 * h, &s[32 * h]);
   }
