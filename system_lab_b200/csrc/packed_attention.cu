@@ -156,6 +156,7 @@ constexpr float PF_SLACK = 8.f;              // a row's maximum may be this far 
 
 struct PackedFwdParams {
   __nv_bfloat16* out;      // [rows, Hq, D]
+  int8_t* rest;            // [rows, Hq, D] the output's lower half, or null
   float* lse;              // [Hq, tiles * 128], base-2 log-sum-exp of the scaled scores; +inf where a row sees nothing
   const int* plan;
   PackedRows q, k, v;
@@ -229,7 +230,17 @@ __device__ __noinline__ void pf_redo(const PackedFwdParams& p, int row, int head
     if (pa_nan(l)) break;
   }
   const float bad = __int_as_float(0x7fffffff), inv = pa_nan(l) || l == 0.f ? bad : 1.f / l;
-  pa_put4(p.out + ((size_t)row * p.Hq + head) * p.D, p.D, o, inv);
+  const size_t at = ((size_t)row * p.Hq + head) * p.D;
+  const int c = (threadIdx.x & 31) * 4;
+  o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+  if (p.rest && c < p.D) {
+    const bool fin = pa_finite(o.x) && pa_finite(o.y) && pa_finite(o.z) && pa_finite(o.w);
+    *reinterpret_cast<uint32_t*>(p.rest + at + c) = fin ? pa_rest(o.x, o.y, o.z, o.w) : 0u;
+    if (fin) *reinterpret_cast<uint2*>(p.out + at + c) = make_uint2(pa_pack_half(o.x, o.y), pa_pack_half(o.z, o.w));
+    else pa_put4(p.out + at, p.D, o, 1.f);
+  } else {
+    pa_put4(p.out + at, p.D, o, 1.f);
+  }
   if ((threadIdx.x & 31) == 0) p.lse[(size_t)head * padded + row] = pa_nan(inv) ? bad : m + log2f(l);
 }
 
@@ -620,7 +631,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     // the next one (the time between an item's last probabilities and its stored rows is some 5 thousand cycles)
     const int lg = warp & 3, r128 = lg * 32 + lane;
     const int tiles = (p.rows + PA_TILE - 1) / PA_TILE;
-    const bool wide = p.D % 16 == 0 && (reinterpret_cast<size_t>(p.out) & 31) == 0;
+    const bool wide = p.D % 16 == 0 && ((reinterpret_cast<size_t>(p.out) | 2 * reinterpret_cast<size_t>(p.rest)) & 31) == 0;
     int done = 0;
     bool ok = true;
     PaReader reader;
@@ -649,30 +660,27 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         }
         const uint32_t o_addr = tmem + 256 + g * 128 + (uint32_t(lg * 32) << 16);
         __nv_bfloat16* o_row = p.out + ((size_t)row * p.Hq + head) * p.D;
+        int8_t* rest = p.rest ? p.rest + ((size_t)row * p.Hq + head) * p.D : nullptr;
         const float f = sees ? 1.f / l : 0.f;
         float sum = l;                         // finite if all of the row is (or as good as: else it is made again for nothing)
 #pragma unroll 1
-        for (int c = 0; c < DP; c += 32) {
-          uint32_t o[32];
+        for (int c = 0; c < DP; c += 16) {
+          uint32_t o[16];
           if (it.n > 0) {
-            tmem_ld_32x32(o_addr + c, o);
+            pa_tmem_ld_16(o_addr + c, o);
             tmem_ld_wait();
-            if (c + 32 == DP) {                // all read: the next item's products may come
+            if (c + 16 == DP) {                // all read: the next item's products may come
               tc_fence_before();
               __syncwarp();
               if (lane == 0) mbar_arrive(&o_empty[g]);
             }
           }
 #pragma unroll
-          for (int k = 0; k < 32; ++k) {
+          for (int k = 0; k < 16; ++k) {
             if (!sees) o[k] = 0u;
             sum += fabsf(__uint_as_float(o[k]));
           }
-          if (row < p.rows) {
-#pragma unroll
-            for (int k = 0; k < 32; k += 16)
-              if (c + k < p.D) pa_put16(o_row + c + k, o, k, f, wide, p.D - c - k);
-          }
+          if (row < p.rows && c < p.D) pa_put16(o_row + c, o, 0, f, wide, p.D - c, rest ? rest + c : nullptr);
         }
         if (row < tiles * PA_TILE) p.lse[(size_t)head * tiles * PA_TILE + row] = sees ? m + log2f(l) : INFINITY;
         for (uint32_t again = __ballot_sync(0xffffffffu, sees && !(pa_finite(sum) && l > 0.f)); again; again &= again - 1) {
@@ -746,8 +754,9 @@ extern "C" int slab_packed_plan_tokens(const void* tokens, int rows, int seq, lo
 }
 
 // q [rows, Hq, D], k and v [rows, Hkv, D] bf16 with the given token and head strides (elements, multiples of 8; bases on 16
-// bytes), out [rows, Hq, D] contiguous, lse [Hq, tiles * 128] fp32, counter: scratch, one int32.  D a multiple of 8 up to 128.
-extern "C" int slab_packed_attn_fwd(const void* q, const void* k, const void* v, void* out, void* lse, const void* plan,
+// bytes), out [rows, Hq, D] contiguous, rest the same in int8 or null (lower half of the output, on 8 bytes), lse [Hq, tiles * 128] fp32, counter: scratch, one int32.  D a multiple of 8 up to 128.
+extern "C" int slab_packed_attn_fwd(const void* q, const void* k, const void* v, void* out, void* rest, void* lse,
+                                    const void* plan,
                                     int rows, int hq, int hkv, int d, long q_ts, long q_hs, long k_ts, long k_hs, long v_ts,
                                     long v_hs, int window, float scale, void* counter, void* status, void* stream) {
   using namespace slab;
@@ -762,6 +771,7 @@ extern "C" int slab_packed_attn_fwd(const void* q, const void* k, const void* v,
   if ((rc = pa_make_map(&mv, v, rows, hkv, d, v_ts, v_hs)) != 0) return rc;
   PackedFwdParams p;
   p.out = (__nv_bfloat16*)out;
+  p.rest = (int8_t*)rest;
   p.lse = (float*)lse;
   p.plan = (const int*)plan;
   p.q = {(const __nv_bfloat16*)q, q_ts, q_hs};

@@ -3,7 +3,7 @@
 //   p_ij = exp2(scale_log2 q_i.k_j - lse_i)     delta_i = do_i.o_i      ds_ij = p_ij (do_i.v_j - delta_i)
 //   dv_j = sum_i p_ij do_i      dk_j = scale sum_i ds_ij q_i      dq_i = scale sum_j ds_ij k_j
 //
-// Two kernels behind a small one for delta: one per query tile for dq, one per key tile for dk and dv.  Each makes the
+// delta is made from the output with its lower half (packed_attention.cuh).  Two kernels behind the one for delta: one per query tile for dq, one per key tile for dk and dv.  Each makes the
 // scores and their gradient again (7 products of 128 x 128 x D a tile pair where one kernel could do with 5), but no sum
 // leaves the tensor cores before it is whole: no atomics, no fp32 copy of dq, and the same bits every time.
 //
@@ -44,8 +44,8 @@ __device__ __forceinline__ void pb_bulk_load(void* dst, const void* src, uint32_
 // reads whole lines.  Rows behind the buffer's end, up to whole tiles, get zero.
 template <int DP>
 __global__ void __launch_bounds__(256)
-packed_delta_kernel(const __nv_bfloat16* out, const __nv_bfloat16* dout, float* delta, int rows, int padded, int hq, int d,
-                    long do_ts, long do_hs, int* counter) {
+packed_delta_kernel(const __nv_bfloat16* out, const int8_t* rest, const __nv_bfloat16* dout, float* delta, int rows, int padded, int hq,
+                    int d, long do_ts, long do_hs, int* counter) {
   if (blockIdx.x == 0 && threadIdx.x < 2) counter[threadIdx.x] = 0;    // of the two kernels behind this one
   constexpr int LANES = DP / 8, ROWS = 8;
   const long unit = (long)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
@@ -53,23 +53,30 @@ packed_delta_kernel(const __nv_bfloat16* out, const __nv_bfloat16* dout, float* 
   const int head = (int)(unit % hq), row0 = (int)(unit / hq) * ROWS;
   if (row0 >= padded) return;                  // (units of a warp end together: 32 / LANES divides ROWS of padded's 128)
   uint4 o[ROWS], g[ROWS];
+  uint2 r[ROWS];
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) {
     o[i] = g[i] = make_uint4(0u, 0u, 0u, 0u);
+    r[i] = make_uint2(0u, 0u);
     if (row0 + i < rows && c < d) {
-      o[i] = __ldg(reinterpret_cast<const uint4*>(out + ((size_t)(row0 + i) * hq + head) * d + c));
+      const size_t at = ((size_t)(row0 + i) * hq + head) * d + c;
+      o[i] = __ldg(reinterpret_cast<const uint4*>(out + at));
+      r[i] = __ldg(reinterpret_cast<const uint2*>(rest + at));
       g[i] = __ldg(reinterpret_cast<const uint4*>(dout + (size_t)(row0 + i) * do_ts + (size_t)head * do_hs + c));
     }
   }
   float sum[ROWS];
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) {
-    float x[8], y[8];
-    unpack8(*reinterpret_cast<const bf16x8*>(&o[i]), x);
+    const uint32_t ow[4] = {o[i].x, o[i].y, o[i].z, o[i].w}, rw[2] = {r[i].x, r[i].y};
+    float y[8];
     unpack8(*reinterpret_cast<const bf16x8*>(&g[i]), y);
     sum[i] = 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sum[i] = fmaf(x[e], y[e], sum[i]);
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t bits = (e & 1) ? ow[e >> 1] >> 16 : ow[e >> 1] & 0xffffu;
+      sum[i] = fmaf(pa_unrest(bits, (int)(int8_t)(rw[e >> 2] >> (8 * (e & 3)))), y[e], sum[i]);
+    }
   }
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) {
@@ -553,27 +560,23 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       __nv_bfloat16* dq_row = p.dq + ((size_t)row * p.Hq + it.head) * p.D;
       float sum = 0.f;
 #pragma unroll 1
-      for (int c = 0; c < DP; c += 32) {
-        uint32_t o[32];
+      for (int c = 0; c < DP; c += 16) {
+        uint32_t o[16];
         if (it.n > 0) {
-          tmem_ld_32x32(base + c, o);
+          pa_tmem_ld_16(base + c, o);
           tmem_ld_wait();
-          if (c + 32 == DP) {                  // all read: the next item's products may come
+          if (c + 16 == DP) {                  // all read: the next item's products may come
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(dq_empty);
           }
         }
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
+        for (int e = 0; e < 16; ++e) {
           if (!sees) o[e] = 0u;
           sum += fabsf(__uint_as_float(o[e]));
         }
-        if (row < p.rows) {
-#pragma unroll
-          for (int e = 0; e < 32; e += 16)
-            if (c + e < p.D) pa_put16(dq_row + c + e, o, e, p.scale, wide, p.D - c - e);
-        }
+        if (row < p.rows && c < p.D) pa_put16(dq_row + c, o, 0, p.scale, wide, p.D - c);
       }
       for (uint32_t m = __ballot_sync(0xffffffffu, sees && !pa_finite(sum)); m; m &= m - 1) {
         const int who = __ffs(m) - 1;
@@ -875,33 +878,31 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         __nv_bfloat16* to = (which == 0 ? p.dv : p.dk) + at;
         float* part = p.partial + (size_t)(2 * it.part + (which == 0)) * p.rows * p.Hkv * p.D + at;
 #pragma unroll 1
-        for (int c = 0; c < DP; c += 32) {
-          uint32_t o[32];
+        for (int c = 0; c < DP; c += 16) {
+          uint32_t o[16];
           if (it.n > 0) {
-            tmem_ld_32x32(base + which * 128 + c, o);
+            pa_tmem_ld_16(base + which * 128 + c, o);
             tmem_ld_wait();
-            if (which == 1 && c + 32 == DP) {                  // all read: the next item's products may come
+            if (which == 1 && c + 16 == DP) {                  // all read: the next item's products may come
               tc_fence_before();
               __syncwarp();
               if (lane == 0) mbar_arrive(out_empty);
             }
           }
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
+          for (int e = 0; e < 16; ++e) {
             if (!any) o[e] = 0u;
             bad[which] += fabsf(__uint_as_float(o[e]));
           }
           if (row < p.rows) {
             if (p.splits > 1) {
 #pragma unroll
-              for (int e = 0; e < 32; e += 4)
+              for (int e = 0; e < 16; e += 4)
                 if (c + e < p.D)
                   *reinterpret_cast<float4*>(part + c + e) = make_float4(__uint_as_float(o[e]) * f, __uint_as_float(o[e + 1]) * f,
                                                                          __uint_as_float(o[e + 2]) * f, __uint_as_float(o[e + 3]) * f);
-            } else {
-#pragma unroll
-              for (int e = 0; e < 32; e += 16)
-                if (c + e < p.D) pa_put16(to + c + e, o, e, f, wide, p.D - c - e);
+            } else if (c < p.D) {
+              pa_put16(to + c, o, 0, f, wide, p.D - c);
             }
           }
         }
@@ -981,9 +982,10 @@ extern "C" int slab_packed_attn_splits(int rows, int hq, int hkv) {
   return s;
 }
 
-// q, k, v, dout with token and head strides as in slab_packed_attn_fwd; out, dq, dk, dv contiguous; lse from the forward pass,
+// q, k, v, dout with token and head strides as in slab_packed_attn_fwd; out, rest, dq, dk, dv contiguous; rest and lse from the forward pass,
 // delta [Hq, tiles * 128] and counter [2] int32 scratch; partial: scratch of splits * 2 * rows * Hkv * D floats where splits > 1.
-extern "C" int slab_packed_attn_bwd(const void* q, const void* k, const void* v, const void* out, const void* dout, const void* lse,
+extern "C" int slab_packed_attn_bwd(const void* q, const void* k, const void* v, const void* out, const void* rest,
+                                    const void* dout, const void* lse,
                                     const void* plan, void* dq, void* dk, void* dv, void* delta, void* counter, void* partial, int splits,
                                     int rows, int hq, int hkv, int d, long q_ts, long q_hs, long k_ts, long k_hs, long v_ts,
                                     long v_hs, long do_ts, long do_hs, int window, float scale, void* status, void* stream) {
@@ -1003,11 +1005,11 @@ extern "C" int slab_packed_attn_bwd(const void* q, const void* k, const void* v,
   const int padded = (rows + PA_TILE - 1) / PA_TILE * PA_TILE;
   const long units = (long)padded / 8 * hq, per = d <= 64 ? 32 : 16;
   if (d <= 64)
-    packed_delta_kernel<64><<<(unsigned)((units + per - 1) / per), 256, 0, st>>>((const __nv_bfloat16*)out, (const __nv_bfloat16*)dout,
-        (float*)delta, rows, padded, hq, d, do_ts, do_hs, (int*)counter);
+    packed_delta_kernel<64><<<(unsigned)((units + per - 1) / per), 256, 0, st>>>((const __nv_bfloat16*)out, (const int8_t*)rest,
+        (const __nv_bfloat16*)dout, (float*)delta, rows, padded, hq, d, do_ts, do_hs, (int*)counter);
   else
-    packed_delta_kernel<128><<<(unsigned)((units + per - 1) / per), 256, 0, st>>>((const __nv_bfloat16*)out, (const __nv_bfloat16*)dout,
-        (float*)delta, rows, padded, hq, d, do_ts, do_hs, (int*)counter);
+    packed_delta_kernel<128><<<(unsigned)((units + per - 1) / per), 256, 0, st>>>((const __nv_bfloat16*)out, (const int8_t*)rest,
+        (const __nv_bfloat16*)dout, (float*)delta, rows, padded, hq, d, do_ts, do_hs, (int*)counter);
   PackedBwdParams p;
   p.dq = (__nv_bfloat16*)dq;
   p.dk = (__nv_bfloat16*)dk;

@@ -20,9 +20,9 @@ from . import cuda
 
 cuda.register("slab_packed_plan", "piippp")
 cuda.register("slab_packed_plan_tokens", "piilppp")
-cuda.register("slab_packed_attn_fwd", "pppppp" + "iiii" + "llllll" + "if" + "ppp")
+cuda.register("slab_packed_attn_fwd", "ppppppp" + "iiii" + "llllll" + "if" + "ppp")
 cuda.register("slab_packed_attn_splits", "iii")
-cuda.register("slab_packed_attn_bwd", "p" * 13 + "i" + "iiii" + "llllllll" + "if" + "pp")
+cuda.register("slab_packed_attn_bwd", "p" * 14 + "i" + "iiii" + "llllllll" + "if" + "pp")
 cuda._KERNELS_PER_CALL.update({"slab_packed_plan": 2, "slab_packed_plan_tokens": 3, "slab_packed_attn_bwd": 3})
 cuda._STATUS_NAMES.update({40: "PACKED_ATTN_Q", 41: "PACKED_ATTN_KV_FULL", 42: "PACKED_ATTN_EMPTY", 43: "PACKED_ATTN_S",
                            44: "PACKED_ATTN_P", 45: "PACKED_ATTN_OUT", 46: "PACKED_ATTN_ITEM"})
@@ -144,24 +144,26 @@ def _readable(t):
     return t.clone(memory_format=torch.contiguous_format), h * d, d
 
 
-def forward(q, k, v, documents: PackedDocuments, scale: float, window: int = 0):
-    """``(out [rows, Hq, d], lse)``, ``lse`` the base-2 log-sum-exp of the scaled scores, ``[Hq, tiles * 128]`` flat, with the
-    kernel's work counter behind it."""
+def forward(q, k, v, documents: PackedDocuments, scale: float, window: int = 0, grads: bool = True):
+    """``(out [rows, Hq, d], rest, lse)``: ``rest`` the output's lower half (int8, most of what bf16 leaves of fp32; None without
+    gradients to come), ``lse`` the base-2 log-sum-exp of the scaled scores, ``[Hq, tiles * 128]`` flat, with the kernel's
+    work counter behind it."""
     rows, hq, d = q.shape
     out = torch.empty((rows, hq, d), dtype=q.dtype, device=q.device)
     stats = hq * ((rows + TILE - 1) // TILE * TILE)
     lse = torch.empty(stats + 1, dtype=torch.float32, device=q.device)
+    rest = torch.empty((rows, hq, d), dtype=torch.int8, device=q.device) if grads else None
     q, qt, qh = _readable(q)
     k, kt, kh = _readable(k)
     v, vt, vh = _readable(v)
     with cuda.on_device(q):
-        cuda.call("slab_packed_attn_fwd", q, k, v, out, lse, documents.plan, rows, hq, k.shape[1], d, qt, qh, kt, kh, vt, vh,
+        cuda.call("slab_packed_attn_fwd", q, k, v, out, rest, lse, documents.plan, rows, hq, k.shape[1], d, qt, qh, kt, kh, vt, vh,
                   min(window, rows), scale, lse.data_ptr() + 4 * stats, cuda.status_word(q.device), cuda.stream())
-    return out, lse
+    return out, rest, lse
 
 
-def backward(q, k, v, out, lse, dout, documents: PackedDocuments, scale: float, window: int = 0):
-    """``(dq, dk, dv)`` from the forward pass's inputs, output and log-sum-exp.  Where a group's heads are cut into parts
+def backward(q, k, v, out, rest, lse, dout, documents: PackedDocuments, scale: float, window: int = 0):
+    """``(dq, dk, dv)`` from what the forward pass took and returned.  Where a group's heads are cut into parts
     (few key tiles for the SMs), the parts' sums are kept in fp32 and added up in their order."""
     rows, hq, d = q.shape
     hkv = k.shape[1]
@@ -177,7 +179,7 @@ def backward(q, k, v, out, lse, dout, documents: PackedDocuments, scale: float, 
     with cuda.on_device(q):
         splits = cuda.lib().slab_packed_attn_splits(rows, hq, hkv)
         partial = torch.empty(splits * 2 * dk.numel(), dtype=torch.float32, device=q.device) if splits > 1 else None
-        cuda.call("slab_packed_attn_bwd", q, k, v, out, dout, lse, documents.plan, dq, dk, dv, delta,
+        cuda.call("slab_packed_attn_bwd", q, k, v, out, rest, dout, lse, documents.plan, dq, dk, dv, delta,
                   delta.data_ptr() + 4 * stats, partial, splits, rows, hq, hkv, d, qt, qh, kt, kh, vt, vh, gt, gh,
                   min(window, rows), scale, cuda.status_word(q.device), cuda.stream())
         if splits > 1:
@@ -189,19 +191,18 @@ class _PackedAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, documents, scale, window):
         q, k, v = (_readable(t)[0] for t in (q, k, v))         # copied once, if at all, for both passes
-        out, lse = forward(q, k, v, documents, scale, window)
-        ctx.save_for_backward(q, k, v, out, lse)
+        out, rest, lse = forward(q, k, v, documents, scale, window)
+        ctx.save_for_backward(q, k, v, out, rest, lse)
         ctx.documents, ctx.scale, ctx.window = documents, scale, window
         return out
 
     @staticmethod
     @cuda.first_order
     def backward(ctx, g):
-        q, k, v, out, lse = ctx.saved_tensors
-        return backward(q, k, v, out, lse, g, ctx.documents, ctx.scale, ctx.window) + (None, None, None)
+        return backward(*ctx.saved_tensors, g, ctx.documents, ctx.scale, ctx.window) + (None, None, None)
 
 
 def attention(q, k, v, documents: PackedDocuments, scale: float, window: int = 0):
     if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)):
-        return forward(q, k, v, documents, scale, window)[0]
+        return forward(q, k, v, documents, scale, window, grads=False)[0]
     return _PackedAttention.apply(q, k, v, documents, scale, window)
