@@ -5,7 +5,7 @@
 
 Times the library path of ``ops/attention.py`` (cuDNN SDPA / flash-attn) and, when the hand-written forward is
 switched on (``SLAB_ATTENTION_KERNEL=1``; ``SLAB_ATTENTION_KERNEL_BWD=1`` adds its backward), ``csrc/attention.cu`` on the
-same packed-qkv inputs, checks the two outputs
+same packed-qkv inputs, and ``ops.packed_attention`` on the rows as packed documents; checks the outputs
 against each other, and reports TFLOP/s (causal: half of the dense FLOPs; a window counts only the visible keys)
 against the measured bf16 GEMM peak.  CUDA events, 3 warm-ups, median, 256 MB write between iterations (cold L2).
 
@@ -80,7 +80,7 @@ def main(argv=None) -> int:
     def line(name, ms, flops):
         tf = flops / (ms * 1e9)
         res[name] = {"ms": ms, "tflops": tf, "of_peak": tf / peak}
-        print(f"{name:34s} {ms:9.3f} ms {tf:9.0f} TFLOP/s  {tf / peak:5.2f} of {'measured' if peaks else 'fallback'} GEMM peak")
+        print(f"{name:44s} {ms:9.3f} ms {tf:9.0f} TFLOP/s  {tf / peak:5.2f} of {'measured' if peaks else 'fallback'} GEMM peak")
 
     line("library forward", time_cuda(lambda: _library(q, k, v, scale, a.window), flush, a.iters), flops_fwd)
     qg, kg, vg = (t.detach().clone().requires_grad_(True) for t in (q, k, v))
@@ -114,6 +114,33 @@ def main(argv=None) -> int:
             cops.check_status()
     else:
         print("kernel forward: skipped (set SLAB_ATTENTION_KERNEL=1; needs head dim 64 / 128 and seq % 128 == 0)")
+    if d % 8 == 0 and d <= 128:
+        # the batch's rows as packed documents, one each, and cut into ragged ones
+        from system_lab_b200.ops import packed as pk_ops
+        for name, cuts in (("one document per row", [s] * b), ("documents of %d" % max(s // 6, 1), None)):
+            if cuts is None:
+                import random
+                rng, cuts = random.Random(0), []
+                for _ in range(b):
+                    left = s
+                    while left:
+                        n = min(left, int(rng.lognormvariate(math.log(max(s // 6, 1)), 0.8)) + 1)
+                        cuts.append(n)
+                        left -= n
+            cu = [0]
+            for n in cuts:
+                cu.append(cu[-1] + n)
+            docs = pk_ops.pack_documents(torch.tensor(cu, device=dev), b * s)
+            qp, kp, vp, gp = (t.flatten(0, 1) for t in (q, k, v, g))
+            fl = 4.0 * hq * d * sum(visible_pairs(n, a.window) for n in cuts)
+            saved = pk_ops.forward(qp, kp, vp, docs, scale, a.window)
+            if len(cuts) == b:
+                ref = _library(q, k, v, scale, a.window).flatten(0, 1)
+                print(f"packed vs library: max abs difference {(saved[0].float() - ref.float()).abs().max().item():.4f}")
+            line(f"packed forward, {name}", time_cuda(lambda: pk_ops.forward(qp, kp, vp, docs, scale, a.window), flush, a.iters), fl)
+            line(f"packed backward, {name}",
+                 time_cuda(lambda: pk_ops.backward(qp, kp, vp, *saved, gp, docs, scale, a.window), flush, a.iters), 2.5 * fl)
+            cops.check_status()
     if a.json:
         os.makedirs(os.path.dirname(a.json) or ".", exist_ok=True)
         json.dump(res, open(a.json, "w"), indent=2)

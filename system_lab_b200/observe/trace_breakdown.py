@@ -33,7 +33,9 @@ RULES: list[tuple[str, tuple[str, ...]]] = [
     ("slab_quant", ("quant_1x128_kernel", "quant_128x128_kernel", "quant_rowwise_kernel", "quant_rowwise_long",
                     "quant_tensorwise_kernel", "amax_bf16_kernel")),
     ("slab_optimizer", ("adamw_kernel", "adamw8_kernel", "sumsq_kernel")),
-    ("slab_attn", ("slab_attn", "attn_fwd_kernel", "attn_bwd_kernel")),
+    ("slab_attn", ("slab_attn", "attn_fwd_kernel", "attn_bwd_kernel", "slab::packed_")),
+    ("slab_embedding", ("embedding_fwd_kernel", "embedding_sort_kernel", "embedding_sum_kernel", "embedding_join_kernel")),
+    ("slab_dropout", ("slab::dropout_kernel",)),
     ("slab_fsdp", ("fsdp_gather_kernel", "fsdp_reduce_scatter_kernel", "fsdp_stage_kernel", "fsdp_rs_adamw")),
     ("nccl_rs", ()), ("nccl_ar", ()), ("nccl_ag", ()), ("nccl_a2a", ()), ("nccl_bcast", ()), ("nccl_generic", ()),
     ("grouped_gemm", ("_grouped", "groupedgemm", "grouped_gemm", "groupedlinear", "te_grouped")),
