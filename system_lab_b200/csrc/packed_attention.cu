@@ -383,7 +383,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   PaQueue queue;
   uint64_t* o_empty = o_full + 2;
   uint64_t* l_full = o_empty + 2;
-  queue.full = l_full + 2;
+  queue.full = l_full + 4;
   queue.empty = queue.full + PA_SLOTS;
   queue.want = queue.empty + PA_SLOTS;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(queue.want + 1);
@@ -404,6 +404,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       mbar_init(&o_full[g], 1);
       mbar_init(&o_empty[g], 4);
       mbar_init(&l_full[g], 4);
+      mbar_init(&l_full[2 + g], 4);
     }
     for (int s = 0; s < NST; ++s) {
       mbar_init(&kv_full[s], 1);
@@ -437,6 +438,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       uint32_t ph = 1;
       bool ok = true;
       int v_row = -1, v_head = 0;              // V tile of the step before, the stage's other half
+      bool empty = false;                      // an item without key tiles came: so are all behind it, and the last V tile is due
       auto load_stage = [&](int k_row, int k_head) {             // (no K behind the last item's last step)
         ok = ok && pa_wait(&kv_empty[st], ph, abort_flag, p.status, ST_PATTN_EMPTY);
         if (ok && elect_one()) {
@@ -451,8 +453,8 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       PaItem next;
       while (ok && reader.next(queue, next, abort_flag, p.status)) {
         const PackedFwdItem it(next);
-        if (it.n < 0) break;
-        if (it.n == 0) continue;
+        empty = it.n == 0;
+        if (it.n <= 0) break;
         load_stage(it.j0 * PA_TILE, it.hk);
         for (int g = 0; g < 2; ++g) {
           ok = ok && pa_wait(&q_empty[g], (done & 1) ^ 1, abort_flag, p.status, ST_PATTN_EMPTY);
@@ -469,6 +471,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         ++done;
       }
       if (ok && v_row >= 0) load_stage(-1, 0);
+      if (ok && empty) reader.drain(queue, abort_flag, p.status);
     } else if (warp == 11) {
       pa_schedule(queue, items, p.counter, [&](int idx) { return pf_item(p, plan, idx, items > (int)gridDim.x); }, abort_flag, p.status);
     } else if (warp == 8) {
@@ -481,14 +484,13 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       const uint64_t kd = make_smem_desc(smem_u32(kv_s + L::TILE), 16, 1024, 2);
       PaReader reader;
       bool ok = true;
-      auto next_len = [&]() {                  // key tiles of the next item that has any, 0 behind the last
+      bool empty = false;                      // an item without key tiles came: so are all behind it
+      auto next_len = [&]() {                  // key tiles of the next item, 0 behind the last that has any
         PaItem next;
-        while (ok) {
-          ok = reader.next(queue, next, abort_flag, p.status);
-          const int n = warp_uniform(next.v[7]);
-          if (ok && n != 0) return n > 0 ? n : 0;
-        }
-        return 0;
+        ok = ok && reader.next(queue, next, abort_flag, p.status);
+        const int n = ok ? warp_uniform(next.v[7]) : 0;
+        empty = ok && n == 0;
+        return n > 0 ? n : 0;
       };
       // This warp's own instructions bound a step once its waits (some 250 cycles each beside the softmax warps) follow one
       // another: what the next step needs is waited for and counted up before the second tile's probabilities are.  (Stages
@@ -570,6 +572,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           umma_commit(&kv_empty[s0]);
         }
       }
+      if (ok && empty) reader.drain(queue, abort_flag, p.status);
     }
   } else if (warp < 8) {
     reg_inc<192>();
@@ -618,11 +621,13 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           pf_part<DP>(s_addr, o_addr, p.scale_log2, vis, first, lastk, m, la, lb, &p_full[g]);
       }
       if (!ok) break;
-      if (it.n > 0) {                          // (the output warps are done with what the item before the last one left there)
+      // (The output warps are done with what the item before the last one left there.  They may not have looked at the last
+      // one's yet, a tile with a short item behind it: so each buffer has its barrier.)
+      if (it.n > 0) {
         stat_s[(buf * 2 + g) * 128 + r128] = make_float2((la.x + la.y) + (lb.x + lb.y), m);
-        buf ^= 1;
         __syncwarp();
-        if (lane == 0) mbar_arrive(&l_full[g]);
+        if (lane == 0) mbar_arrive(&l_full[2 * buf + g]);
+        buf ^= 1;
       }
     }
   } else {
@@ -650,7 +655,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         const bool sees = lo <= row;           // (a row that sees nothing gets zeros)
         float l = 0.f, m = 0.f;
         if (it.n > 0) {
-          ok = pa_wait(&l_full[g], done & 1, abort_flag, p.status, ST_PATTN_OUT) &&
+          ok = pa_wait(&l_full[2 * (done & 1) + g], (done >> 1) & 1, abort_flag, p.status, ST_PATTN_OUT) &&
                pa_wait(&o_full[g], done & 1, abort_flag, p.status, ST_PATTN_OUT);
           if (!ok) break;
           tc_fence_after();

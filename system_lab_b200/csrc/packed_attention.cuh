@@ -51,7 +51,9 @@ inline __host__ __device__ PackedPlan packed_plan(const int* base, int rows) {
 // the plan's dependent loads (2 to 3 thousand cycles an item), when the softmax warps are PA_EARLY steps from their item's end:
 // taken as early as there is room, the first three rounds would be dealt out at once (one document of 8192 rows: dk and dv 2101
 // us, 1755 so).  Issuers and copies may be an item ahead of the softmax warps; nobody waits for an item that is given out only
-// once he has done something for the one before.
+// once he has done something for the one before.  So issuers (and the forward pass's copies) stop at the first item without steps (all behind it, by falling
+// work, have none either), finish what they have, and only then read the rest (PaReader::drain): output warps that still wait
+// for the issuer's last product have not read that item, and the second one behind it needs its slot.
 constexpr int PA_SLOTS = 2, PA_EARLY = 3;
 struct PaQueue {
   uint64_t* full;                            // [PA_SLOTS]
@@ -67,6 +69,8 @@ struct PaReader {
   int s = 0;
   uint32_t ph = 0;
   __device__ __forceinline__ bool next(const PaQueue& q, PaItem& it, volatile int* abort_flag, int* status);
+  // reads items up to the end, for a role that has nothing to do for them
+  __device__ __forceinline__ void drain(const PaQueue& q, volatile int* abort_flag, int* status);
 };
 
 // ---------------------------------------------------------------- tensor memory
@@ -126,6 +130,10 @@ __device__ __forceinline__ bool PaReader::next(const PaQueue& q, PaItem& it, vol
   if ((threadIdx.x & 31) == 0) mbar_arrive(&q.empty[s]);
   if (++s == PA_SLOTS) { s = 0; ph ^= 1; }
   return true;
+}
+__device__ __forceinline__ void PaReader::drain(const PaQueue& q, volatile int* abort_flag, int* status) {
+  PaItem it;
+  while (next(q, it, abort_flag, status) && it.v[7] >= 0) {}
 }
 // The taking warp: decode(index) makes an item of the list's index.
 template <typename Decode>

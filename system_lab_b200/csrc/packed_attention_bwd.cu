@@ -403,7 +403,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       const uint64_t qd = make_smem_desc(smem_u32(q_s), 16, 1024, 2), dod = make_smem_desc(smem_u32(do_s), 16, 1024, 2);
       const uint64_t kd = make_smem_desc(smem_u32(k_s), 16, 1024, 2), vd = make_smem_desc(smem_u32(v_s), 16, 1024, 2);
       const uint64_t kt = make_smem_desc(smem_u32(k_s), 16384, 1024, 2);      // K with its rows as the reduction
-      bool ok = true, more = true;             // more: the queue has not ended
+      bool ok = true, more = true, empty = false;   // more: no item without steps, and not the end, has come; empty: the former has
       PaReader reader;
       // Scores run two steps ahead, dP one; each walk counts its item's steps, stages and parities (counted, not computed: see
       // elect_one).  What a product needs beside ds is waited for while others run.
@@ -415,8 +415,9 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           PaItem next;
           ok = reader.next(queue, next, abort_flag, p.status);
           const int n = warp_uniform(next.v[7]);
-          more = ok && n >= 0;
-          if (more && n > 0) {
+          more = ok && n > 0;
+          empty = ok && n == 0;
+          if (more) {
             if (lane == 0) lens[ws.items & 3] = n;
             __syncwarp();
             ws.begin(n);
@@ -491,6 +492,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         qbuf ^= 1;
         if (++sq == KST) sq = 0;
       }
+      if (ok && empty) reader.drain(queue, abort_flag, p.status);
     }
   } else if (warp < 8) {
     reg_inc<176>();
@@ -727,7 +729,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       const uint64_t kd = make_smem_desc(smem_u32(k_s), 16, 1024, 2), vd = make_smem_desc(smem_u32(v_s), 16, 1024, 2);
       const uint64_t qd = make_smem_desc(smem_u32(q_s), 16, 1024, 2), dod = make_smem_desc(smem_u32(do_s), 16, 1024, 2);
       const uint64_t qt = make_smem_desc(smem_u32(q_s), 16384, 1024, 2), dot = make_smem_desc(smem_u32(do_s), 16384, 1024, 2);
-      bool ok = true, more = true;             // more: the queue has not ended
+      bool ok = true, more = true, empty = false;   // more: no item without steps, and not the end, has come; empty: the former has
       PaReader reader;
       // (stages and parities are counted, not computed: see elect_one)
       PbWalk w;                                // the step whose scores and dP come next
@@ -736,8 +738,9 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           PaItem next;
           ok = reader.next(queue, next, abort_flag, p.status);
           const int n = warp_uniform(next.v[7]);
-          more = ok && n >= 0;
-          if (more && n > 0) w.begin(n);
+          more = ok && n > 0;
+          empty = ok && n == 0;
+          if (more) w.begin(n);
         }
       };
       bool done = false;                       // behind the last step
@@ -800,6 +803,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         dprob();
         par ^= 1;
       }
+      if (ok && empty) reader.drain(queue, abort_flag, p.status);
     }
   } else if (warp < 8) {
     reg_inc<176>();

@@ -150,6 +150,41 @@ def test_rows_behind_the_last_document(hq, hkv, d):
         assert (x[311:] == 0).all()
 
 
+@pytest.mark.parametrize("hq,hkv,d", [(8, 8, 64), (8, 2, 128), (3, 1, 128)])
+def test_blocks_with_documents_also_take_tiles_without(hq, hkv, d):
+    """Far more tiles without documents than blocks: those whose tile has some meet many empty ones behind it."""
+    cu = cu_of([40, 300])
+    q, k, v, dout = make(40000, hq, hkv, d)
+    docs = ops.pack_documents(torch.tensor(cu, dtype=torch.int32, device=DEV), len(q))
+    for _ in range(3):
+        got = run(q, k, v, docs, dout)
+        for x in got:
+            assert not x[cu[-1]:].any()
+        close([x[:cu[-1]] for x in got], reference(q[:cu[-1]], k[:cu[-1]], v[:cu[-1]], cu, 1 / math.sqrt(d), 0, dout[:cu[-1]]))
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(4, 2, 64), (3, 3, 128)])
+def test_short_items_behind_rows_that_are_made_again(hq, hkv, d):
+    """One tile of an item is stored slowly (all its rows are NaN and made again) while the next item is one step long."""
+    cu = cu_of([128] * 400)
+    q, k, v, _ = make(cu[-1], hq, hkv, d)
+    bad = 200 * 128
+    q[:bad, 0] = float("nan")
+    docs = ops.pack_documents(torch.tensor(cu, dtype=torch.int32, device=DEV), len(q))
+    scale = 1 / math.sqrt(d)
+    qq, kk, vv = (t.unflatten(0, (400, 128)).transpose(1, 2).double() for t in (q, k, v))
+    kk, vv = (t.repeat_interleave(hq // hkv, dim=1) for t in (kk, vv))
+    p = (qq @ kk.mT * scale).masked_fill(~torch.ones(128, 128, dtype=torch.bool, device=DEV).tril(), -math.inf).softmax(-1)
+    want, bound = ((p @ x).transpose(1, 2).flatten(0, 1) for x in (vv, vv.abs()))
+    for _ in range(3):
+        out = ops.packed_attention(q, k, v, docs)
+        torch.cuda.synchronize()
+        cuda.check_status(out.device)
+        assert out[:bad, 0].isnan().all()
+        close([out[:, 1:]], [(want[:, 1:], bound[:, 1:], None)])
+        close([out[bad:]], [(want[bad:], bound[bad:], None)])
+
+
 @pytest.mark.parametrize("what", ["q", "k", "v", "dout"])
 @pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
 @pytest.mark.parametrize("window", [0, 16])
