@@ -388,7 +388,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   queue.want = queue.empty + PA_SLOTS;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(queue.want + 1);
   queue.slot = reinterpret_cast<int4*>(smem + 512);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);         // [3], see pa_wait
   float2* stat_s = reinterpret_cast<float2*>(smem + L::STAT_OFF);       // [2 items][2 tiles][128] sum and maximum of a row
   uint8_t* q_s = smem + L::Q_OFF;
   uint8_t* kv_s = smem + L::KV_OFF;
@@ -415,7 +415,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       mbar_init(&queue.empty[q], 14);          // softmax warps, output warps, issuer, copies
     }
     mbar_init(queue.want, 1);
-    *abort_flag = 0;
+    pa_init_abort(abort_flag);
     fence_mbar_init();
     prefetch_tmap(&map_q);
     prefetch_tmap(&map_k);
@@ -692,6 +692,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           const int who = __ffs(again) - 1;
           __syncwarp();
           pf_redo(p, row - lane + who, head, __shfl_sync(0xffffffffu, lo, who));
+          pa_redone(abort_flag);
         }
       }
       if (it.n > 0) ++done;

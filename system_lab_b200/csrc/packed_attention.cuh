@@ -116,10 +116,39 @@ __device__ __forceinline__ void reg_inc() { asm volatile("setmaxnreg.inc.sync.al
 template <int N>
 __device__ __forceinline__ void reg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
-// mbar_wait_warp, shorter where the barrier has completed already
+// A bounded wait of a whole warp (mbar_wait_warp) that is patient while rows are made again: a tile of them can take longer
+// than the limit (a key tile of 64 heads x 6000 rows: some 3 s).  Behind the abort flag stands the time at which the last such
+// row was done (pa_redone); the limit counts from there.
+__device__ __forceinline__ bool pa_wait_slow(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
+#pragma unroll 1
+  for (int i = 0; i < 32; ++i)
+    if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = globaltimer_ns();
+  uint32_t spins = 0;
+  while (true) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((++spins & 255u) == 0) {
+      if (*abort_flag) return false;
+      if (globaltimer_ns() - t0 > SLAB_WAIT_NS) {
+        const uint64_t row = *reinterpret_cast<volatile uint64_t*>(abort_flag + 1);
+        if (globaltimer_ns() - row > SLAB_WAIT_NS) {
+          *abort_flag = 1;
+          atomicCAS(status, 0, code);
+          return false;
+        }
+      }
+    }
+  }
+}
 __device__ __forceinline__ bool pa_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
   if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
-  return mbar_wait_warp(bar, parity, abort_flag, status, code);
+  return __all_sync(0xffffffffu, pa_wait_slow(bar, parity, abort_flag, status, code));
+}
+__device__ __forceinline__ void pa_redone(volatile int* abort_flag) {
+  if ((threadIdx.x & 31) == 0) *reinterpret_cast<volatile uint64_t*>(abort_flag + 1) = globaltimer_ns();
+}
+__device__ __forceinline__ void pa_init_abort(volatile int* abort_flag) {
+  abort_flag[0] = abort_flag[1] = abort_flag[2] = 0;
 }
 
 __device__ __forceinline__ bool PaReader::next(const PaQueue& q, PaItem& it, volatile int* abort_flag, int* status) {

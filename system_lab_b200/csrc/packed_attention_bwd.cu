@@ -342,7 +342,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(queue.want + 1);
   queue.slot = reinterpret_cast<int4*>(smem + 512);
   int* lens = reinterpret_cast<int*>(smem + 768);              // [4] the issuer's items in flight
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);         // [3], see pa_wait
   uint8_t *q_s = smem + L::Q_OFF, *do_s = smem + L::DO_OFF, *k_s = smem + L::K_OFF, *v_s = smem + L::V_OFF;
   const int warp = warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const PackedPlan plan = packed_plan(p.plan, p.rows);
@@ -351,7 +351,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     for (uint64_t* b = q_full; b < queue.empty; ++b) mbar_init(b, b == ds_full ? 8 : b == dq_empty ? 4 : 1);
     for (int q = 0; q < PA_SLOTS; ++q) mbar_init(&queue.empty[q], 14);           // softmax warps, output warps, issuer, copies
     mbar_init(queue.want, 1);
-    *abort_flag = 0;
+    pa_init_abort(abort_flag);
     fence_mbar_init();
     prefetch_tmap(&map_q);
     prefetch_tmap(&map_k);
@@ -584,6 +584,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         const int who = __ffs(m) - 1;
         __syncwarp();
         pb_redo_dq(p, it.row + lg * 32 + who, it.head, __shfl_sync(0xffffffffu, lo, who));
+        pa_redone(abort_flag);
       }
     }
   }
@@ -660,7 +661,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   queue.want = queue.empty + PA_SLOTS;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(queue.want + 1);
   queue.slot = reinterpret_cast<int4*>(smem + 512);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);         // [3], see pa_wait
   float* lse_s = reinterpret_cast<float*>(smem + L::STAT_OFF);
   float* delta_s = lse_s + ST * PA_TILE;
   uint8_t *k_s = smem + L::K_OFF, *v_s = smem + L::V_OFF, *q_s = smem + L::Q_OFF, *do_s = smem + L::DO_OFF;
@@ -672,7 +673,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     for (uint64_t* b = k_full; b < queue.empty; ++b) mbar_init(b, b == p_full || b == ds_full ? 8 : b == out_empty ? 4 : 1);
     for (int q = 0; q < PA_SLOTS; ++q) mbar_init(&queue.empty[q], 14);           // softmax warps, output warps, issuer, copies
     mbar_init(queue.want, 1);
-    *abort_flag = 0;
+    pa_init_abort(abort_flag);
     fence_mbar_init();
     prefetch_tmap(&map_q);
     prefetch_tmap(&map_k);
@@ -917,6 +918,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           const int who = __ffs(m) - 1;
           __syncwarp();
           pb_redo_dkv(p, which == 0, it.row + lg * 32 + who, it.hk, it.h0, it.heads, it.part, __shfl_sync(0xffffffffu, hi, who));
+          pa_redone(abort_flag);
         }
       }
     }

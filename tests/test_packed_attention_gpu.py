@@ -185,6 +185,20 @@ def test_short_items_behind_rows_that_are_made_again(hq, hkv, d):
         close([out[bad:]], [(want[bad:], bound[bad:], None)])
 
 
+def test_rows_made_again_for_longer_than_a_wait_lasts():
+    """Key tiles of the long document take seconds each: every sum of dv meets an infinity in the last row."""
+    lens = [6000] + [100] * 140
+    cu = cu_of(lens)
+    q, k, v, dout = make(cu[-1], 64, 1, 64)
+    dout[5999] = math.inf
+    docs = ops.pack_documents(torch.tensor(cu, dtype=torch.int32, device=DEV), len(q))
+    got = run(q, k, v, docs, dout)                     # (asks for the status)
+    assert got[3][:6000].isinf().all()
+    rest = [x[6000:] for x in (q, k, v)]
+    want = reference(*rest, [c - 6000 for c in cu[1:]], 1 / 8, 0, dout[6000:])
+    close([x[6000:] for x in got], want)
+
+
 @pytest.mark.parametrize("what", ["q", "k", "v", "dout"])
 @pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
 @pytest.mark.parametrize("window", [0, 16])
