@@ -34,7 +34,7 @@ def check(tokens, weight, scale) -> float:
 
 
 def supports(weight, dtype) -> bool:
-    return weight.dtype in _TYPES and dtype in _TYPES and weight.shape[0] < 2 ** 31 and weight.shape[1] < 2 ** 28
+    return weight.dtype in _TYPES and dtype in _TYPES and weight.shape[0] < 2 ** 31 and weight.shape[1] <= 2 ** 23
 
 
 class _Embedding(torch.autograd.Function):
@@ -43,8 +43,8 @@ class _Embedding(torch.autograd.Function):
         tok = tokens.long().contiguous()
         w = weight.contiguous()
         v, h = w.shape
-        if tok.numel() >= 2 ** 31 - 1:
-            raise ValueError(f"{tok.numel()} tokens")
+        if tok.numel() > 2 ** 30:                  # (positions are counted in 32 bits, in whole groups)
+            raise ValueError(f"{tok.numel()} tokens: at most 2^30 in one call")
         out = torch.empty(*tokens.shape, h, dtype=dtype, device=w.device)
         if tok.numel():
             with cuda.on_device(w):

@@ -5,8 +5,8 @@ in one buffer of rows, and a row attends to its own document only (and, with ``w
 the plan of a batch once; every layer's forward and backward pass uses it.  Nothing is read back to the host.
 
 The kernels take bf16 and head widths that are multiples of 8 up to 128, with any token and head strides (slices of a
-packed projection are read where they lie).  Everything else is refused on the GPU: the dense oracle would need memory
-that grows with the square of the length.  CPU tensors take the oracle (``reference.packed_attention``).
+packed projection are read where they lie).  Other types and widths, and CPU tensors, take the oracle
+(``reference.packed_attention``), whose scores lie in memory, 512 query rows at a time.
 
 Reference: the packed fine-tuning batches of ``notes/mlperf-llama/2026-04-29_llama2_70b_lora_baseline_trace_breakdown.md``.
 """
@@ -71,7 +71,9 @@ def pack_documents(cu_seqlens: torch.Tensor, rows: int) -> PackedDocuments:
         lo = torch.where(inside, cu[s], i + 1)
         hi = torch.where(inside, cu[(s + 1).clamp_max(cu.numel() - 1)], i)
         return PackedDocuments(rows, torch.cat([lo, hi]).int())
-    cu = cu_seqlens.to(torch.int32).contiguous()
+    # (offsets past 32 bits have to stay past the buffer's end)
+    cu = cu_seqlens.clamp(-1, 2 ** 31 - 1) if cu_seqlens.dtype == torch.int64 else cu_seqlens
+    cu = cu.to(torch.int32).contiguous()
     plan = torch.empty(_plan_words(rows), dtype=torch.int32, device=cu.device)
     with cuda.on_device(cu):
         cuda.call("slab_packed_plan", cu, cu.numel() - 1, rows, plan, cuda.status_word(cu.device), cuda.stream())

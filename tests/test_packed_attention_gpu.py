@@ -290,6 +290,24 @@ def test_bad_offsets_are_reported_and_stay_inside():
     assert docs.doc_lo.min() >= 0 and docs.doc_hi.max() <= 300
 
 
+@pytest.mark.parametrize("cu", [[0, 2 ** 32 + 300], [0, -2 ** 32 + 100, 300], [2 ** 32, 300]])
+def test_offsets_past_32_bits_are_reported(cu):
+    cuda.clear_status()
+    ops.pack_documents(torch.tensor(cu, dtype=torch.int64, device=DEV), 300)
+    with pytest.raises(cuda.DeviceHang, match="BAD_INDEX"):
+        torch.cuda.synchronize()
+        cuda.check_status(torch.device(DEV, torch.cuda.current_device()))
+    cuda.clear_status()
+
+
+def test_no_documents_at_all():
+    q, k, v, dout = make(500, 4, 2, 64)
+    for cu in ([0], [0, 0, 0]):
+        docs = ops.pack_documents(torch.tensor(cu, dtype=torch.int32, device=DEV), 500)
+        for x in run(q, k, v, docs, dout):
+            assert not x.any()
+
+
 def test_graph_replay_with_new_documents_and_values():
     """The plan and both passes captured once: a replay takes what the buffers hold then."""
     t = 640
