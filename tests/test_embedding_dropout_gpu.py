@@ -190,6 +190,22 @@ def test_dropout(shape, p, residual, dtype):
         assert torch.equal(grads[1], dout)
 
 
+@pytest.mark.parametrize("n", [2 ** 22 - 1, 2 ** 22, 2 ** 22 + 1, 2 ** 22 + 8 * 256 + 5, 2 ** 22 + 8192 + 4099])
+@pytest.mark.parametrize("residual", [False, True])
+def test_dropout_of_many_elements(n, residual):
+    """Around the size from which a thread takes several blocks, whole and ragged."""
+    x = torch.randn(n, device=DEV).bfloat16()
+    r = torch.randn(n, device=DEV).bfloat16() if residual else None
+    t = ref.dropout_threshold(0.25)
+    keep = ref.philox_bits(n, 3, 9, x.device) >= t
+    want = torch.where(keep, x.double() * 65536 / (65536 - t), 0.0) + (r.double() if residual else 0.0)
+    got = ops.dropout(x, 0.25, 3, 9, residual=r)
+    # one rounding to bf16 behind a product and a sum in fp32 (two roundings of 2^-24 of the terms)
+    bound = want.abs() * 2.0 ** -8 + (x.double().abs() * 1.34 + want.abs()) * 2.0 ** -23
+    assert bool(((got.double() - want).abs() <= bound).all())
+    assert not got[~keep].any() if not residual else torch.equal(got[~keep], r[~keep])
+
+
 def test_dropped_elements_may_be_anything():
     x = torch.randn(4096, device=DEV)
     _, keep = plain(x, 0.5, 1, 0, None)
