@@ -39,6 +39,13 @@ __device__ __forceinline__ void pb_bulk_load(void* dst, const void* src, uint32_
                : "memory");
 }
 
+// The three kernels follow one another closely: each lets the next begin once its own blocks all have (griddepcontrol), and waits for
+// the one before where it needs it.  dk and dv wait behind their set-up.  dq needs delta only, which is whole once dk and dv
+// have begun, so its blocks take over SMs as those of dk and dv end; they wait for the last of them before they end
+// themselves, so that what comes behind dq finds dk and dv whole.
+__device__ __forceinline__ void pb_next_may_begin() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void pb_wait_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ================================================================ delta
 // DP / 8 lanes per head, eight neighbouring rows each, all of whose loads are in flight together; heads fastest, so that a block
 // reads whole lines.  Rows behind the buffer's end, up to whole tiles, get zero.
@@ -46,6 +53,7 @@ template <int DP>
 __global__ void __launch_bounds__(256)
 packed_delta_kernel(const __nv_bfloat16* out, const int8_t* rest, const __nv_bfloat16* dout, float* delta, int rows, int padded, int hq,
                     int d, long do_ts, long do_hs, int* counter) {
+  pb_next_may_begin();
   if (blockIdx.x == 0 && threadIdx.x < 2) counter[threadIdx.x] = 0;    // of the two kernels behind this one
   constexpr int LANES = DP / 8, ROWS = 8;
   const long unit = (long)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
@@ -600,6 +608,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
+  if (threadIdx.x == 0) pb_wait_before();      // dk and dv
 }
 
 // ================================================================ dk, dv
@@ -684,6 +693,8 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
+  pb_wait_before();                            // delta, and the counters
+  pb_next_may_begin();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -953,6 +964,20 @@ packed_join_kernel(const float* partial, __nv_bfloat16* dk, __nv_bfloat16* dv, l
   *reinterpret_cast<bf16x8*>(to) = pack8(sum);
 }
 
+template <typename... P, typename... A>
+static cudaError_t pb_launch(void (*kernel)(P...), long blocks, int smem, cudaStream_t stream, A... args) {
+  cudaLaunchAttribute early;
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3((unsigned)blocks);
+  config.blockDim = dim3(PB_THREADS);
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  config.attrs = &early;
+  config.numAttrs = 1;
+  return cudaLaunchKernelEx(&config, kernel, args...);
+}
 template <int DP>
 static int packed_bwd_launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mdo,
                              const PackedBwdParams& p, cudaStream_t stream) {
@@ -962,10 +987,10 @@ static int packed_bwd_launch(const CUtensorMap& mq, const CUtensorMap& mk, const
   SLAB_CUDA_CHECK(cudaFuncSetAttribute(packed_dq_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, PackedDqSmem<DP>::TOTAL));
   SLAB_CUDA_CHECK(cudaFuncSetAttribute(packed_dkv_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, PackedDkvSmem<DP>::TOTAL));
   const int sms = sm_count();
-  packed_dkv_kernel<DP><<<dkv_items < sms ? (int)dkv_items : sms, PB_THREADS, PackedDkvSmem<DP>::TOTAL, stream>>>(
-      mq, mk, mv, mdo, p, (int)dkv_items);
-  packed_dq_kernel<DP><<<dq_items < sms ? (int)dq_items : sms, PB_THREADS, PackedDqSmem<DP>::TOTAL, stream>>>(
-      mq, mk, mv, mdo, p, (int)dq_items);
+  SLAB_CUDA_CHECK(pb_launch(packed_dkv_kernel<DP>, dkv_items < sms ? dkv_items : sms, PackedDkvSmem<DP>::TOTAL, stream, mq, mk, mv, mdo, p,
+                            (int)dkv_items));
+  SLAB_CUDA_CHECK(pb_launch(packed_dq_kernel<DP>, dq_items < sms ? dq_items : sms, PackedDqSmem<DP>::TOTAL, stream, mq, mk, mv, mdo, p,
+                            (int)dq_items));
   if (p.splits > 1) {
     const long n = (long)p.rows * p.Hkv * p.D;
     packed_join_kernel<<<(unsigned)((2 * n / 8 + 255) / 256), 256, 0, stream>>>(p.partial, p.dk, p.dv, n, p.splits);
