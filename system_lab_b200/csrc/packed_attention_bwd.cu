@@ -26,9 +26,9 @@ struct PackedBwdParams {
   PackedRows q, k, v, dout;
   int rows, Hq, Hkv, D;
   int window;
-  int splits;
+  int splits;                    // most parts that partial has room for
   float scale, scale_log2;
-  int* counter;                  // [2] items taken behind the first of every block (dk and dv, dq), zero at launch
+  int* counter;                  // [2] items taken behind the first of every block (dk and dv, dq); [1] parts (packed_delta_kernel)
   int* status;
 };
 
@@ -46,15 +46,51 @@ __device__ __forceinline__ void pb_bulk_load(void* dst, const void* src, uint32_
 __device__ __forceinline__ void pb_next_may_begin() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pb_wait_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+// Query tiles that see key tile t
+__device__ __forceinline__ int pb_query_tiles(const PackedPlan& plan, int t, int window) {
+  int hi = plan.tile_hi[t];
+  if (window > 0) hi = min(hi, t * PA_TILE + PA_TILE - 1 + window);
+  return hi <= 0 ? 0 : (hi - 1) / PA_TILE - t + 1;
+}
+// Into how many parts a group's heads are cut for dk and dv (a whole block): a key tile's steps are a serial chain, and the longest
+// should be no more than 3/2 of what an SM does in all (dq fills what is then left).  The documents decide, so it is found on the
+// device; the host gives the most that there is room for.  8192 rows, 32/4 heads of 128, backward in 1 and 2 parts: documents
+// around 300 rows (the longest chain is 1.4 shares) 262 and 288 us, around 2000 (1.2) 503 and 531, around 700 (1.8) 474 and 384;
+// 4096 rows of one document (2.2) 738 and 456, in 4 parts the same.
+__device__ __forceinline__ void pb_choose_parts(const int* base, int rows, int hq, int hkv, int window, int most, int sms, int* parts) {
+  __shared__ int longest, total;
+  if (threadIdx.x == 0) longest = total = 0;
+  __syncthreads();
+  const PackedPlan plan = packed_plan(base, rows);
+  int l = 0, sum = 0;
+  for (int t = threadIdx.x; t < (rows + PA_TILE - 1) / PA_TILE; t += blockDim.x) {
+    const int n = pb_query_tiles(plan, t, window);
+    l = max(l, n);
+    sum += n;
+  }
+  atomicMax(&longest, l);
+  atomicAdd(&total, sum);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const int group = hq / hkv;
+    int s = 1;
+    while (s < most && (group % s || 2l * longest * sms > 3l * total * hkv * s)) ++s;
+    *parts = s;
+  }
+}
+
 // ================================================================ delta
 // DP / 8 lanes per head, eight neighbouring rows each, all of whose loads are in flight together; heads fastest, so that a block
 // reads whole lines.  Rows behind the buffer's end, up to whole tiles, get zero.
 template <int DP>
 __global__ void __launch_bounds__(256)
 packed_delta_kernel(const __nv_bfloat16* out, const int8_t* rest, const __nv_bfloat16* dout, float* delta, int rows, int padded, int hq,
-                    int d, long do_ts, long do_hs, int* counter) {
+                    int d, long do_ts, long do_hs, int* counter, const int* plan, int hkv, int window, int splits, int sms) {
   pb_next_may_begin();
-  if (blockIdx.x == 0 && threadIdx.x < 2) counter[threadIdx.x] = 0;    // of the two kernels behind this one
+  if (blockIdx.x == 0) {                       // for the kernels behind this one
+    if (threadIdx.x < 2) counter[threadIdx.x] = 0;
+    pb_choose_parts(plan, rows, hq, hkv, window, splits, sms, counter + 2);
+  }
   constexpr int LANES = DP / 8, ROWS = 8;
   const long unit = (long)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
   const int c = (threadIdx.x % LANES) * 8;
@@ -293,7 +329,7 @@ __device__ __noinline__ void pb_redo_dq(const PackedBwdParams& p, int row, int h
   pa_put4(p.dq + ((size_t)row * p.Hq + head) * p.D, p.D, sum, p.scale);
 }
 // dk or dv of one key row for heads h0 .. h0 + heads - 1 over the queries row .. hi - 1 alone (a whole warp)
-__device__ __noinline__ void pb_redo_dkv(const PackedBwdParams& p, bool dv, int row, int hk, int h0, int heads, int part, int hi) {
+__device__ __noinline__ void pb_redo_dkv(const PackedBwdParams& p, bool dv, int row, int hk, int h0, int heads, int part, int parts, int hi) {
   const float4 k = pa_row4(p.k, row, hk, p.D), v = pa_row4(p.v, row, hk, p.D);
   float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
   bool bad = false;
@@ -308,7 +344,7 @@ __device__ __noinline__ void pb_redo_dkv(const PackedBwdParams& p, bool dv, int 
   if (bad) sum.x = sum.y = sum.z = sum.w = __int_as_float(0x7fffffff);
   const size_t at = ((size_t)row * p.Hkv + hk) * p.D;
   const float f = dv ? 1.f : p.scale;
-  if (p.splits > 1) {
+  if (parts > 1) {
     const int c = (threadIdx.x & 31) * 4;
     if (c < p.D)
       *reinterpret_cast<float4*>(p.partial + (size_t)(2 * part + (dv ? 1 : 0)) * p.rows * p.Hkv * p.D + at + c) =
@@ -628,13 +664,11 @@ struct PackedDkvItem {
   __device__ __forceinline__ explicit PackedDkvItem(const PaItem& i)
       : tile(i.v[0]), row(i.v[0] * PA_TILE), hk(i.v[1]), part(i.v[2]), h0(i.v[3]), heads(i.v[4]), tiles(i.v[5]), n(i.v[7]) {}
 };
-__device__ __forceinline__ PaItem pb_dkv_item(const PackedBwdParams& p, const PackedPlan& plan, int idx, bool sorted) {
-  const int per = p.Hkv * p.splits, o = idx / per, rest = idx - o * per, G = p.Hq / p.Hkv;
-  const int tile = sorted ? plan.k_order[o] : o, hk = rest / p.splits, part = rest - hk * p.splits;
-  const int a = part * G / p.splits, b = (part + 1) * G / p.splits;
-  int hi = plan.tile_hi[tile];
-  if (p.window > 0) hi = min(hi, tile * PA_TILE + PA_TILE - 1 + p.window);
-  const int tiles = hi <= 0 ? 0 : (hi - 1) / PA_TILE - tile + 1;
+__device__ __forceinline__ PaItem pb_dkv_item(const PackedBwdParams& p, const PackedPlan& plan, int parts, int idx, bool sorted) {
+  const int per = p.Hkv * parts, o = idx / per, rest = idx - o * per, G = p.Hq / p.Hkv;
+  const int tile = sorted ? plan.k_order[o] : o, hk = rest / parts, part = rest - hk * parts;
+  const int a = part * G / parts, b = (part + 1) * G / parts;
+  const int tiles = pb_query_tiles(plan, tile, p.window);
   return {{tile, hk, part, hk * G + a, b - a, tiles, 0, tiles * (b - a)}};
 }
 
@@ -642,7 +676,7 @@ template <int DP>
 __global__ void __launch_bounds__(PB_THREADS, 1)
 packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                   const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do,
-                  const PackedBwdParams p, const int items) {
+                  const PackedBwdParams p) {
   using L = PackedDkvSmem<DP>;
   constexpr int ST = L::ST;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -733,7 +767,9 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         ++done;
       }
     } else if (warp == 11) {
-      pa_schedule(queue, items, p.counter, [&](int idx) { return pb_dkv_item(p, plan, idx, items > (int)gridDim.x); }, abort_flag, p.status);
+      const int parts = p.counter[2], items = (p.rows + PA_TILE - 1) / PA_TILE * p.Hkv * parts;
+      pa_schedule(queue, items, p.counter, [&](int idx) { return pb_dkv_item(p, plan, parts, idx, items > (int)gridDim.x); }, abort_flag,
+                  p.status);
     } else if (warp == 8) {
       constexpr uint32_t idesc_s = make_idesc(1, 1, 0, 0, PA_TILE, PA_TILE);
       constexpr uint32_t idesc_d = make_idesc(1, 1, 0, 1, PA_TILE, DP);
@@ -868,6 +904,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     const int lg = warp & 3;
     const uint32_t base = tmem + 256 + (uint32_t(lg * 32) << 16);
     const bool wide = p.D % 16 == 0 && ((reinterpret_cast<size_t>(p.dk) | reinterpret_cast<size_t>(p.dv)) & 31) == 0;
+    const int parts = p.counter[2];
     int done = 0;
     PaReader reader;
     PaItem next;
@@ -911,7 +948,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             bad[which] += fabsf(__uint_as_float(o[e]));
           }
           if (row < p.rows) {
-            if (p.splits > 1) {
+            if (parts > 1) {
 #pragma unroll
               for (int e = 0; e < 16; e += 4)
                 if (c + e < p.D)
@@ -928,7 +965,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         for (uint32_t m = __ballot_sync(0xffffffffu, any && !pa_finite(bad[which])); m; m &= m - 1) {
           const int who = __ffs(m) - 1;
           __syncwarp();
-          pb_redo_dkv(p, which == 0, it.row + lg * 32 + who, it.hk, it.h0, it.heads, it.part, __shfl_sync(0xffffffffu, hi, who));
+          pb_redo_dkv(p, which == 0, it.row + lg * 32 + who, it.hk, it.h0, it.heads, it.part, parts, __shfl_sync(0xffffffffu, hi, who));
           pa_redone(abort_flag);
         }
       }
@@ -950,7 +987,9 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
 
 // dk, dv = the parts' sums, in the parts' order
 __global__ void __launch_bounds__(256)
-packed_join_kernel(const float* partial, __nv_bfloat16* dk, __nv_bfloat16* dv, long n, int splits) {
+packed_join_kernel(const float* partial, __nv_bfloat16* dk, __nv_bfloat16* dv, long n, const int* parts) {
+  const int splits = *parts;
+  if (splits == 1) return;                     // written by dk and dv themselves
   const long v = ((long)blockIdx.x * 256 + threadIdx.x) * 8;
   if (v >= 2 * n) return;
   float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
@@ -987,34 +1026,34 @@ static int packed_bwd_launch(const CUtensorMap& mq, const CUtensorMap& mk, const
   SLAB_CUDA_CHECK(cudaFuncSetAttribute(packed_dq_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, PackedDqSmem<DP>::TOTAL));
   SLAB_CUDA_CHECK(cudaFuncSetAttribute(packed_dkv_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, PackedDkvSmem<DP>::TOTAL));
   const int sms = sm_count();
-  SLAB_CUDA_CHECK(pb_launch(packed_dkv_kernel<DP>, dkv_items < sms ? dkv_items : sms, PackedDkvSmem<DP>::TOTAL, stream, mq, mk, mv, mdo, p,
-                            (int)dkv_items));
+  SLAB_CUDA_CHECK(pb_launch(packed_dkv_kernel<DP>, dkv_items < sms ? dkv_items : sms, PackedDkvSmem<DP>::TOTAL, stream, mq, mk, mv, mdo, p));
   SLAB_CUDA_CHECK(pb_launch(packed_dq_kernel<DP>, dq_items < sms ? dq_items : sms, PackedDqSmem<DP>::TOTAL, stream, mq, mk, mv, mdo, p,
                             (int)dq_items));
   if (p.splits > 1) {
     const long n = (long)p.rows * p.Hkv * p.D;
-    packed_join_kernel<<<(unsigned)((2 * n / 8 + 255) / 256), 256, 0, stream>>>(p.partial, p.dk, p.dv, n, p.splits);
+    packed_join_kernel<<<(unsigned)((2 * n / 8 + 255) / 256), 256, 0, stream>>>(p.partial, p.dk, p.dv, n, p.counter + 2);
   }
   return (int)cudaGetLastError();
 }
 
 }  // namespace slab
 
-// Into how many parts a group's heads are cut for dk and dv: a key tile's steps are a serial chain, and the longest, of
-// tiles * G steps, should be no more than what an SM does in all, tiles (tiles + 1) / 2 * Hq / SMs.  (8192 rows in documents of
-// 700, 32/4 heads, dk and dv in 1, 2, 4, 8 parts: 346, 275, 276, 334 us; one document, 64/8: 1755, 1789, 1884, 2171.)
-extern "C" int slab_packed_attn_splits(int rows, int hq, int hkv) {
-  if (rows <= 0 || hkv <= 0 || hq % hkv) return -10;
+// Most parts that a group's heads are cut into for dk and dv (pb_choose_parts): room for so many sums.  Twice what one document
+// needs, as the longest of several has less beside it.
+extern "C" int slab_packed_attn_splits(int rows, int hq, int hkv, int window) {
+  if (rows <= 0 || hkv <= 0 || hq % hkv || window < 0) return -10;
   const long tiles = ((long)rows + slab::PA_TILE - 1) / slab::PA_TILE;
+  const long seen = window > 0 && (window + slab::PA_TILE - 2) / slab::PA_TILE + 1 < tiles ? (window + slab::PA_TILE - 2) / slab::PA_TILE + 1 : tiles;
   const int group = hq / hkv;
-  const long want = (2l * slab::sm_count() + (tiles + 1) * hkv - 1) / ((tiles + 1) * hkv);
+  // longest chain: seen * group steps; all of them: seen (tiles - (seen - 1) / 2) * hq
+  const long all = (2 * tiles - seen + 1) * hkv, want = (8l * slab::sm_count() + 3 * all - 1) / (3 * all);
   int s = want < group ? (int)want : group;
   while (group % s) ++s;
   return s;
 }
 
 // q, k, v, dout with token and head strides as in slab_packed_attn_fwd; out, rest, dq, dk, dv contiguous; rest and lse from the forward pass,
-// delta [Hq, tiles * 128] and counter [2] int32 scratch; partial: scratch of splits * 2 * rows * Hkv * D floats where splits > 1.
+// delta [Hq, tiles * 128] and counter [3] int32 scratch; partial: scratch of splits * 2 * rows * Hkv * D floats where splits > 1.
 extern "C" int slab_packed_attn_bwd(const void* q, const void* k, const void* v, const void* out, const void* rest,
                                     const void* dout, const void* lse,
                                     const void* plan, void* dq, void* dk, void* dv, void* delta, void* counter, void* partial, int splits,
@@ -1037,10 +1076,12 @@ extern "C" int slab_packed_attn_bwd(const void* q, const void* k, const void* v,
   const long units = (long)padded / 8 * hq, per = d <= 64 ? 32 : 16;
   if (d <= 64)
     packed_delta_kernel<64><<<(unsigned)((units + per - 1) / per), 256, 0, st>>>((const __nv_bfloat16*)out, (const int8_t*)rest,
-        (const __nv_bfloat16*)dout, (float*)delta, rows, padded, hq, d, do_ts, do_hs, (int*)counter);
+        (const __nv_bfloat16*)dout, (float*)delta, rows, padded, hq, d, do_ts, do_hs, (int*)counter,
+        (const int*)plan, hkv, window, splits, sm_count());
   else
     packed_delta_kernel<128><<<(unsigned)((units + per - 1) / per), 256, 0, st>>>((const __nv_bfloat16*)out, (const int8_t*)rest,
-        (const __nv_bfloat16*)dout, (float*)delta, rows, padded, hq, d, do_ts, do_hs, (int*)counter);
+        (const __nv_bfloat16*)dout, (float*)delta, rows, padded, hq, d, do_ts, do_hs, (int*)counter,
+        (const int*)plan, hkv, window, splits, sm_count());
   PackedBwdParams p;
   p.dq = (__nv_bfloat16*)dq;
   p.dk = (__nv_bfloat16*)dk;

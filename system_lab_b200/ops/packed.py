@@ -21,7 +21,7 @@ from . import cuda
 cuda.register("slab_packed_plan", "piippp")
 cuda.register("slab_packed_plan_tokens", "piilppp")
 cuda.register("slab_packed_attn_fwd", "ppppppp" + "iiii" + "llllll" + "if" + "ppp")
-cuda.register("slab_packed_attn_splits", "iii")
+cuda.register("slab_packed_attn_splits", "iiii")
 cuda.register("slab_packed_attn_bwd", "p" * 14 + "i" + "iiii" + "llllllll" + "if" + "pp")
 cuda._KERNELS_PER_CALL.update({"slab_packed_plan": 2, "slab_packed_plan_tokens": 3, "slab_packed_attn_bwd": 3})
 cuda._STATUS_NAMES.update({40: "PACKED_ATTN_Q", 41: "PACKED_ATTN_KV_FULL", 42: "PACKED_ATTN_EMPTY", 43: "PACKED_ATTN_S",
@@ -166,20 +166,20 @@ def forward(q, k, v, documents: PackedDocuments, scale: float, window: int = 0, 
 
 def backward(q, k, v, out, rest, lse, dout, documents: PackedDocuments, scale: float, window: int = 0):
     """``(dq, dk, dv)`` from what the forward pass took and returned.  Where a group's heads are cut into parts
-    (few key tiles for the SMs), the parts' sums are kept in fp32 and added up in their order."""
+    (long documents, few key tiles for the SMs), the parts' sums are kept in fp32 and added up in their order."""
     rows, hq, d = q.shape
     hkv = k.shape[1]
     dq = torch.empty((rows, hq, d), dtype=q.dtype, device=q.device)
     dk = torch.empty((rows, hkv, d), dtype=q.dtype, device=q.device)
     dv = torch.empty_like(dk)
     stats = lse.numel() - 1
-    delta = torch.empty(stats + 2, dtype=torch.float32, device=q.device)          # and two work counters
+    delta = torch.empty(stats + 3, dtype=torch.float32, device=q.device)          # and two work counters, the number of parts
     q, qt, qh = _readable(q)
     k, kt, kh = _readable(k)
     v, vt, vh = _readable(v)
     dout, gt, gh = _readable(dout)
     with cuda.on_device(q):
-        splits = cuda.lib().slab_packed_attn_splits(rows, hq, hkv)
+        splits = cuda.lib().slab_packed_attn_splits(rows, hq, hkv, min(window, rows))
         partial = torch.empty(splits * 2 * dk.numel(), dtype=torch.float32, device=q.device) if splits > 1 else None
         cuda.call("slab_packed_attn_bwd", q, k, v, out, rest, dout, lse, documents.plan, dq, dk, dv, delta,
                   delta.data_ptr() + 4 * stats, partial, splits, rows, hq, hkv, d, qt, qh, kt, kh, vt, vh, gt, gh,

@@ -185,6 +185,21 @@ def test_short_items_behind_rows_that_are_made_again(hq, hkv, d):
         close([out[bad:]], [(want[bad:], bound[bad:], None)])
 
 
+@pytest.mark.parametrize("lens", [[128] * 8, [900, 60, 64], [1024], [1, 1000, 0, 23], [0]])
+@pytest.mark.parametrize("hq,hkv,window", [(8, 1, 0), (12, 2, 0), (16, 1, 300)])
+def test_heads_of_a_group_in_as_many_parts_as_the_documents_ask_for(hq, hkv, window, lens):
+    cu = cu_of(lens)
+    rows = max(cu[-1], 1024)
+    q, k, v, dout = make(rows, hq, hkv, 64)
+    docs = ops.pack_documents(torch.tensor(cu, dtype=torch.int32, device=DEV), rows)
+    assert cuda.lib().slab_packed_attn_splits(rows, hq, hkv, window) > 1
+    got = run(q, k, v, docs, dout, window=window)
+    if cu[-1]:
+        close(got, reference(q, k, v, cu, 1 / 8, window, dout))
+    for x in got:
+        assert not x[cu[-1]:].any()
+
+
 def test_rows_made_again_for_longer_than_a_wait_lasts():
     """Key tiles of the long document take seconds each: every sum of dv meets an infinity in the last row."""
     lens = [6000] + [100] * 140
