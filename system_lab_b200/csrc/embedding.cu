@@ -102,6 +102,7 @@ __device__ __forceinline__ int em_bin(long long id, int v0) {
 __global__ void __launch_bounds__(EM_WARPS * 32)
 embedding_sort_kernel(const long long* __restrict__ tokens, int n, int vocab, int slice, int* __restrict__ order, int* valid,
                       uint32_t* __restrict__ named, int keep) {
+  next_may_begin();
   extern __shared__ int hist[];              // [warps][slice], [slice] totals, and with `keep` the tokens for the second pass
   __shared__ int below_s, warp_sums[EM_WARPS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -242,6 +243,8 @@ __device__ __forceinline__ void em_fill(const uint32_t* named, TW* dw, int vocab
 template <typename TW, typename TO, int VEC>
 __global__ void __launch_bounds__(256)
 embedding_sum_kernel(const EmSum p, const TO* __restrict__ dout, TW* __restrict__ dw) {
+  next_may_begin();
+  wait_before();                             // the sorted positions
   if ((int)blockIdx.x >= p.sum_blocks) {
     if (blockIdx.y == 0) em_fill(p.named, dw, p.vocab, p.h, blockIdx.x - p.sum_blocks, gridDim.x - p.sum_blocks);
     return;
@@ -304,6 +307,7 @@ embedding_sum_kernel(const EmSum p, const TO* __restrict__ dout, TW* __restrict_
 template <typename TW, int VEC>
 __global__ void __launch_bounds__(256)
 embedding_join_kernel(const EmSum p, TW* __restrict__ dw) {
+  wait_before();                             // the pieces
   const int chunk = blockIdx.x * blockDim.y + threadIdx.y;
   const int c = (blockIdx.y * blockDim.x + threadIdx.x) * VEC;
   const int valid = *p.valid, chunks = (valid + p.chunk - 1) / p.chunk;
@@ -400,8 +404,9 @@ static int em_bwd(const void* tokens, const void* dout, void* dw, int* order, fl
   p.sum_blocks = (int)grid.x;
   const int fill_blocks = accumulate ? 0 : (vocab + 7) / 8 < 8 * sms ? (vocab + 7) / 8 : 8 * sms;
   p.ends = reinterpret_cast<int2*>(pieces + (size_t)chunks * 2 * h);
-  embedding_sum_kernel<TW, TO, VEC><<<dim3(grid.x + fill_blocks, grid.y), block, block.y * (p.chunk + 2) * sizeof(int2), st>>>(p, (const TO*)dout, (TW*)dw);
-  if (chunks > 1) embedding_join_kernel<TW, VEC><<<grid, block, 0, st>>>(p, (TW*)dw);
+  SLAB_CUDA_CHECK(launch_early(embedding_sum_kernel<TW, TO, VEC>, dim3(grid.x + fill_blocks, grid.y), block,
+                               block.y * (p.chunk + 2) * sizeof(int2), st, p, (const TO*)dout, (TW*)dw));
+  if (chunks > 1) SLAB_CUDA_CHECK(launch_early(embedding_join_kernel<TW, VEC>, grid, block, 0, st, p, (TW*)dw));
   return (int)cudaGetLastError();
 }
 

@@ -8,13 +8,18 @@
 // tile.  Rows of no document get zeros.
 //
 // Roles (512 threads, one persistent block per SM): warps 0-3 and 4-7 softmax, one query tile of 128 rows each, a row per
-// thread; warp 8 issues the MMAs, warp 9 the copies, warp 11 takes items; warps 12-15 store finished rows.  The two query tiles share the key and value tiles: two heads of one
-// group on the same rows where the group is even (nothing is masked for one tile only), else the next 128 rows.
+// thread; warp 8 issues the MMAs, warp 9 the copies, warp 11 takes items; warps 12-15 store finished rows.  The two query tiles
+// share the key and value tiles: two heads of one group on the same rows where the group is even (nothing is masked for one
+// tile only), else the next 128 rows.
 // S and O live in tensor memory (2 x 128 + 2 x DP columns).  The probabilities go back over the scores they came from, as
 // bf16, and are the A operand of P V from there.  While one tile's softmax runs, the tensor cores do P V of the other
 // and its next scores.  O is brought to a new maximum only when a row's maximum has grown by 2^8: until then its
 // probabilities are at most 2^8 too large, and so is their sum.  Statistics and sums are fp32; probabilities are rounded
 // to bf16 once, as the operand of P V.
+//
+// Long documents are bound by the tensor cores and the exponentials side by side (8192 rows of one document, 64/8 heads of 128: 848
+// us, 1.30 PFLOP/s, 0.79 of cuBLAS in a burst), short ones by their masked tiles and an item's start and end, some 5 thousand
+// cycles (8192 rows in documents around 700, 32/4 heads: 115 us; 16384 rows, window 128, 64/8 heads of 64: 162 us).
 #include "packed_attention.cuh"
 
 namespace slab {

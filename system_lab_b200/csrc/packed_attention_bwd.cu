@@ -3,14 +3,19 @@
 //   p_ij = exp2(scale_log2 q_i.k_j - lse_i)     delta_i = do_i.o_i      ds_ij = p_ij (do_i.v_j - delta_i)
 //   dv_j = sum_i p_ij do_i      dk_j = scale sum_i ds_ij q_i      dq_i = scale sum_j ds_ij k_j
 //
-// delta is made from the output with its lower half (packed_attention.cuh).  Two kernels behind the one for delta: one per query tile for dq, one per key tile for dk and dv.  Each makes the
-// scores and their gradient again (7 products of 128 x 128 x D a tile pair where one kernel could do with 5), but no sum
-// leaves the tensor cores before it is whole: no atomics, no fp32 copy of dq, and the same bits every time.
+// delta is made from the output with its lower half (packed_attention.cuh).  Two kernels behind the one for delta: one per query
+// tile for dq, one per key tile for dk and dv.  Each makes the scores and their gradient again (7 products of 128 x 128 x D a
+// tile pair where one kernel could do with 5), but no sum leaves the tensor cores before it is whole: no atomics, no fp32
+// copy of dq, and the same bits every time.
 //
 // Roles as in the forward pass (512 threads): warps 0-3 and 4-7 take the left and the right 64 columns of every 128 x 128
-// tile, a row per thread; warp 8 issues the MMAs, warp 9 the copies, warp 11 takes items; warps 12-15 store what is finished.  p and ds go back over the scores and products they
-// came from, as bf16, and are the A operand of the next product from tensor memory.  Statistics, p - delta and all sums
-// are fp32; p and ds are rounded to bf16 once, as operands.
+// tile, a row per thread; warp 8 issues the MMAs, warp 9 the copies, warp 11 takes items; warps 12-15 store what is finished.  p
+// and ds go back over the scores and products they came from, as bf16, and are the A operand of the next product from tensor
+// memory.  Statistics, p - delta and all sums are fp32; p and ds are rounded to bf16 once, as operands.
+//
+// Bound by the chain of one tile pair: scores, p, dP, ds, product, with two hand-overs of 250 to 350 cycles beside what the
+// tensor cores (half busy) and the exponentials take.  One document of 8192 rows, 64/8 heads of 128: dk and dv 1.69 ms, dq 1.30
+// (1.3 PFLOP/s of the seven products, 0.79 of cuBLAS in a burst); 8192 rows in documents around 700, 32/4 heads: 382 us in all.
 #include "packed_attention.cuh"
 
 namespace slab {
@@ -39,12 +44,9 @@ __device__ __forceinline__ void pb_bulk_load(void* dst, const void* src, uint32_
                : "memory");
 }
 
-// The three kernels follow one another closely: each lets the next begin once its own blocks all have (griddepcontrol), and waits for
-// the one before where it needs it.  dk and dv wait behind their set-up.  dq needs delta only, which is whole once dk and dv
+// The three kernels follow one another closely (launch_early).  dk and dv wait behind their set-up.  dq needs delta only, which is whole once dk and dv
 // have begun, so its blocks take over SMs as those of dk and dv end; they wait for the last of them before they end
 // themselves, so that what comes behind dq finds dk and dv whole.
-__device__ __forceinline__ void pb_next_may_begin() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void pb_wait_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // Query tiles that see key tile t
 __device__ __forceinline__ int pb_query_tiles(const PackedPlan& plan, int t, int window) {
@@ -86,7 +88,7 @@ template <int DP>
 __global__ void __launch_bounds__(256)
 packed_delta_kernel(const __nv_bfloat16* out, const int8_t* rest, const __nv_bfloat16* dout, float* delta, int rows, int padded, int hq,
                     int d, long do_ts, long do_hs, int* counter, const int* plan, int hkv, int window, int splits, int sms) {
-  pb_next_may_begin();
+  next_may_begin();
   if (blockIdx.x == 0) {                       // for the kernels behind this one
     if (threadIdx.x < 2) counter[threadIdx.x] = 0;
     pb_choose_parts(plan, rows, hq, hkv, window, splits, sms, counter + 2);
@@ -644,7 +646,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
-  if (threadIdx.x == 0) pb_wait_before();      // dk and dv
+  if (threadIdx.x == 0) wait_before();      // dk and dv
 }
 
 // ================================================================ dk, dv
@@ -727,8 +729,8 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
-  pb_wait_before();                            // delta, and the counters
-  pb_next_may_begin();
+  wait_before();                            // delta, and the counters
+  next_may_begin();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -1003,20 +1005,6 @@ packed_join_kernel(const float* partial, __nv_bfloat16* dk, __nv_bfloat16* dv, l
   *reinterpret_cast<bf16x8*>(to) = pack8(sum);
 }
 
-template <typename... P, typename... A>
-static cudaError_t pb_launch(void (*kernel)(P...), long blocks, int smem, cudaStream_t stream, A... args) {
-  cudaLaunchAttribute early;
-  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  early.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t config = {};
-  config.gridDim = dim3((unsigned)blocks);
-  config.blockDim = dim3(PB_THREADS);
-  config.dynamicSmemBytes = smem;
-  config.stream = stream;
-  config.attrs = &early;
-  config.numAttrs = 1;
-  return cudaLaunchKernelEx(&config, kernel, args...);
-}
 template <int DP>
 static int packed_bwd_launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mdo,
                              const PackedBwdParams& p, cudaStream_t stream) {
@@ -1026,9 +1014,10 @@ static int packed_bwd_launch(const CUtensorMap& mq, const CUtensorMap& mk, const
   SLAB_CUDA_CHECK(cudaFuncSetAttribute(packed_dq_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, PackedDqSmem<DP>::TOTAL));
   SLAB_CUDA_CHECK(cudaFuncSetAttribute(packed_dkv_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, PackedDkvSmem<DP>::TOTAL));
   const int sms = sm_count();
-  SLAB_CUDA_CHECK(pb_launch(packed_dkv_kernel<DP>, dkv_items < sms ? dkv_items : sms, PackedDkvSmem<DP>::TOTAL, stream, mq, mk, mv, mdo, p));
-  SLAB_CUDA_CHECK(pb_launch(packed_dq_kernel<DP>, dq_items < sms ? dq_items : sms, PackedDqSmem<DP>::TOTAL, stream, mq, mk, mv, mdo, p,
-                            (int)dq_items));
+  SLAB_CUDA_CHECK(launch_early(packed_dkv_kernel<DP>, dim3((unsigned)(dkv_items < sms ? dkv_items : sms)), dim3(PB_THREADS),
+                               PackedDkvSmem<DP>::TOTAL, stream, mq, mk, mv, mdo, p));
+  SLAB_CUDA_CHECK(launch_early(packed_dq_kernel<DP>, dim3((unsigned)(dq_items < sms ? dq_items : sms)), dim3(PB_THREADS),
+                               PackedDqSmem<DP>::TOTAL, stream, mq, mk, mv, mdo, p, (int)dq_items));
   if (p.splits > 1) {
     const long n = (long)p.rows * p.Hkv * p.D;
     packed_join_kernel<<<(unsigned)((2 * n / 8 + 255) / 256), 256, 0, stream>>>(p.partial, p.dk, p.dv, n, p.counter + 2);
