@@ -60,11 +60,13 @@ __device__ __forceinline__ int pb_query_tiles(const PackedPlan& plan, int t, int
 // around 300 rows (the longest chain is 1.4 shares) 262 and 288 us, around 2000 (1.2) 503 and 531, around 700 (1.8) 474 and 384;
 // 4096 rows of one document (2.2) 738 and 456, in 4 parts the same.
 __device__ __forceinline__ void pb_choose_parts(const int* base, int rows, int hq, int hkv, int window, int most, int sms, int* parts) {
-  __shared__ int longest, total;
-  if (threadIdx.x == 0) longest = total = 0;
+  __shared__ int longest;
+  __shared__ unsigned long long total;
+  if (threadIdx.x == 0) { longest = 0; total = 0; }
   __syncthreads();
   const PackedPlan plan = packed_plan(base, rows);
-  int l = 0, sum = 0;
+  int l = 0;
+  unsigned long long sum = 0;
   for (int t = threadIdx.x; t < (rows + PA_TILE - 1) / PA_TILE; t += blockDim.x) {
     const int n = pb_query_tiles(plan, t, window);
     l = max(l, n);
@@ -76,7 +78,7 @@ __device__ __forceinline__ void pb_choose_parts(const int* base, int rows, int h
   if (threadIdx.x == 0) {
     const int group = hq / hkv;
     int s = 1;
-    while (s < most && (group % s || 2l * longest * sms > 3l * total * hkv * s)) ++s;
+    while (s < most && (group % s || 2l * longest * sms > 3l * (long)total * hkv * s)) ++s;
     *parts = s;
   }
 }

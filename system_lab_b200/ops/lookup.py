@@ -28,6 +28,8 @@ def check(tokens, weight, scale) -> float:
         raise ValueError(f"a table [vocabulary, hidden] wanted, got {tuple(weight.shape)}")
     if tokens.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"token ids have to be int32 or int64, not {tokens.dtype}")
+    if tokens.numel() > 2 ** 30:                       # (positions are counted in 32 bits, in whole groups)
+        raise ValueError(f"{tokens.numel()} tokens: at most 2^30 in one call")
     if tokens.device != weight.device:
         raise ValueError(f"tokens on {tokens.device}, table on {weight.device}")
     return float(scale)
@@ -43,8 +45,6 @@ class _Embedding(torch.autograd.Function):
         tok = tokens.long().contiguous()
         w = weight.contiguous()
         v, h = w.shape
-        if tok.numel() > 2 ** 30:                  # (positions are counted in 32 bits, in whole groups)
-            raise ValueError(f"{tok.numel()} tokens: at most 2^30 in one call")
         out = torch.empty(*tokens.shape, h, dtype=dtype, device=w.device)
         if tok.numel():
             with cuda.on_device(w):

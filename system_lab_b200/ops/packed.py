@@ -28,6 +28,7 @@ cuda._STATUS_NAMES.update({40: "PACKED_ATTN_Q", 41: "PACKED_ATTN_KV_FULL", 42: "
                            44: "PACKED_ATTN_P", 45: "PACKED_ATTN_OUT", 46: "PACKED_ATTN_ITEM"})
 
 TILE = 128
+MAX_ROWS = 2 ** 30 - 256                            # a row and a window together stay below 2^31
 
 
 class PackedDocuments:
@@ -58,8 +59,8 @@ def pack_documents(cu_seqlens: torch.Tensor, rows: int) -> PackedDocuments:
     bad ones set the status word (``cuda.check_status``) and never lead a kernel out of the buffer."""
     if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1 or cu_seqlens.dtype not in (torch.int32, torch.int64):
         raise ValueError("cu_seqlens has to be a one-dimensional int32 or int64 tensor of document offsets")
-    if not 0 < rows < 2 ** 31 - 256:
-        raise ValueError(f"{rows} rows")
+    if not 0 < rows <= MAX_ROWS:
+        raise ValueError(f"{rows} rows: has to be 1 to {MAX_ROWS}")
     if not cu_seqlens.is_cuda:
         cu = cu_seqlens.long()
         if int(cu[0]) != 0 or int(cu[-1]) > rows or bool((cu[1:] < cu[:-1]).any()):
@@ -87,8 +88,8 @@ def documents_from_tokens(tokens: torch.Tensor, end_token: int) -> PackedDocumen
         raise ValueError("tokens has to be a non-empty [B, S] int64 tensor")
     b, s = tokens.shape
     rows = b * s
-    if rows >= 2 ** 31 - 256:
-        raise ValueError(f"{rows} rows")
+    if rows > MAX_ROWS:
+        raise ValueError(f"{rows} rows: at most {MAX_ROWS}")
     tok = tokens.contiguous()
     if not tok.is_cuda:
         i = torch.arange(rows)

@@ -74,3 +74,8 @@ def test_refusals():
                    (torch.zeros(2, dtype=torch.int64), torch.randn(0, 4)), (torch.zeros(2, dtype=torch.bool), torch.randn(3, 4))):
         with pytest.raises(ValueError):
             ops.embedding(tok, w)
+
+
+def test_more_tokens_than_the_kernels_count_are_refused():
+    with pytest.raises(ValueError, match="tokens"):
+        ops.embedding(torch.zeros(1, dtype=torch.int64).expand(2 ** 30 + 1), torch.zeros(4, 8))

@@ -85,3 +85,10 @@ def test_refusals():
         args.update(kw)
         with pytest.raises(ValueError):
             ops.packed_attention(**args)
+
+
+def test_more_rows_than_the_kernels_count_are_refused():
+    with pytest.raises(ValueError, match="rows"):
+        ops.pack_documents(torch.tensor([0, 4]), 2 ** 30)
+    with pytest.raises(ValueError, match="rows"):
+        ops.documents_from_tokens(torch.zeros(1, 1, dtype=torch.int64).expand(2 ** 15, 2 ** 15), 0)
