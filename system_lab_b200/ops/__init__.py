@@ -10,6 +10,8 @@ from __future__ import annotations
 
 import torch
 
+from . import drop, lookup
+from . import packed as pa
 from . import reference as ref
 
 _MODE = "auto"          # auto: kernels on CUDA tensors | reference: oracle everywhere
@@ -158,7 +160,6 @@ def embedding(tokens, weight, scale=1.0, dtype=None):
     """``scale * weight[tokens]`` in ``dtype`` (the table's own by default), differentiable in ``weight [V, H]``.  On the
     GPU the gradient is summed in fp32 by sorted tokens, in the order of the positions; ids outside the table look up zeros,
     get no gradient and set the status word (``BAD_INDEX``)."""
-    from . import lookup
     scale = lookup.check(tokens, weight, scale)
     dtype = weight.dtype if dtype is None else dtype
     if use_kernels(weight) and lookup.supports(weight, dtype):
@@ -171,7 +172,6 @@ def dropout(x, p, seed, offset=0, residual=None):
     the same call gives the same mask, on the CPU too; another seed or offset gives another.  ``p`` is taken to the next
     multiple of 2^-16, and kept elements are scaled for that one.  ``seed`` is an integer or an int64 tensor of one element
     (read when the kernel runs)."""
-    from . import drop
     drop.check(x, p, seed, offset, residual)
     if use_kernels(x):
         return drop.dropout(x, p, seed, offset, residual)
@@ -181,14 +181,12 @@ def dropout(x, p, seed, offset=0, residual=None):
 def pack_documents(cu_seqlens, rows):
     """Plan of a buffer of ``rows`` rows that holds document ``s`` at rows ``cu_seqlens[s] .. cu_seqlens[s + 1] - 1``, for
     :func:`packed_attention`: made once per batch, used by every layer's forward and backward pass."""
-    from . import packed as pa
     return pa.pack_documents(cu_seqlens, rows)
 
 
 def documents_from_tokens(tokens, end_token):
     """The same plan for token rows ``[B, S]`` seen as one buffer of ``B * S`` rows: a document ends behind every
     ``end_token`` and with every row."""
-    from . import packed as pa
     return pa.documents_from_tokens(tokens, end_token)
 
 
@@ -197,7 +195,6 @@ def packed_attention(q, k, v, documents, scale=None, window=0):
     with any strides -> ``[rows, heads, d]``.  ``window > 0`` restricts a row to the last ``window`` keys.  Rows of no
     document give zeros (and get zero gradients); nothing that one document holds reaches another.  The kernels take bf16
     and ``d`` a multiple of 8 up to 128; other types and widths run on the oracle."""
-    from . import packed as pa
     scale = pa.check(q, k, v, documents, scale, window)
     if use_kernels(q) and pa.supports(q, k, v):
         return pa.attention(q, k, v, documents, scale, int(window))

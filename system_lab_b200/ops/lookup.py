@@ -45,7 +45,7 @@ class _Embedding(torch.autograd.Function):
         tok = tokens.long().contiguous()
         w = weight.contiguous()
         v, h = w.shape
-        out = torch.empty(*tokens.shape, h, dtype=dtype, device=w.device)
+        out = w.new_empty((*tokens.shape, h), dtype=dtype)
         if tok.numel():
             with cuda.on_device(w):
                 cuda.call("slab_embedding_fwd", tok, w, int(w.dtype == torch.bfloat16), out, int(dtype == torch.bfloat16),
@@ -65,7 +65,7 @@ class _Embedding(torch.autograd.Function):
         mg = getattr(ctx.w_ref, "main_grad", None)
         into = mg if mg is not None and mg.dtype in _TYPES and mg.is_contiguous() else None
         accumulate = into is not None and ctx.w_ref.main_grad_written
-        dw = into if into is not None else torch.empty(v, h, dtype=dtype, device=g.device)
+        dw = into if into is not None else g.new_empty((v, h), dtype=dtype)
         if rows == 0:
             if not accumulate:
                 dw.zero_()
@@ -74,7 +74,7 @@ class _Embedding(torch.autograd.Function):
             with cuda.on_device(g):
                 chunk = _chunk(rows)
                 at = (rows + 1 + (v + 31) // 32 + 3) // 4 * 4      # the sorted positions, their number, which rows; then the pieces
-                scratch = torch.empty(at + (rows + chunk - 1) // chunk * (2 * h + 2), dtype=torch.int32, device=g.device)
+                scratch = g.new_empty(at + (rows + chunk - 1) // chunk * (2 * h + 2), dtype=torch.int32)
                 base = scratch.data_ptr()
                 cuda.call("slab_embedding_bwd", tok, g, int(g.dtype == torch.bfloat16), dw, int(dw.dtype == torch.bfloat16),
                           base, base + 4 * at, rows, chunk, v, h, ctx.scale, int(accumulate), cuda.stream())

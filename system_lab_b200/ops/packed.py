@@ -152,10 +152,10 @@ def forward(q, k, v, documents: PackedDocuments, scale: float, window: int = 0, 
     gradients to come), ``lse`` the base-2 log-sum-exp of the scaled scores, ``[Hq, tiles * 128]`` flat, with the kernel's
     work counter behind it."""
     rows, hq, d = q.shape
-    out = torch.empty((rows, hq, d), dtype=q.dtype, device=q.device)
+    out = q.new_empty((rows, hq, d))
     stats = hq * ((rows + TILE - 1) // TILE * TILE)
-    lse = torch.empty(stats + 1, dtype=torch.float32, device=q.device)
-    rest = torch.empty((rows, hq, d), dtype=torch.int8, device=q.device) if grads else None
+    lse = q.new_empty(stats + 1, dtype=torch.float32)
+    rest = q.new_empty((rows, hq, d), dtype=torch.int8) if grads else None
     q, qt, qh = _readable(q)
     k, kt, kh = _readable(k)
     v, vt, vh = _readable(v)
@@ -170,18 +170,18 @@ def backward(q, k, v, out, rest, lse, dout, documents: PackedDocuments, scale: f
     (long documents, few key tiles for the SMs), the parts' sums are kept in fp32 and added up in their order."""
     rows, hq, d = q.shape
     hkv = k.shape[1]
-    dq = torch.empty((rows, hq, d), dtype=q.dtype, device=q.device)
-    dk = torch.empty((rows, hkv, d), dtype=q.dtype, device=q.device)
+    dq = q.new_empty((rows, hq, d))
+    dk = q.new_empty((rows, hkv, d))
     dv = torch.empty_like(dk)
     stats = lse.numel() - 1
-    delta = torch.empty(stats + 3, dtype=torch.float32, device=q.device)          # and two work counters, the number of parts
+    delta = q.new_empty(stats + 3, dtype=torch.float32)         # and two work counters, the number of parts
     q, qt, qh = _readable(q)
     k, kt, kh = _readable(k)
     v, vt, vh = _readable(v)
     dout, gt, gh = _readable(dout)
     with cuda.on_device(q):
         splits = cuda.lib().slab_packed_attn_splits(rows, hq, hkv, min(window, rows))
-        partial = torch.empty(splits * 2 * dk.numel(), dtype=torch.float32, device=q.device) if splits > 1 else None
+        partial = q.new_empty(splits * 2 * dk.numel(), dtype=torch.float32) if splits > 1 else None
         cuda.call("slab_packed_attn_bwd", q, k, v, out, rest, dout, lse, documents.plan, dq, dk, dv, delta,
                   delta.data_ptr() + 4 * stats, partial, splits, rows, hq, hkv, d, qt, qh, kt, kh, vt, vh, gt, gh,
                   min(window, rows), scale, cuda.status_word(q.device), cuda.stream())
