@@ -265,3 +265,29 @@ def test_seed_changed_between_forward_and_backward():
     seed.fill_(4)
     (dx,) = torch.autograd.grad(y, x, torch.ones_like(x))
     assert torch.equal(dx != 0, y != 0)
+
+
+def test_elements_past_32_bits():
+    """A table and a dropped tensor of more than 2^31 elements: their last rows."""
+    v, h = 2 ** 20 + 3, 2056
+    w = torch.empty(v, h, dtype=torch.bfloat16, device=DEV)
+    w[-2:] = torch.randn(2, h, device=DEV).bfloat16()
+    w.requires_grad_(True)
+    tokens = torch.tensor([v - 1, v - 2, v - 1], device=DEV)
+    out = ops.embedding(tokens, w, 2.0)
+    assert torch.equal(out, (w.detach()[tokens].float() * 2).bfloat16())
+    dout = torch.randn(3, h, device=DEV).bfloat16()
+    grad = torch.autograd.grad(out, w, dout)[0]
+    assert torch.equal(grad[-2], (dout[1].float() * 2).bfloat16())
+    assert torch.equal(grad[-1], ((dout[0].float() + dout[2].float()) * 2).bfloat16())
+    assert not grad[:-2].any()
+    del grad, out
+    x = w.detach().flatten()
+    x.fill_(1.0)
+    y = ops.dropout(x, 0.25, 3)
+    last = y[-2 ** 20 - 5:]
+    kept = last != 0
+    assert torch.equal(last[kept], torch.full_like(last[kept], 4 / 3))
+    assert abs(kept.float().mean().item() - 0.75) < 6 * (0.25 * 0.75 / 2 ** 20) ** 0.5
+    del x, y, w
+    torch.cuda.empty_cache()

@@ -392,3 +392,17 @@ def test_one_document_is_causal_attention():
     got = ops.packed_attention(q, k, v, docs)
     want = ops.causal_attention(*(x.unflatten(0, (b, s)) for x in (q, k, v))).flatten(0, 1)
     assert (got.float() - want.float()).abs().max().item() <= 2 * EPS * want.float().abs().max().item()
+
+
+def test_elements_past_32_bits():
+    """More than 2^31 elements of q, out and their gradients; the last documents against the reference."""
+    rows, hq, hkv, d = 2 ** 18 + 77, 64, 1, 128
+    cu = [*range(0, rows, 100), rows]
+    q, k, v, dout = make(rows, hq, hkv, d)
+    docs = ops.pack_documents(torch.tensor(cu, dtype=torch.int32, device=DEV), rows)
+    got = run(q, k, v, docs, dout)
+    at = cu[-3]
+    want = reference(*(t[at:] for t in (q, k, v)), [c - at for c in cu[-3:]], 1 / math.sqrt(d), 0, dout[at:])
+    close([x[at:] for x in got], want)
+    del got, q, k, v, dout
+    torch.cuda.empty_cache()
