@@ -21,6 +21,7 @@
 namespace slab {
 
 constexpr int PB_THREADS = 512;
+constexpr long PB_LONGEST = 1l << 18;        // steps of an item, whose end others wait for: half a second of the two that a wait may last
 constexpr int PB_EVERY = 8;                  // of that many pairs of exponentials, one is made on the multiply-add units
 
 struct PackedBwdParams {
@@ -78,7 +79,7 @@ __device__ __forceinline__ void pb_choose_parts(const int* base, int rows, int h
   if (threadIdx.x == 0) {
     const int group = hq / hkv;
     int s = 1;
-    while (s < most && (group % s || 2l * longest * sms > 3l * (long)total * hkv * s)) ++s;
+    while (s < most && (group % s || 2l * longest * sms > 3l * (long)total * hkv * s || (long)longest * group > PB_LONGEST * s)) ++s;
     *parts = s;
   }
 }
@@ -1037,7 +1038,9 @@ extern "C" int slab_packed_attn_splits(int rows, int hq, int hkv, int window) {
   const long seen = window > 0 && (window + slab::PA_TILE - 2) / slab::PA_TILE + 1 < tiles ? (window + slab::PA_TILE - 2) / slab::PA_TILE + 1 : tiles;
   const int group = hq / hkv;
   // longest chain: seen * group steps; all of them: seen (tiles - (seen - 1) / 2) * hq
-  const long all = (2 * tiles - seen + 1) * hkv, want = (8l * slab::sm_count() + 3 * all - 1) / (3 * all);
+  const long all = (2 * tiles - seen + 1) * hkv, bound = (seen * group + slab::PB_LONGEST - 1) / slab::PB_LONGEST;
+  long want = (8l * slab::sm_count() + 3 * all - 1) / (3 * all);
+  want = want > bound ? want : bound;
   int s = want < group ? (int)want : group;
   while (group % s) ++s;
   return s;

@@ -180,7 +180,7 @@ def dropout(x, p, seed, offset=0, residual=None):
 
 def pack_documents(cu_seqlens, rows):
     """Plan of a buffer of ``rows`` rows that holds document ``s`` at rows ``cu_seqlens[s] .. cu_seqlens[s + 1] - 1``, for
-    :func:`packed_attention`: made once per batch, used by every layer's forward and backward pass."""
+    :func:`packed_attention`: made once per batch, used by every layer's forward and backward pass.  At most 2^25 rows."""
     return pa.pack_documents(cu_seqlens, rows)
 
 

@@ -28,7 +28,7 @@ cuda._STATUS_NAMES.update({40: "PACKED_ATTN_Q", 41: "PACKED_ATTN_KV_FULL", 42: "
                            44: "PACKED_ATTN_P", 45: "PACKED_ATTN_OUT", 46: "PACKED_ATTN_ITEM"})
 
 TILE = 128
-MAX_ROWS = 2 ** 30 - 256                            # a row and a window together stay below 2^31
+MAX_ROWS = 2 ** 25                                  # a row's key tiles are one item, whose end is waited for: half a second of them
 
 
 class PackedDocuments:

@@ -200,6 +200,16 @@ def test_heads_of_a_group_in_as_many_parts_as_the_documents_ask_for(hq, hkv, win
         assert not x[cu[-1]:].any()
 
 
+@pytest.mark.parametrize("rows,hq,hkv,window,least", [(2 ** 21, 64, 1, 0, 4), (2 ** 25, 8, 1, 0, 8), (2 ** 22, 128, 2, 0, 8),
+                                                       (2 ** 25, 64, 1, 1024, 1)])
+def test_no_item_is_longer_than_a_wait(rows, hq, hkv, window, least):
+    """Steps of the longest item of dk and dv: query tiles times heads of a part, 2^18 at most."""
+    parts = cuda.lib().slab_packed_attn_splits(rows, hq, hkv, window)
+    assert parts >= least and (hq // hkv) % parts == 0
+    tiles = min(rows, window + 127 if window else rows) // 128 + 1
+    assert tiles * (hq // hkv // parts) <= 2 ** 18 + hq
+
+
 def test_rows_made_again_for_longer_than_a_wait_lasts():
     """Key tiles of the long document take seconds each: every sum of dv meets an infinity in the last row."""
     lens = [6000] + [100] * 140
