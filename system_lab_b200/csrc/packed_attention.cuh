@@ -317,22 +317,32 @@ __device__ __forceinline__ float pa_max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
+// The larger of two; NaN if either is
+__device__ __forceinline__ float pa_max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
 // 2^x for two numbers on the multiply-add units: x = n + f with n whole (adding 1.5 * 2^23 rounds it into the mantissa's low
 // bits) and |f| <= 1/2; a cubic in f, fitted to 2^f for the least largest relative error (7.5e-5; probabilities are then
-// rounded to bf16, 3.9e-3); n goes into the exponent.  Below -126 the result is 2^-126: only for
-// keys that are seen, never for masked ones, whose probability has to be zero.
+// rounded to bf16, 3.9e-3); n goes into the exponent.  x below -126 (-inf among it) is taken as -126, and would then weigh 2^-126,
+// which is not nothing where a value is large; NaN (an infinity less itself among it) would leave the exponent's sum as a finite
+// number.  Both are put right by adding x k at the end: k = 66567 * 2^-149 is 2^-126 (as the cubic has it, 8387401 * 2^-149) / 126
+// rounded up, so what was cut off ends at -41 * 2^-149, which bf16 rounds to zero and no sum sees, other results change by less
+// than 2^-126, and NaN stays NaN.
 __device__ __forceinline__ float2 pa_exp2_fma(float2 x) {
-  const float2 magic = make_float2(12582912.f, 12582912.f);
-  x.x = fmaxf(x.x, -126.f);
-  x.y = fmaxf(x.y, -126.f);
+  const float2 magic = make_float2(12582912.f, 12582912.f), k = make_float2(__uint_as_float(66567u), __uint_as_float(66567u));
+  x.x = pa_max_nan(x.x, -126.f);
+  x.y = pa_max_nan(x.y, -126.f);
   const float2 t = pa_add2(x, magic);
   const float2 n = pa_add2(t, make_float2(-12582912.f, -12582912.f));
   const float2 f = pa_fma2(n, make_float2(-1.f, -1.f), x);
   float2 p = pa_fma2(f, make_float2(0.05517167f, 0.05517167f), make_float2(0.24261113f, 0.24261113f));
   p = pa_fma2(p, f, make_float2(0.69326097f, 0.69326097f));
   p = pa_fma2(p, f, make_float2(0.99992806f, 0.99992806f));
-  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
-                     __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
+  p = make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
+                  __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
+  return pa_fma2(x, k, p);
 }
 
 // Tile of 128 rows x DP columns of one head, as boxes of 64 columns ([128 rows][128 bytes], 128-byte swizzle).  Columns at
