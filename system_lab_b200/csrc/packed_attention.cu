@@ -226,8 +226,8 @@ __device__ __noinline__ void pf_redo(const PackedFwdParams& p, int row, int head
   for (int j = lo; j <= row; ++j) {
     const float s = pa_dot4(q, pa_row4(p.k, j, hk, p.D)) * p.scale_log2;
     if (pa_nan(s)) { l = s; break; }                                   // and so is the whole row
-    if (s == -INFINITY) continue;
-    const float top = fmaxf(m, s), alpha = m == -INFINITY ? 0.f : pa_exp2(m - top), e = pa_exp2(s - top);
+    // (a score of -inf weighs zero; what is no number beside it makes the sum none either)
+    const float top = fmaxf(m, s), alpha = m == -INFINITY ? 1.f : pa_exp2(m - top), e = s == -INFINITY ? 0.f : pa_exp2(s - top);
     l = fmaf(l, alpha, e);
     o = make_float4(o.x * alpha, o.y * alpha, o.z * alpha, o.w * alpha);
     pa_add4(o, e, pa_row4(p.v, j, hk, p.D));

@@ -98,9 +98,9 @@ def test_scores_that_are_all_minus_infinity(hq, hkv, d):
 
 @pytest.mark.parametrize("hq,hkv,d", [(4, 2, 64), (3, 3, 128)])
 @pytest.mark.parametrize("value", [math.nan, math.inf])
-@pytest.mark.parametrize("low", [-2.0 ** 16])
+@pytest.mark.parametrize("low", [-2.0 ** 16, -math.inf])
 def test_a_value_without_weight(low, value, hq, hkv, d):
-    """Zero times what is no number is no number."""
+    """Zero times what is no number is no number, whether the zero is an exponential's or that of a score of -inf."""
     q, k, v, dout = make(hq, hkv, d)
     q[:, :, 3] = q[:, :, 3].abs() + 0.25
     k[14, :, 3] = low
