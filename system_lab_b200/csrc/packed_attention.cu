@@ -217,7 +217,8 @@ __device__ __forceinline__ PaItem pf_item(const PackedFwdParams& p, const Packed
   return {{row0, row1, head0, head1, head0 / (p.Hq / p.Hkv), j0, 0, lo == PA_NONE ? 0 : last - j0 + 1}};
 }
 
-// One row over its visible keys lo .. row alone (a whole warp)
+// One row over its visible keys lo .. row alone (a whole warp).  The values' mean is carried, not their sum, which can pass fp32
+// where the mean does not (two values near the type's largest).
 __device__ __noinline__ void pf_redo(const PackedFwdParams& p, int row, int head, int lo) {
   const int hk = head / (p.Hq / p.Hkv), padded = (p.rows + PA_TILE - 1) / PA_TILE * PA_TILE;
   const float4 q = pa_row4(p.q, row, head, p.D);
@@ -226,18 +227,20 @@ __device__ __noinline__ void pf_redo(const PackedFwdParams& p, int row, int head
   for (int j = lo; j <= row; ++j) {
     const float s = pa_dot4(q, pa_row4(p.k, j, hk, p.D)) * p.scale_log2;
     if (pa_nan(s)) { l = s; break; }                                   // and so is the whole row
-    // (a score of -inf weighs zero; what is no number beside it makes the sum none either)
-    const float top = fmaxf(m, s), alpha = m == -INFINITY ? 1.f : pa_exp2(m - top), e = s == -INFINITY ? 0.f : pa_exp2(s - top);
-    l = fmaf(l, alpha, e);
-    o = make_float4(o.x * alpha, o.y * alpha, o.z * alpha, o.w * alpha);
-    pa_add4(o, e, pa_row4(p.v, j, hk, p.D));
+    // (a score of -inf weighs zero; what is no number beside it makes the mean none either)
+    const float top = fmaxf(m, s), old = m == -INFINITY ? 0.f : l * pa_exp2(m - top), e = s == -INFINITY ? 0.f : pa_exp2(s - top);
+    l = old + e;
+    const float keep = l == 0.f ? 1.f : old / l;
+    o = make_float4(o.x * keep, o.y * keep, o.z * keep, o.w * keep);
+    pa_add4(o, l == 0.f ? 0.f : e / l, pa_row4(p.v, j, hk, p.D));
     m = top;
     if (pa_nan(l)) break;
   }
-  const float bad = __int_as_float(0x7fffffff), inv = pa_nan(l) || l == 0.f ? bad : 1.f / l;
+  const float bad = __int_as_float(0x7fffffff);
+  const bool none = pa_nan(l) || l == 0.f;
+  if (none) o = make_float4(bad, bad, bad, bad);
   const size_t at = ((size_t)row * p.Hq + head) * p.D;
   const int c = (threadIdx.x & 31) * 4;
-  o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
   if (p.rest && c < p.D) {
     const bool fin = pa_finite(o.x) && pa_finite(o.y) && pa_finite(o.z) && pa_finite(o.w);
     *reinterpret_cast<uint32_t*>(p.rest + at + c) = fin ? pa_rest(o.x, o.y, o.z, o.w) : 0u;
@@ -246,7 +249,7 @@ __device__ __noinline__ void pf_redo(const PackedFwdParams& p, int row, int head
   } else {
     pa_put4(p.out + at, p.D, o, 1.f);
   }
-  if ((threadIdx.x & 31) == 0) p.lse[(size_t)head * padded + row] = pa_nan(inv) ? bad : m + log2f(l);
+  if ((threadIdx.x & 31) == 0) p.lse[(size_t)head * padded + row] = none ? bad : m + log2f(l);
 }
 
 // A row's running sums come to a maximum that has grown by more than the slack.  All rows of a warp together.

@@ -122,3 +122,20 @@ def test_keys_far_below_the_maximum_weigh_nothing(hq, hkv, d):
     ref, bound = reference(q, k, v, dout)[0]
     off = (out.double() - ref).abs() - EPS * (ref.abs() + bound)
     assert off[33:].max().item() <= 1e-6
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(4, 2, 64), (3, 3, 128)])
+@pytest.mark.parametrize("signs", [False, True])
+def test_values_near_the_largest(signs, hq, hkv, d):
+    """A mean of values near the type's largest is a number, though their sum is none."""
+    q, k, v, dout = make(hq, hkv, d)
+    large = torch.finfo(torch.bfloat16).max
+    v = torch.where(v > 0, large, -large).bfloat16() if signs else torch.full_like(v, -large)
+    docs = ops.pack_documents(torch.tensor([0, ROWS], dtype=torch.int32, device=DEV), ROWS)
+    ref, bound = reference(q, k, v, dout)[0]
+    for x in (q, q.detach().requires_grad_(True)):
+        out = ops.packed_attention(x, k, v, docs).detach()
+        torch.cuda.synchronize()
+        cuda.check_status(out.device)
+        assert out.isfinite().all()
+        assert ((out.double() - ref).abs() <= EPS * (ref.abs() + bound)).all()
