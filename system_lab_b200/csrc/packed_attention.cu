@@ -219,12 +219,13 @@ __device__ __forceinline__ PaItem pf_item(const PackedFwdParams& p, const Packed
 
 // One row over its visible keys lo .. row alone (a whole warp).  The values' mean is carried, not their sum, which can pass fp32
 // where the mean does not (two values near the type's largest).
-__device__ __noinline__ void pf_redo(const PackedFwdParams& p, int row, int head, int lo) {
+__device__ __noinline__ void pf_redo(const PackedFwdParams& p, int row, int head, int lo, volatile int* abort_flag) {
   const int hk = head / (p.Hq / p.Hkv), padded = (p.rows + PA_TILE - 1) / PA_TILE * PA_TILE;
   const float4 q = pa_row4(p.q, row, head, p.D);
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   float m = -INFINITY, l = 0.f;
   for (int j = lo; j <= row; ++j) {
+    pa_redoing(j - lo, abort_flag);
     const float s = pa_dot4(q, pa_row4(p.k, j, hk, p.D)) * p.scale_log2;
     if (pa_nan(s)) { l = s; break; }                                   // and so is the whole row
     // (a score of -inf weighs zero; what is no number beside it makes the mean none either)
@@ -699,7 +700,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         for (uint32_t again = __ballot_sync(0xffffffffu, sees && !(pa_finite(sum) && l > 0.f)); again; again &= again - 1) {
           const int who = __ffs(again) - 1;
           __syncwarp();
-          pf_redo(p, row - lane + who, head, __shfl_sync(0xffffffffu, lo, who));
+          pf_redo(p, row - lane + who, head, __shfl_sync(0xffffffffu, lo, who), abort_flag);
           pa_redone(abort_flag);
         }
       }

@@ -117,8 +117,9 @@ template <int N>
 __device__ __forceinline__ void reg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
 // A bounded wait of a whole warp (mbar_wait_warp) that is patient while rows are made again: a tile of them can take longer
-// than the limit (a key tile of 64 heads x 6000 rows: some 3 s).  Behind the abort flag stands the time at which the last such
-// row was done (pa_redone); the limit counts from there.
+// than the limit (a key tile of 64 heads x 6000 rows: some 3 s), and so can a single row (alone, some 1.1 us a pair: 64 heads x 30
+// thousand rows).  Behind the abort flag stands the time at which such a row was last known to get on (pa_redone: behind every
+// PA_STAMP pairs, a few milliseconds, and behind the row); the limit counts from there.
 __device__ __forceinline__ bool pa_wait_slow(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
 #pragma unroll 1
   for (int i = 0; i < 32; ++i)
@@ -146,6 +147,10 @@ __device__ __forceinline__ bool pa_wait(uint64_t* bar, uint32_t parity, volatile
 }
 __device__ __forceinline__ void pa_redone(volatile int* abort_flag) {
   if ((threadIdx.x & 31) == 0) *reinterpret_cast<volatile uint64_t*>(abort_flag + 1) = globaltimer_ns();
+}
+constexpr int PA_STAMP = 4096;
+__device__ __forceinline__ void pa_redoing(int pair, volatile int* abort_flag) {
+  if ((pair & (PA_STAMP - 1)) == PA_STAMP - 1) pa_redone(abort_flag);
 }
 __device__ __forceinline__ void pa_init_abort(volatile int* abort_flag) {
   abort_flag[0] = abort_flag[1] = abort_flag[2] = 0;

@@ -321,11 +321,12 @@ __device__ __forceinline__ float2 pb_pair(const PackedBwdParams& p, int head, in
   return make_float2(prob, prob * (pa_dot4(dout, v) - p.delta[at]));
 }
 // dq of one row over its visible keys lo .. row alone (a whole warp)
-__device__ __noinline__ void pb_redo_dq(const PackedBwdParams& p, int row, int head, int lo) {
+__device__ __noinline__ void pb_redo_dq(const PackedBwdParams& p, int row, int head, int lo, volatile int* abort_flag) {
   const int hk = head / (p.Hq / p.Hkv);
   const float4 q = pa_row4(p.q, row, head, p.D), dout = pa_row4(p.dout, row, head, p.D);
   float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int j = lo; j <= row; ++j) {
+    pa_redoing(j - lo, abort_flag);
     const float4 k = pa_row4(p.k, j, hk, p.D);
     const float ds = pb_pair(p, head, row, q, k, pa_row4(p.v, j, hk, p.D), dout).y;
     pa_add4(sum, ds, k);
@@ -334,12 +335,15 @@ __device__ __noinline__ void pb_redo_dq(const PackedBwdParams& p, int row, int h
   pa_put4(p.dq + ((size_t)row * p.Hq + head) * p.D, p.D, sum, p.scale);
 }
 // dk or dv of one key row for heads h0 .. h0 + heads - 1 over the queries row .. hi - 1 alone (a whole warp)
-__device__ __noinline__ void pb_redo_dkv(const PackedBwdParams& p, bool dv, int row, int hk, int h0, int heads, int part, int parts, int hi) {
+__device__ __noinline__ void pb_redo_dkv(const PackedBwdParams& p, bool dv, int row, int hk, int h0, int heads, int part, int parts, int hi,
+                                         volatile int* abort_flag) {
   const float4 k = pa_row4(p.k, row, hk, p.D), v = pa_row4(p.v, row, hk, p.D);
   float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
   bool bad = false;
   for (int h = h0; h < h0 + heads && !bad; ++h) {
+    pa_redone(abort_flag);
     for (int i = row; i < hi && !bad; ++i) {
+      pa_redoing(i - row, abort_flag);
       const float4 q = pa_row4(p.q, i, h, p.D), dout = pa_row4(p.dout, i, h, p.D);
       const float2 w = pb_pair(p, h, i, q, k, v, dout);
       pa_add4(sum, dv ? w.x : w.y, dv ? dout : q);
@@ -632,7 +636,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       for (uint32_t m = __ballot_sync(0xffffffffu, sees && !pa_finite(sum)); m; m &= m - 1) {
         const int who = __ffs(m) - 1;
         __syncwarp();
-        pb_redo_dq(p, it.row + lg * 32 + who, it.head, __shfl_sync(0xffffffffu, lo, who));
+        pb_redo_dq(p, it.row + lg * 32 + who, it.head, __shfl_sync(0xffffffffu, lo, who), abort_flag);
         pa_redone(abort_flag);
       }
     }
@@ -970,7 +974,8 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         for (uint32_t m = __ballot_sync(0xffffffffu, any && !pa_finite(bad[which])); m; m &= m - 1) {
           const int who = __ffs(m) - 1;
           __syncwarp();
-          pb_redo_dkv(p, which == 0, it.row + lg * 32 + who, it.hk, it.h0, it.heads, it.part, parts, __shfl_sync(0xffffffffu, hi, who));
+          pb_redo_dkv(p, which == 0, it.row + lg * 32 + who, it.hk, it.h0, it.heads, it.part, parts, __shfl_sync(0xffffffffu, hi, who),
+                      abort_flag);
           pa_redone(abort_flag);
         }
       }

@@ -139,3 +139,27 @@ def test_values_near_the_largest(signs, hq, hkv, d):
         cuda.check_status(out.device)
         assert out.isfinite().all()
         assert ((out.double() - ref).abs() <= EPS * (ref.abs() + bound)).all()
+
+
+def test_one_row_that_takes_longer_than_a_wait_lasts():
+    """dv of the first key is 2^127 in three columns, whose sum passes fp32: the row is made again, four million pairs one by one,
+    some four seconds.  Nothing else is (v is small beside dout's large columns, so dP and delta stay numbers)."""
+    rows, hq, d = 60000, 64, 64
+    g = torch.Generator(device=DEV)
+    g.manual_seed(5)
+    q, k, v, dout = (torch.randn(rows, n, d, device=DEV, generator=g).bfloat16() for n in (hq, 1, 1, hq))
+    v[:, :, :3] *= 2.0 ** -20
+    q[-1, 0] = 8 * k[0, 0]                            # the last query sees the first key: e^60 and more, the others at most e^40
+    dout[-1, 0] = 0.0
+    dout[-1, 0, :3] = 2.0 ** 127
+    docs = ops.pack_documents(torch.tensor([0, rows], dtype=torch.int32, device=DEV), rows)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    grads = torch.autograd.grad(ops.packed_attention(*leaves, docs), leaves, dout)
+    torch.cuda.synchronize()
+    cuda.check_status(q.device)
+    for x in grads:
+        assert x.isfinite().all()
+    # (p is 1 within 2^-9 there, every other term is nothing beside it)
+    assert ((grads[2][0, 0, :3].double() / 2.0 ** 127 - 1).abs() <= 2 * EPS).all()
+    del leaves, grads, q, k, v, dout
+    torch.cuda.empty_cache()
