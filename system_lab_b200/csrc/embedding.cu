@@ -387,6 +387,8 @@ static int em_bwd(const void* tokens, const void* dout, void* dw, int* order, fl
     SLAB_CUDA_CHECK(cudaFuncSetAttribute(embedding_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   embedding_sort_kernel<<<(vocab + slice - 1) / slice, EM_WARPS * 32, smem, st>>>((const long long*)tokens, rows, vocab, slice, order,
                                                                                   valid, named, keep ? 1 : 0);
+  // (the sums take positions from what it has written: without it they must not run)
+  SLAB_CUDA_CHECK(cudaGetLastError());
   EmSum p;
   p.tokens = (const long long*)tokens;
   p.order = order;
