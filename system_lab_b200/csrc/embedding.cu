@@ -383,8 +383,9 @@ static int em_bwd(const void* tokens, const void* dout, void* dw, int* order, fl
   const int bins = (EM_WARPS + 1) * slice * 4;
   const bool keep = rows <= (EM_SORT_SMEM - bins) / 4;
   const int smem = bins + (keep ? rows * 4 : 0);
+  // (the most it ever takes, not this call's: another thread may come between the setting and the launch)
   if (smem > 48 * 1024)
-    SLAB_CUDA_CHECK(cudaFuncSetAttribute(embedding_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    SLAB_CUDA_CHECK(cudaFuncSetAttribute(embedding_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, EM_SORT_SMEM));
   embedding_sort_kernel<<<(vocab + slice - 1) / slice, EM_WARPS * 32, smem, st>>>((const long long*)tokens, rows, vocab, slice, order,
                                                                                   valid, named, keep ? 1 : 0);
   // (the sums take positions from what it has written: without it they must not run)
