@@ -21,6 +21,7 @@ constexpr int EM_WARPS = 32;                 // of a sorting block
 constexpr int EM_BATCH = 8;                  // tokens per lane read together
 constexpr int EM_MAX_SLICE = 1536;           // vocabulary rows per sorting block: 32 histograms of 6 KB
 constexpr int EM_SORT_SMEM = 220 * 1024;     // histograms, and the tokens where they fit beside them
+constexpr int EM_MAX_ROWS = 1 << 30;         // of tokens, and of the table: both are counted in 32 bits, in whole groups and slices
 
 // Vectors of a row as they are in memory (Raw: a quarter of the registers that 32-bit numbers take) and as numbers
 template <typename T, int VEC>
@@ -437,11 +438,12 @@ extern "C" int slab_embedding_fwd(const void* tokens, const void* w, int w_bf16,
 }
 
 // dw [vocab, h] (all of it written, or added to), dout [rows, h]; order: scratch of rows + 1 + ceil(vocab / 32) int32, pieces: scratch of
-// ceil(rows / chunk) * (2 * h + 2) floats, chunk: positions of the sorted list that a group of threads adds up
+// ceil(rows / chunk) * (2 * h + 2) floats, chunk: positions of the sorted list that a group of threads adds up; at most 2^30 tokens and
+// rows of the table
 extern "C" int slab_embedding_bwd(const void* tokens, const void* dout, int out_bf16, void* dw, int w_bf16, void* order, void* pieces,
                                   int rows, int chunk, int vocab, int h, float scale, int accumulate, void* stream) {
   using namespace slab;
-  if (rows <= 0 || h <= 0 || vocab <= 0 || chunk <= 0) return -10;
+  if (rows <= 0 || rows > EM_MAX_ROWS || h <= 0 || vocab <= 0 || vocab > EM_MAX_ROWS || chunk <= 0) return -10;
   const bool vec = h % 8 == 0 && (((size_t)dw | (size_t)dout | (size_t)pieces) & 15) == 0;
   return em_types(w_bf16, out_bf16, vec, [&](auto a, auto b, auto v) {
     return em_bwd<decltype(a), decltype(b), decltype(v)::value>(tokens, dout, dw, (int*)order, (float*)pieces, rows, chunk, vocab, h, scale,

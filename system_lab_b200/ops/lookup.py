@@ -15,6 +15,7 @@ cuda.register("slab_embedding_bwd", "ppipippiiiifis")
 cuda._KERNELS_PER_CALL["slab_embedding_bwd"] = 3
 
 _TYPES = (torch.float32, torch.bfloat16)
+MAX_ROWS = 2 ** 30                                   # of tokens, and of the table: counted in 32 bits, in whole groups and slices
 
 
 def _chunk(rows: int) -> int:
@@ -28,7 +29,7 @@ def check(tokens, weight, scale) -> float:
         raise ValueError(f"a table [vocabulary, hidden] wanted, got {tuple(weight.shape)}")
     if tokens.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"token ids have to be int32 or int64, not {tokens.dtype}")
-    if tokens.numel() > 2 ** 30:                       # (positions are counted in 32 bits, in whole groups)
+    if tokens.numel() > MAX_ROWS:
         raise ValueError(f"{tokens.numel()} tokens: at most 2^30 in one call")
     if tokens.device != weight.device:
         raise ValueError(f"tokens on {tokens.device}, table on {weight.device}")
@@ -36,7 +37,7 @@ def check(tokens, weight, scale) -> float:
 
 
 def supports(weight, dtype) -> bool:
-    return weight.dtype in _TYPES and dtype in _TYPES and weight.shape[0] < 2 ** 31 and weight.shape[1] <= 2 ** 23
+    return weight.dtype in _TYPES and dtype in _TYPES and weight.shape[0] <= MAX_ROWS and weight.shape[1] <= 2 ** 23
 
 
 class _Embedding(torch.autograd.Function):
