@@ -124,6 +124,11 @@ def on_device(t):
     return _HERE if i is None or i == torch.cuda.current_device() else torch.cuda.device(i)
 
 
+def forward_mode() -> bool:
+    """Whether a level of forward-mode differentiation is open, in which tensors may carry tangents."""
+    return torch.autograd.forward_ad._current_level >= 0
+
+
 def first_order(fn):
     """Backward of a Function whose gradients cannot be differentiated again: plain, unless a graph of the backward pass is
     asked for, and then with an error in its place."""

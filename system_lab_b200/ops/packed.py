@@ -206,6 +206,7 @@ class _PackedAttention(torch.autograd.Function):
 
 
 def attention(q, k, v, documents: PackedDocuments, scale: float, window: int = 0):
-    if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)):
+    # (there is no forward mode: tangents go to the Function, which refuses them)
+    if not (cuda.forward_mode() or torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)):
         return forward(q, k, v, documents, scale, window, grads=False)[0]
     return _PackedAttention.apply(q, k, v, documents, scale, window)
