@@ -157,9 +157,10 @@ def causal_attention(q, k, v, scale=None, window=0):
 
 
 def embedding(tokens, weight, scale=1.0, dtype=None):
-    """``scale * weight[tokens]`` in ``dtype`` (the table's own by default), differentiable in ``weight [V, H]``.  On the
-    GPU the gradient is summed in fp32 by sorted tokens, in the order of the positions; ids outside the table look up zeros,
-    get no gradient and set the status word (``BAD_INDEX``)."""
+    """``scale * weight[tokens]`` in ``dtype`` (the table's own by default), differentiable in ``weight [V, H]``.  The kernels take
+    fp32 and bf16; there the gradient is summed in fp32 by sorted tokens, in the order of the positions, and ids outside the
+    table look up zeros, get no gradient and set the status word (``BAD_INDEX``).  Other types, forward mode and ``torch.func``'s
+    transforms run on the oracle, where such ids are an error."""
     scale = lookup.check(tokens, weight, scale)
     dtype = weight.dtype if dtype is None else dtype
     if use_kernels(weight) and lookup.supports(weight, dtype):

@@ -129,6 +129,11 @@ def forward_mode() -> bool:
     return torch.autograd.forward_ad._current_level >= 0
 
 
+def transformed() -> bool:
+    """Whether tensors may be a transform's (``torch.func``) or carry tangents: more than a Function without rules for it takes."""
+    return forward_mode() or torch._C._functorch.peek_interpreter_stack() is not None
+
+
 def first_order(fn):
     """Backward of a Function whose gradients cannot be differentiated again: plain, unless a graph of the backward pass is
     asked for, and then with an error in its place."""

@@ -3,6 +3,9 @@
 The gradient is summed in fp32 in the order of the positions, so it is the same bits every time.  If the table carries
 ``main_grad`` (a view of the flat gradient buffer set by the FSDP engine) it is written there, or added to what an earlier
 micro-batch left there, which touches only the rows the batch names; otherwise autograd gets the whole gradient.
+
+Forward mode and ``torch.func``'s transforms take the oracle; a gradient that is itself differentiated (``create_graph``) or comes
+as a batch (``is_grads_batched``) is made by the library's gradient of a lookup, and always handed to autograd.
 """
 from __future__ import annotations
 
@@ -37,7 +40,14 @@ def check(tokens, weight, scale) -> float:
 
 
 def supports(weight, dtype) -> bool:
-    return weight.dtype in _TYPES and dtype in _TYPES and weight.shape[0] <= MAX_ROWS and weight.shape[1] <= 2 ** 23
+    return not cuda.transformed() and weight.dtype in _TYPES and dtype in _TYPES and weight.shape[0] <= MAX_ROWS and weight.shape[1] <= 2 ** 23
+
+
+def _plain_gradient(tok, g, v: int, scale: float, dtype):
+    """The table's gradient by library operations, which can be differentiated and batched."""
+    inside = (tok >= 0) & (tok < v)
+    g = torch.where(inside[..., None], g.float() * scale, 0.0)
+    return torch.ops.aten.embedding_dense_backward(g, torch.where(inside, tok, 0), v, -1, False).to(dtype)
 
 
 class _Embedding(torch.autograd.Function):
@@ -56,12 +66,13 @@ class _Embedding(torch.autograd.Function):
         return out
 
     @staticmethod
-    @cuda.first_order
     def backward(ctx, g):
         if not ctx.needs_input_grad[1]:
             return None, None, None, None
         (tok,) = ctx.saved_tensors
         v, h, dtype = ctx.table
+        if torch.is_grad_enabled() or not cuda._plain_tensor(g):
+            return None, _plain_gradient(tok, g, v, ctx.scale, dtype), None, None
         rows = tok.numel()
         mg = getattr(ctx.w_ref, "main_grad", None)
         into = mg if mg is not None and mg.dtype in _TYPES and mg.is_contiguous() else None

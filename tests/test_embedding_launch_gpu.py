@@ -58,3 +58,24 @@ def test_threads_with_tables_of_different_sizes():
     for t in threads:
         t.join()
     assert not wrong, wrong
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_transforms_and_gradients_of_gradients(dtype):
+    """The lookup is linear in the table and whole-number weights are exact: everything is equal."""
+    g = torch.Generator(device=DEV)
+    g.manual_seed(2)
+    w, t = (torch.randint(-8, 9, (50, 24), device=DEV, generator=g).to(dtype) for _ in range(2))
+    tok = torch.randint(0, 50, (3, 7), device=DEV, generator=g)
+    dout = torch.randint(-2, 3, (2, 3, 7, 24), device=DEV, generator=g).to(dtype)
+    look = lambda a: ops.embedding(tok, a, scale=2.0)
+    out, tangent = torch.func.jvp(look, (w,), (t,))
+    assert torch.equal(out, look(w)) and torch.equal(tangent, look(t))
+    assert torch.equal(torch.func.vmap(look)(torch.stack([w, t])), torch.stack([look(w), look(t)]))
+    leaf = w.requires_grad_(True)
+    want = torch.stack([torch.autograd.grad(look(leaf), leaf, d)[0] for d in dout])
+    assert torch.equal(torch.autograd.grad(look(leaf), leaf, dout, is_grads_batched=True)[0], want)
+    first = dout[0].clone().requires_grad_(True)
+    (got,) = torch.autograd.grad(look(leaf), leaf, first, create_graph=True)
+    assert torch.equal(got, want[0])
+    assert torch.equal(torch.autograd.grad(got, first, t)[0], look(t))
