@@ -1062,8 +1062,7 @@ extern "C" int slab_packed_attn_bwd(const void* q, const void* k, const void* v,
   if (rows <= 0 || hq <= 0 || hkv <= 0 || hq % hkv || d <= 0 || d > 128 || d % 8 || window < 0 || !(scale > 0.f)) return -10;
   if ((q_ts | q_hs | k_ts | k_hs | v_ts | v_hs | do_ts | do_hs) & 7) return -11;
   if (splits < 1 || splits > hq / hkv || (splits > 1 && !partial)) return -13;
-  static thread_local bool ctx_ready = false;
-  if (!ctx_ready) { cudaFree(0); ctx_ready = true; }
+  tma_need_context();
   CUtensorMap mq, mk, mv, mdo;
   int rc;
   if ((rc = pa_make_map(&mq, q, rows, hq, d, q_ts, q_hs)) != 0) return rc;

@@ -30,6 +30,21 @@ inline TmaEncodeTiledFn tma_encode_fn() {
   return fn;
 }
 
+// The driver's entry point needs a current context; threads that have only been handed tensors (the autograd engine's workers) may not
+// have touched the runtime yet.  (Where there is a context nothing else is called: cudaFree ends a stream capture.)
+inline void tma_need_context() {
+  static thread_local bool ready = false;
+  if (ready) return;
+  typedef CUresult (*GetCurrentFn)(CUcontext*);
+  void* fn = nullptr;
+  cudaDriverEntryPointQueryResult q;
+  CUcontext ctx = nullptr;
+  if (cudaGetDriverEntryPoint("cuCtxGetCurrent", &fn, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess ||
+      reinterpret_cast<GetCurrentFn>(fn)(&ctx) != CUDA_SUCCESS || !ctx)
+    cudaFree(0);
+  ready = true;
+}
+
 struct TmaMapKey {
   const void* base;
   uint64_t rows, cols, row_stride_bytes;
@@ -71,7 +86,6 @@ inline int tma_make_map_2d(CUtensorMap* m, const void* base, CUtensorMapDataType
                            uint64_t cols, uint64_t row_stride_elems, uint32_t box_rows, uint32_t box_cols,
                            int panels = 0) {
   static thread_local TmaMapSlot* cache = nullptr;
-  static thread_local bool ctx_ready = false;
   TmaMapKey key;
   memset(&key, 0, sizeof(key));
   key.base = base;
@@ -90,12 +104,7 @@ inline int tma_make_map_2d(CUtensorMap* m, const void* base, CUtensorMapDataType
   }
   TmaEncodeTiledFn enc = tma_encode_fn();
   if (!enc) return -1;
-  // the driver entry point needs a current context; threads that have only been handed tensors (the
-  // autograd engine's workers) may not have touched the runtime yet
-  if (!ctx_ready) {
-    cudaFree(0);
-    ctx_ready = true;
-  }
+  tma_need_context();
   cuuint64_t dims[3] = {panels > 0 ? box_cols : cols, rows, panels > 0 ? cols / box_cols : (cuuint64_t)-panels};
   cuuint64_t strides[2] = {key.row_stride_bytes, panels > 0 ? (cuuint64_t)box_cols * esize : rows * key.row_stride_bytes};
   cuuint32_t box[3] = {box_cols, box_rows, panels > 0 ? (cuuint32_t)panels : 1};
