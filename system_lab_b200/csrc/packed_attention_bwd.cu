@@ -1018,7 +1018,6 @@ static int packed_bwd_launch(const CUtensorMap& mq, const CUtensorMap& mk, const
                              const PackedBwdParams& p, cudaStream_t stream) {
   const long tiles = (p.rows + PA_TILE - 1) / PA_TILE;
   const long dq_items = tiles * p.Hq, dkv_items = tiles * p.Hkv * p.splits;
-  if (dq_items > 0x3fffffff || dkv_items > 0x3fffffff) return -12;
   SLAB_CUDA_CHECK(cudaFuncSetAttribute(packed_dq_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, PackedDqSmem<DP>::TOTAL));
   SLAB_CUDA_CHECK(cudaFuncSetAttribute(packed_dkv_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, PackedDkvSmem<DP>::TOTAL));
   const int sms = sm_count();
@@ -1071,6 +1070,8 @@ extern "C" int slab_packed_attn_bwd(const void* q, const void* k, const void* v,
   if ((rc = pa_make_map(&mdo, dout, rows, hq, d, do_ts, do_hs)) != 0) return rc;
   cudaStream_t st = (cudaStream_t)stream;
   const int padded = (rows + PA_TILE - 1) / PA_TILE * PA_TILE;
+  const long tiles = padded / PA_TILE;
+  if (tiles * hq > 0x3fffffff || tiles * hkv * splits > 0x3fffffff) return -12;
   const long units = (long)padded / 8 * hq, per = d <= 64 ? 32 : 16;
   if (d <= 64)
     packed_delta_kernel<64><<<(unsigned)((units + per - 1) / per), 256, 0, st>>>((const __nv_bfloat16*)out, (const int8_t*)rest,
@@ -1080,6 +1081,8 @@ extern "C" int slab_packed_attn_bwd(const void* q, const void* k, const void* v,
     packed_delta_kernel<128><<<(unsigned)((units + per - 1) / per), 256, 0, st>>>((const __nv_bfloat16*)out, (const int8_t*)rest,
         (const __nv_bfloat16*)dout, (float*)delta, rows, padded, hq, d, do_ts, do_hs, (int*)counter,
         (const int*)plan, hkv, window, splits, sm_count());
+  // (the kernels behind it take counts from what it has written: without it they must not run)
+  SLAB_CUDA_CHECK(cudaGetLastError());
   PackedBwdParams p;
   p.dq = (__nv_bfloat16*)dq;
   p.dk = (__nv_bfloat16*)dk;
