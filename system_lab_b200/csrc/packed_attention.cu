@@ -738,10 +738,11 @@ static int packed_fwd_launch(const CUtensorMap& mq, const CUtensorMap& mk, const
 
 }  // namespace slab
 
-// int32 words of a plan for `rows` rows
-extern "C" long slab_packed_plan_words(int rows) {
-  const long tiles = ((long)rows + slab::PA_TILE - 1) / slab::PA_TILE;
-  return 2l * rows + 4 * tiles + (tiles + 1) / 2;
+// int32 words of a plan for `rows` rows, 2^25 at most
+extern "C" int slab_packed_plan_words(int rows) {
+  if (rows <= 0 || rows > 1 << 25) return -10;
+  const int* base = reinterpret_cast<const int*>(16);
+  return (int)(slab::packed_plan(base, rows).end - base);
 }
 
 // cu [docs + 1] int32: rows of document s are cu[s] .. cu[s + 1] - 1

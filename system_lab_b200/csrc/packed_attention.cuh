@@ -30,6 +30,7 @@ struct PackedPlan {
   const int* q_order;
   const int* k_order;
   const int* pair_order;
+  const int* end;                            // one past the plan
 };
 inline __host__ __device__ PackedPlan packed_plan(const int* base, int rows) {
   const int tiles = (rows + PA_TILE - 1) / PA_TILE;
@@ -41,6 +42,7 @@ inline __host__ __device__ PackedPlan packed_plan(const int* base, int rows) {
   p.q_order = p.tile_hi + tiles;
   p.k_order = p.q_order + tiles;
   p.pair_order = p.k_order + tiles;
+  p.end = p.pair_order + (tiles + 1) / 2;
   return p;
 }
 

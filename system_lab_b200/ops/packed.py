@@ -18,6 +18,7 @@ import torch
 
 from . import cuda
 
+cuda.register("slab_packed_plan_words", "i")
 cuda.register("slab_packed_plan", "piippp")
 cuda.register("slab_packed_plan_tokens", "piilppp")
 cuda.register("slab_packed_attn_fwd", "ppppppp" + "iiii" + "llllll" + "if" + "ppp")
@@ -48,11 +49,6 @@ class PackedDocuments:
         return self.plan[self.rows:2 * self.rows]
 
 
-def _plan_words(rows: int) -> int:
-    tiles = (rows + TILE - 1) // TILE
-    return 2 * rows + 4 * tiles + (tiles + 1) // 2
-
-
 def pack_documents(cu_seqlens: torch.Tensor, rows: int) -> PackedDocuments:
     """Plan of ``rows`` rows that hold documents ``s`` at ``cu_seqlens[s] .. cu_seqlens[s + 1] - 1`` (starting at 0, not
     falling, documents may be empty; rows behind the last one belong to none).  Offsets on the GPU are checked there:
@@ -75,7 +71,7 @@ def pack_documents(cu_seqlens: torch.Tensor, rows: int) -> PackedDocuments:
     # (offsets past 32 bits have to stay past the buffer's end)
     cu = cu_seqlens.clamp(-1, 2 ** 31 - 1) if cu_seqlens.dtype == torch.int64 else cu_seqlens
     cu = cu.to(torch.int32).contiguous()
-    plan = torch.empty(_plan_words(rows), dtype=torch.int32, device=cu.device)
+    plan = torch.empty(cuda.lib().slab_packed_plan_words(rows), dtype=torch.int32, device=cu.device)
     with cuda.on_device(cu):
         cuda.call("slab_packed_plan", cu, cu.numel() - 1, rows, plan, cuda.status_word(cu.device), cuda.stream())
     return PackedDocuments(rows, plan)
@@ -99,7 +95,7 @@ def documents_from_tokens(tokens: torch.Tensor, end_token: int) -> PackedDocumen
         ends = torch.where(torch.cat([start[1:], torch.ones(1, dtype=torch.bool)]), i + 1, rows)
         hi = ends.flip(0).cummin(0).values.flip(0)
         return PackedDocuments(rows, torch.cat([lo, hi]).int())
-    plan = torch.empty(_plan_words(rows), dtype=torch.int32, device=tok.device)
+    plan = torch.empty(cuda.lib().slab_packed_plan_words(rows), dtype=torch.int32, device=tok.device)
     starts = torch.empty(2 * ((rows + TILE - 1) // TILE), dtype=torch.int32, device=tok.device)
     with cuda.on_device(tok):
         cuda.call("slab_packed_plan_tokens", tok, rows, s, int(end_token), starts, plan, cuda.stream())
