@@ -27,7 +27,7 @@ def check(x, p, seed, offset, residual):
     if not x.is_floating_point():
         raise ValueError(f"dropout of {x.dtype}")
     if not 0.0 <= p < 1.0 or ref.dropout_threshold(p) > 65535:
-        raise ValueError(f"dropout probability {p}: has to be at least 0 and at most 1 - 2^-17")
+        raise ValueError(f"dropout probability {p}: has to be at least 0 and below 1 - 2^-17")
     if isinstance(seed, torch.Tensor):
         if seed.numel() != 1 or seed.dtype != torch.int64 or seed.device != x.device:
             raise ValueError("a seed in a tensor has to be one int64 on x's device")
