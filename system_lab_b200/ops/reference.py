@@ -83,11 +83,10 @@ def _mul_hi_lo(a: int, b: torch.Tensor):
     return mid >> 16, ((mid & 0xFFFF) << 16) | (low & 0xFFFF)
 
 
-def philox_bits(n: int, seed: int, offset: int, device=None) -> torch.Tensor:
-    """16 random bits for each of ``n`` elements (int64): Philox-4x32 with ten rounds (Salmon, Moraes, Dror and Shaw, 2011),
-    key ``seed``, counter ``(element // 8, offset)``, eight halves of words per block, low half first."""
-    block = torch.arange((n + 7) // 8, dtype=torch.int64, device=device)
-    c = [block & 0xFFFFFFFF, block >> 32, torch.full_like(block, offset & 0xFFFFFFFF),
+def philox_words(block: torch.Tensor, seed: int, offset: int) -> list[torch.Tensor]:
+    """Philox-4x32 with ten rounds (Salmon, Moraes, Dror and Shaw, 2011): the four words (int64) of each block of the generator;
+    64-bit counter halves ``block`` (low, as int64) and ``offset`` (high), key ``seed``."""
+    c = [block & 0xFFFFFFFF, (block >> 32) & 0xFFFFFFFF, torch.full_like(block, offset & 0xFFFFFFFF),
          torch.full_like(block, (offset >> 32) & 0xFFFFFFFF)]
     k0, k1 = seed & 0xFFFFFFFF, (seed >> 32) & 0xFFFFFFFF
     for _ in range(10):
@@ -95,7 +94,13 @@ def philox_bits(n: int, seed: int, offset: int, device=None) -> torch.Tensor:
         hi1, lo1 = _mul_hi_lo(0xCD9E8D57, c[2])
         c = [hi1 ^ c[1] ^ k0, lo1, hi0 ^ c[3] ^ k1, lo0]
         k0, k1 = (k0 + 0x9E3779B9) & 0xFFFFFFFF, (k1 + 0xBB67AE85) & 0xFFFFFFFF
-    words = torch.stack(c, dim=-1)
+    return c
+
+
+def philox_bits(n: int, seed: int, offset: int, device=None) -> torch.Tensor:
+    """16 random bits for each of ``n`` elements (int64): key ``seed``, counter ``(element // 8, offset)``, eight halves of words
+    per block, low half first."""
+    words = torch.stack(philox_words(torch.arange((n + 7) // 8, dtype=torch.int64, device=device), seed, offset), dim=-1)
     return torch.stack([words & 0xFFFF, words >> 16], dim=-1).reshape(-1)[:n]
 
 
