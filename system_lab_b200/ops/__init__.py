@@ -170,7 +170,7 @@ def embedding(tokens, weight, scale=1.0, dtype=None):
 
 def dropout(x, p, seed, offset=0, residual=None):
     """``keep / (1 - p) * x (+ residual)`` with a mask that is a function of ``(seed, offset, element)`` and is never stored:
-    the same call gives the same mask, on the CPU too; another seed or offset gives another.  ``p`` is taken to the next
+    the same call gives the same mask, on the CPU too; another seed or offset gives another.  ``p`` is taken to the nearest
     multiple of 2^-16, and kept elements are scaled for that one.  ``seed`` is an integer or an int64 tensor of one element
     (read when the kernel runs)."""
     drop.check(x, p, seed, offset, residual)

@@ -2,11 +2,12 @@
 in one buffer of rows, and a row attends to its own document only (and, with ``window``, to the last ``window`` keys of it).
 
 :func:`pack_documents` (from offsets) or :func:`documents_from_tokens` (from token ids and an end-of-document id) makes
-the plan of a batch once; every layer's forward and backward pass uses it.  Nothing is read back to the host.
+the plan of a batch once; every layer's forward and backward pass uses it.  The kernels' path reads nothing back to the host.
 
 The kernels take bf16 and head widths that are multiples of 8 up to 128, with any token and head strides (slices of a
 packed projection are read where they lie).  Other types and widths, and CPU tensors, take the oracle
-(``reference.packed_attention``), whose scores lie in memory, 512 query rows at a time.
+(``reference.packed_attention``), which reads the plan back and whose scores lie in memory, 512 query rows at a time.  The
+kernels have no forward mode: they refuse tangents.
 
 Reference: the packed fine-tuning batches of ``notes/mlperf-llama/2026-04-29_llama2_70b_lora_baseline_trace_breakdown.md``.
 """
